@@ -14,7 +14,7 @@ from typing import List, Optional, Sequence
 
 MODES = ("sequential", "model", "pipeline", "data")
 SYNC_MODES = ("allreduce", "ps")
-OPTIMIZERS = ("sgd", "lars", "adam")
+OPTIMIZERS = ("sgd", "lars", "adam", "muon")
 
 
 @dataclass
@@ -74,6 +74,8 @@ class Config:
             raise ValueError(f"sync must be one of {SYNC_MODES}")
         if self.optimizer not in OPTIMIZERS:
             raise ValueError(f"optimizer must be one of {OPTIMIZERS}")
+        if self.optimizer == "muon" and self.sync == "ps":
+            raise ValueError("muon needs whole matrices on every rank: use sync='allreduce'")
         if self.pipeline_schedule not in ("1f1b", "gpipe"):
             raise ValueError("pipeline_schedule must be 1f1b or gpipe")
         if self.batch < 1 or self.epochs < 0 or self.run < 1 or self.pipeline < 1 or self.stages < 1:

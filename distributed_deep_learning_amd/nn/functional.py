@@ -12,9 +12,11 @@ from __future__ import annotations
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ..ops import kernels as K
 from ..ops import streams
+from ..ops._lib import device_of
 
 BF16 = torch.bfloat16
 
@@ -886,3 +888,160 @@ class SoftmaxCrossEntropy(torch.autograd.Function):
     def backward(ctx, gloss, _gout):
         (dl,) = ctx.saved_tensors
         return dl * gloss.to(dl.dtype), None
+
+
+class TokenLogProbs(torch.autograd.Function):
+    """Log probabilities of given tokens, entropies and the most likely tokens (``csrc/logprob.hip``): one pass over the logits forward,
+    one backward, whichever of the three outputs carry a gradient.  Use :func:`token_logprobs`."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, top):
+        logp, ent, norm, tv, ti = K.token_logprobs_fwd(logits, tokens, top)
+        ctx.save_for_backward(logits, tokens, norm, ent, ti)
+        ctx.mark_non_differentiable(ti)
+        ctx.set_materialize_grads(False)
+        return logp, ent, tv, ti
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logp, g_ent, g_top, _):
+        logits, tokens, norm, ent, ti = ctx.saved_tensors
+        if g_logp is None and g_ent is None and g_top is None:
+            return None, None, None
+        with device_of(logits):
+            return K.token_logprobs_bwd(logits, tokens, norm, ent, g_logp, g_ent, g_top, ti), None, None
+
+
+def _token_logprobs_cpu(logits, tokens, top):
+    z = logits.float()
+    V = z.shape[-1]
+    empty = (z == float("-inf")).all(-1, keepdim=True)
+    logq = torch.log_softmax(torch.where(empty, 0.0, z), -1)
+    q = logq.exp()
+    ent = -(q * torch.where(q == 0, 0.0, logq)).sum(-1)
+    logq = torch.where(empty, float("-inf"), logq)
+    inside = (tokens >= 0) & (tokens < V)
+    logp = torch.where(inside, logq.gather(-1, tokens.clamp(0, V - 1)[:, None])[:, 0], 0.0)
+    idx = torch.sort(z.detach(), dim=-1, descending=True, stable=True)[1][:, :top]
+    return logp, torch.where(empty[:, 0], 0.0, ent), logq.gather(-1, idx), idx
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
+    """``logits`` bf16 / fp32 ``[..., V]``, ``tokens`` int64 ``[...]`` -> ``(logp, entropy, top_logp, top_index)``: fp32 ``[...]``, ``[...]``,
+    ``[..., top]`` and int64 ``[..., top]``.
+
+    ``logp`` is the log probability of the given token under ``softmax(logits)`` (0, and no gradient, for a token outside ``[0, V)``:
+    padding), ``entropy`` that of the whole distribution in nats, ``top_logp`` / ``top_index`` the ``top`` (at most 64) most likely tokens,
+    descending, equal logits by the lowest index.  All but the indices are differentiable.  Logits of ``-inf`` are masked tokens; a row of
+    nothing else gives ``logp = top_logp = -inf``, entropy 0 and no gradient."""
+    if tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"token_logprobs: tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    if not 0 <= top <= min(V, K.LOGPROB_MAX_TOP):
+        raise ValueError(f"token_logprobs: top must be between 0 and min(V, {K.LOGPROB_MAX_TOP}), got {top} with V = {V}")
+    z, t = logits.reshape(-1, V), tokens.reshape(-1)
+    if logits.is_cuda:
+        with device_of(logits):
+            out = TokenLogProbs.apply(z, t, int(top))
+    else:
+        out = _token_logprobs_cpu(z, t, int(top))
+    logp, ent, tv, ti = out
+    return logp.reshape(lead), ent.reshape(lead), tv.reshape(*lead, top), ti.reshape(*lead, top)
+
+
+def _weight16(w: torch.Tensor) -> torch.Tensor:
+    """bf16 values of a weight: itself, the arena's shadow when that is current, or a fresh copy."""
+    if w.dtype == BF16:
+        return w.detach()
+    if getattr(w, "_ddl_shadow", None) is not None and getattr(w, "_ddl_shadow_version", -1) == w._version:
+        return w._ddl_shadow
+    return w.detach().to(BF16)
+
+
+class GatedMLP(torch.autograd.Function):
+    """The gated feed-forward block on ``csrc/gated.hip``: two launches forward, three backward.  Use :func:`gated_mlp`.  Gradients of fp32
+    weights that live in an arena are added straight into it (on the side stream, like every other weight gradient)."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, activation):
+        D, F_ = x.shape[1], w_gate.shape[0]
+        pd, pf = -D % 8, -F_ % 8                                       # widths that are no multiples of 8: zero columns
+        pad = torch.nn.functional.pad
+        x16 = _bf16(x.detach())
+        wg, wu, wd = (_weight16(w) for w in (w_gate, w_up, w_down))
+        if pd or pf:
+            x16 = pad(x16, (0, pd))
+            wg, wu, wd = pad(wg, (0, pd, 0, pf)), pad(wu, (0, pd, 0, pf)), pad(wd, (0, pf, 0, pd))
+        x16, wg, wu, wd = (K._aligned(t) for t in (x16, wg, wu, wd))
+        train = any(ctx.needs_input_grad[:4])
+        h, g, u = K.gated_up(x16, wg, wu, activation, save=train)
+        y = K.gated_down(h, wd)
+        if train:
+            ctx.save_for_backward(x16, wg, wu, wd, h, g, u)
+            ctx.meta = (D, F_, activation, x.dtype, (w_gate, w_up, w_down))
+        return y[:, :D] if pd else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, wg, wu, wd, h, g, u = ctx.saved_tensors
+        D, F_, activation, x_dtype, weights = ctx.meta
+        need = ctx.needs_input_grad
+        padded = x.shape[1] != D or h.shape[1] != F_
+        with device_of(x):
+            dy = _bf16(dy)
+            if x.shape[1] != D:
+                dy = torch.nn.functional.pad(dy, (0, x.shape[1] - D))
+            dy = K._aligned(dy)
+            dg = du = dx = None
+            if need[0] or need[1] or need[2]:
+                dg, du = K.gated_dh(dy, wd, g, u, activation)
+            if need[0]:
+                dx = K.gated_dx(dg, du, wg, wu)
+                dx = (dx[:, :D] if x.shape[1] != D else dx).to(x_dtype)
+            grads = [None, None, None]
+            want = [w if n else None for w, n in zip(weights, need[1:4])]
+            live = [w for w in want if w is not None]
+            if live:
+                arena = getattr(live[0], "_ddl_arena", None)
+                direct = not padded and arena is not None and all(
+                    getattr(w, "_ddl_arena", None) is arena and arena.grad_is_arena_view(w) and w.grad.is_contiguous() for w in live)
+                if direct:
+                    with streams.fork(x, dy, h, dg, du):
+                        K.gated_dw(x, dy, h, dg, du, [None if w is None else w.grad for w in want], accumulate=True)
+                    for w in reversed(live):
+                        arena.notify_grad_ready(w)
+                else:
+                    fp32 = any(w.dtype == torch.float32 for w in live)
+                    make = torch.zeros_like if fp32 else torch.empty_like
+                    out = [None if w is None else make(w16, dtype=torch.float32 if fp32 else BF16)
+                           for w, w16 in zip(want, (wg, wu, wd))]
+                    K.gated_dw(x, dy, h, dg, du, out, accumulate=fp32)
+                    grads = [None if t is None else t[:w.shape[0], :w.shape[1]].to(w.dtype) for t, w in zip(out, weights)]
+        return dx, *grads, None
+
+
+def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """``(act(x w_gate^T) * (x w_up^T)) w_down^T``: ``x`` ``[..., D]``, ``w_gate`` and ``w_up`` ``[F, D]``, ``w_down`` ``[D, F]``; ``activation``
+    ``"silu"``, ``"gelu"`` (exact) or ``"relu"``.
+
+    On the GPU the products run on bf16 operands (fp32 inputs and weights are rounded; fp32 weights of an arena use its shadow) with
+    fp32 sums, the result is bf16; gradients come in the dtype of what they belong to.  On the CPU: plain torch ops in the inputs' dtype."""
+    if activation not in K.GATED_ACTIVATIONS:
+        raise ValueError(f"gated_mlp: activation must be one of {sorted(K.GATED_ACTIVATIONS)}, got {activation!r}")
+    D = x.shape[-1] if x.dim() else -1
+    if w_gate.dim() != 2 or w_gate.shape != w_up.shape or w_gate.shape[1] != D or tuple(w_down.shape) != (D, w_gate.shape[0]):
+        raise ValueError(f"gated_mlp: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)} and w_down "
+                         f"{tuple(w_down.shape)} do not fit [..., D], [F, D], [F, D], [D, F]")
+    if not x.is_cuda:
+        act = {"silu": torch.nn.functional.silu, "gelu": torch.nn.functional.gelu, "relu": torch.relu}[activation]
+        lin = torch.nn.functional.linear
+        return lin(act(lin(x, w_gate)) * lin(x, w_up), w_down)
+    if any(t.dtype not in (BF16, torch.float32) for t in (x, w_gate, w_up, w_down)):
+        raise TypeError("gated_mlp: inputs and weights must be bf16 or fp32")
+    if any(t.device != x.device for t in (w_gate, w_up, w_down)):
+        raise ValueError("gated_mlp: inputs and weights must be on one device")
+    if D == 0 or w_gate.shape[0] == 0:
+        raise ValueError("gated_mlp: empty widths")
+    with device_of(x):
+        return GatedMLP.apply(x.reshape(-1, D), w_gate, w_up, w_down, activation).reshape(x.shape)

@@ -402,6 +402,23 @@ class Linear(tnn.Linear):
                                  float(dropout) if self.training else 0.0)
 
 
+class GatedMLP(tnn.Module):
+    """Gated feed-forward block without biases: ``down(act(gate(x)) * up(x))`` over ``[..., dim]``.  GPU path:
+    :func:`functional.gated_mlp` - both projections, activation and product in one launch, the down projection in another."""
+
+    def __init__(self, dim: int, hidden: int, activation: str = "silu"):
+        super().__init__()
+        if activation not in K.GATED_ACTIVATIONS:
+            raise ValueError(f"GatedMLP: activation must be one of {sorted(K.GATED_ACTIVATIONS)}, got {activation!r}")
+        self.gate = Linear(dim, hidden, bias=False)
+        self.up = Linear(dim, hidden, bias=False)
+        self.down = Linear(hidden, dim, bias=False)
+        self.activation = activation
+
+    def forward(self, x):
+        return F.gated_mlp(x, self.gate.weight, self.up.weight, self.down.weight, self.activation)
+
+
 class L1Loss(tnn.Module):
     """Mean absolute error (the reference's LSTM criterion); GPU path = one fused forward+gradient launch."""
 
@@ -440,3 +457,16 @@ class SoftmaxCrossEntropyLoss(tnn.Module):
             t = target if target.dim() == 1 else target.argmax(1)
             self.last_correct = (lg.argmax(1) == t).sum().float()
         return loss
+
+
+class TokenLogProbs(tnn.Module):
+    """``(logp, entropy, top_logp, top_index)`` of ``tokens`` under ``softmax(logits)``: see :func:`functional.token_logprobs`."""
+
+    def __init__(self, top: int = 0):
+        super().__init__()
+        if not 0 <= top <= K.LOGPROB_MAX_TOP:
+            raise ValueError(f"TokenLogProbs: top must be between 0 and {K.LOGPROB_MAX_TOP}, got {top}")
+        self.top = int(top)
+
+    def forward(self, logits, tokens):
+        return F.token_logprobs(logits, tokens, self.top)

@@ -101,10 +101,26 @@ _SIGS = {
     "ddl_lstm_fwd": [_vp, _ll, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
     "ddl_lstm_bwd": [_vp, _ll, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp],
     "ddl_rows_gemm_nt": [_vp, _vp, _vp, _i, _i, _i, _vp],
+    "ddl_ns_workspace": [_i, _i, _i],
+    "ddl_ns_max_parts": [],
+    "ddl_ns_mat_bytes": [],
+    "ddl_ns_blocks": [_i, _i, _i, _vp],
+    "ddl_orthogonalize": [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _f, _vp],
+    "ddl_muon_step": [_vp] * 14 + [_i, _i, _vp, _f, _i, _vp],
+    "ddl_gated_up": [_vp] * 6 + [_i, _i, _i, _i, _vp],
+    "ddl_gated_down": [_vp, _vp, _vp, _i, _i, _i, _vp],
+    "ddl_gated_dh": [_vp] * 6 + [_i, _i, _i, _i, _vp],
+    "ddl_gated_dx": [_vp] * 5 + [_i, _i, _i, _vp],
+    "ddl_gated_dw": [_vp] * 8 + [_i, _i, _i, _i, _vp],
+    "ddl_logprob_top_max": [],
+    "ddl_logprob_workspace": [_ll, _i, _i, _i],
+    "ddl_logprob_fwd": [_vp, _i, _vp, _ll, _i, _i] + [_vp] * 7,
+    "ddl_logprob_bwd": [_vp, _i] + [_vp] * 7 + [_ll, _i, _i, _vp, _vp],
 }
 
 
-_LONG_RESULT = {"ddl_conv_wgrad_plan", "ddl_conv_c64_launches", "ddl_wgrad_halo_launches"}
+_LONG_RESULT = {"ddl_conv_wgrad_plan", "ddl_conv_c64_launches", "ddl_wgrad_halo_launches", "ddl_ns_workspace",
+                "ddl_logprob_workspace"}
 
 
 def _load():

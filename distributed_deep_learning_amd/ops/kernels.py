@@ -1164,3 +1164,206 @@ def softmax_xent(logits, target, want_grad=True):
     check(lib.ddl_softmax_xent(ptr(logits), int(logits.dtype == BF16), ptr(labels), ptr(probs), ptr(dl), ptr(out), B, V,
                                stream_ptr()), "softmax_xent")
     return out, dl
+
+
+# ----------------------------------------------------------------------------------------------- token log probabilities
+LOGPROB_MAX_TOP = 64                     # mirrors csrc/logprob.hip
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself when it is contiguous and starts on a 16-byte boundary (a slice of a tensor may not), else a copy."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def token_logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
+    """``logits`` bf16 / fp32 ``[N, V]``, ``tokens`` int64 ``[N]`` -> fp32 ``(logp [N], entropy [N], norm [N, 2],
+    top_logp [N, top])`` and int64 ``top_index [N, top]`` (descending, equal values by the lowest index), one pass over the logits
+    (``csrc/logprob.hip``); ``norm`` is what the backward pass needs: the row's maximum and the log of its sum.  A token outside ``[0, V)`` (padding) gives log probability 0."""
+    lib = _lib.require()
+    if logits.dtype not in (BF16, torch.float32):
+        raise TypeError(f"token_logprobs: logits must be bf16 or fp32, got {logits.dtype}")
+    if logits.dim() != 2 or tokens.dim() != 1 or tokens.shape[0] != logits.shape[0]:
+        raise ValueError(f"token_logprobs: need logits [N, V] and tokens [N], got {tuple(logits.shape)} and {tuple(tokens.shape)}")
+    if tokens.dtype != torch.int64:
+        raise TypeError(f"token_logprobs: tokens must be int64, got {tokens.dtype}")
+    if not logits.is_cuda or tokens.device != logits.device:
+        raise TypeError(f"token_logprobs: logits and tokens must be on one GPU, got {logits.device} and {tokens.device}")
+    _lib.check_device(logits, "token_logprobs")
+    N, V = logits.shape
+    if not 0 <= top <= min(V, LOGPROB_MAX_TOP):
+        raise ValueError(f"token_logprobs: top must be between 0 and min(V, {LOGPROB_MAX_TOP}), got {top} with V = {V}")
+    if V < 1:
+        raise ValueError("token_logprobs: the vocabulary is empty")
+    logits, tokens = logits.contiguous(), tokens.contiguous()
+    dev = logits.device
+    logp, ent = (torch.empty(N, dtype=torch.float32, device=dev) for _ in range(2))
+    norm = torch.empty((N, 2), dtype=torch.float32, device=dev)
+    tv = torch.empty((N, top), dtype=torch.float32, device=dev)
+    ti = torch.empty((N, top), dtype=torch.int64, device=dev)
+    if N > 0:
+        is16 = int(logits.dtype == BF16)
+        ws = torch.empty(lib.ddl_logprob_workspace(N, V, is16, top), dtype=torch.uint8, device=dev)
+        check(lib.ddl_logprob_fwd(ptr(logits), is16, ptr(tokens), N, V, top, ptr(ws), ptr(logp), ptr(ent), ptr(norm), ptr(tv), ptr(ti),
+                                  stream_ptr()), "token_logprobs")
+    return logp, ent, norm, tv, ti
+
+
+def token_logprobs_bwd(logits, tokens, norm, entropy, g_logp=None, g_entropy=None, g_top=None, top_index=None):
+    """Gradient of :func:`token_logprobs_fwd` with respect to the logits (their dtype), one pass: reads them, writes it.  Absent
+    upstream gradients are ``None``."""
+    lib = _lib.require()
+    _lib.check_device(logits, "token_logprobs_bwd")
+    N, V = logits.shape
+    logits, tokens = logits.contiguous(), tokens.contiguous()
+    dz = torch.empty_like(logits)
+    g_logp, g_entropy, g_top = (None if g is None else g.to(torch.float32).contiguous() for g in (g_logp, g_entropy, g_top))
+    k = 0 if g_top is None else g_top.shape[1]
+    if k == 0:
+        g_top = None
+    for g, shape in ((g_logp, (N,)), (g_entropy, (N,)), (g_top, (N, k)), (top_index if k else None, (N, k))):
+        if g is not None and tuple(g.shape) != shape:
+            raise ValueError(f"token_logprobs_bwd: a gradient or index has shape {tuple(g.shape)}, expected {shape}")
+    if N > 0:
+        check(lib.ddl_logprob_bwd(ptr(logits), int(logits.dtype == BF16), ptr(tokens), ptr(norm), ptr(entropy), ptr(g_logp),
+                                  ptr(g_entropy), ptr(g_top), ptr(top_index) if k else None, N, V, k, ptr(dz), stream_ptr()), "token_logprobs_bwd")
+    return dz
+
+
+# ----------------------------------------------------------------------------------------------- gated feed-forward block
+GATED_ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}        # mirrors csrc/gated.hip
+
+
+def _chk_gated(name: str, **mats):
+    """Every argument: ``(tensor, shape)`` - contiguous 16-byte aligned bf16 on the current GPU."""
+    for k, (t, shape) in mats.items():
+        if t is None:
+            continue
+        _chk_act(t, f"{name}: {k}")
+        if tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError(f"{name}: {k} must be a contiguous, 16-byte aligned {tuple(shape)} tensor, got {tuple(t.shape)}")
+
+
+def gated_up(x, w_gate, w_up, activation: str = "silu", save: bool = False):
+    """``h = act(x @ w_gate^T) * (x @ w_up^T)``: ``x`` ``[M, D]``, weights ``[F, D]``, all bf16, ``D`` and ``F`` multiples of 8.
+    Returns ``(h, g, u)``; the projections ``g`` and ``u`` are kept with ``save`` (training), else ``None``."""
+    lib = _lib.require()
+    M, D = x.shape
+    F_ = w_gate.shape[0]
+    if D % 8 or F_ % 8:
+        raise ValueError("gated_up: widths must be multiples of 8")
+    _chk_gated("gated_up", x=(x, (M, D)), w_gate=(w_gate, (F_, D)), w_up=(w_up, (F_, D)))
+    h = torch.empty((M, F_), dtype=BF16, device=x.device)
+    g, u = (torch.empty_like(h), torch.empty_like(h)) if save else (None, None)
+    if M > 0:
+        check(lib.ddl_gated_up(ptr(x), ptr(w_gate), ptr(w_up), ptr(h), ptr(g), ptr(u), M, D, F_, GATED_ACTIVATIONS[activation],
+                               stream_ptr()), "gated_up")
+    return h, g, u
+
+
+def gated_down(h, w_down):
+    """``y = h @ w_down^T``: ``h`` ``[M, F]``, ``w_down`` ``[D, F]``, bf16."""
+    lib = _lib.require()
+    M, F_ = h.shape
+    D = w_down.shape[0]
+    if D % 8 or F_ % 8:
+        raise ValueError("gated_down: widths must be multiples of 8")
+    _chk_gated("gated_down", h=(h, (M, F_)), w_down=(w_down, (D, F_)))
+    y = torch.empty((M, D), dtype=BF16, device=h.device)
+    if M > 0:
+        check(lib.ddl_gated_down(ptr(h), ptr(w_down), ptr(y), M, D, F_, stream_ptr()), "gated_down")
+    return y
+
+
+def gated_dh(dy, w_down, g, u, activation: str = "silu"):
+    """``dh = dy @ w_down`` folded straight into ``(dg, du) = (dh u act'(g), dh act(g))``, bf16 ``[M, F]``."""
+    lib = _lib.require()
+    M, D = dy.shape
+    F_ = w_down.shape[1]
+    _chk_gated("gated_dh", dy=(dy, (M, D)), w_down=(w_down, (D, F_)), g=(g, (M, F_)), u=(u, (M, F_)))
+    dg, du = torch.empty_like(g), torch.empty_like(g)
+    if M > 0:
+        check(lib.ddl_gated_dh(ptr(dy), ptr(w_down), ptr(g), ptr(u), ptr(dg), ptr(du), M, D, F_, GATED_ACTIVATIONS[activation],
+                               stream_ptr()), "gated_dh")
+    return dg, du
+
+
+def gated_dx(dg, du, w_gate, w_up):
+    """``dx = dg @ w_gate + du @ w_up`` (one reduction over both), bf16 ``[M, D]``."""
+    lib = _lib.require()
+    M, F_ = dg.shape
+    D = w_gate.shape[1]
+    _chk_gated("gated_dx", dg=(dg, (M, F_)), du=(du, (M, F_)), w_gate=(w_gate, (F_, D)), w_up=(w_up, (F_, D)))
+    dx = torch.empty((M, D), dtype=BF16, device=dg.device)
+    if M > 0:
+        check(lib.ddl_gated_dx(ptr(dg), ptr(du), ptr(w_gate), ptr(w_up), ptr(dx), M, D, F_, stream_ptr()), "gated_dx")
+    return dx
+
+
+def gated_dw(x, dy, h, dg, du, out, accumulate: bool = False):
+    """Weight gradients ``dg^T x``, ``du^T x`` (``[F, D]``) and ``dy^T h`` (``[D, F]``) in one launch into the three tensors of ``out``
+    (``None``: not wanted): bf16, overwritten, or with ``accumulate`` fp32, added to (arena gradients)."""
+    lib = _lib.require()
+    M, D = x.shape
+    F_ = h.shape[1]
+    _chk_gated("gated_dw", x=(x, (M, D)), dy=(dy, (M, D)), h=(h, (M, F_)), dg=(dg, (M, F_)), du=(du, (M, F_)))
+    want = torch.float32 if accumulate else BF16
+    for t, shape in zip(out, ((F_, D), (F_, D), (D, F_))):
+        if t is not None and (t.dtype != want or tuple(t.shape) != shape or not t.is_contiguous() or t.data_ptr() % 16):
+            raise ValueError(f"gated_dw: outputs must be contiguous, 16-byte aligned {want} tensors {shape}")
+    if M > 0:
+        check(lib.ddl_gated_dw(ptr(x), ptr(dy), ptr(h), ptr(dg), ptr(du), ptr(out[0]), ptr(out[1]), ptr(out[2]), M, D, F_,
+                               int(accumulate), stream_ptr()), "gated_dw")
+    elif not accumulate:
+        for t in out:
+            if t is not None:
+                t.zero_()
+
+
+# ----------------------------------------------------------------------------------------------- orthogonalisation
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)      # steep at zero, singular values end in about [0.7, 1.2]
+NS_STEPS, NS_EPS = 5, 1e-7
+
+
+def check_newton_schulz(steps: int, coefficients) -> tuple:
+    """Refuses polynomials whose iterates leave the range the kernels hold (fp16 at 2^12: a few units): every singular value starts
+    in [0, 1]; ``x`` after every step and the factor ``b s^2 + c s^4`` must stay below 8.  Returns the coefficients as floats."""
+    a, b, c = (float(v) for v in coefficients)
+    if steps < 1:
+        raise ValueError("orthogonalize: at least one step")
+    lim = 1.0
+    for _ in range(steps):
+        pts = [lim * i / 2000.0 for i in range(2001)]
+        top = max(abs(a * s + b * s ** 3 + c * s ** 5) for s in pts)
+        factor = max(abs(b * s ** 2 + c * s ** 4) for s in pts)
+        if not (top < 2.5 and factor < 8.0):
+            raise ValueError(f"orthogonalize: with coefficients {(a, b, c)} singular values in [0, 1] grow to {top:.3g} (factor {factor:.3g})")
+        lim = max(1.02 * top, 0.5)
+    return a, b, c
+
+
+def orthogonalize(g: torch.Tensor, steps: int = NS_STEPS, coefficients=NS_COEFFICIENTS, eps: float = NS_EPS) -> torch.Tensor:
+    """The orthogonal factor of every matrix in ``g`` (``[m, n]`` or ``[batch, m, n]``, bf16 or fp32), approximately: ``steps``
+    Newton-Schulz steps ``X <- a X + (b S + c S S) X``, ``S = X X^T``, from ``X = G / (|G|_F + eps)`` (``csrc/ortho.hip``).  The result has
+    ``g``'s shape and dtype; fp32 matrices are multiplied to fp32's accuracy, bf16 ones with 11-bit operands."""
+    import ctypes as C
+    lib = _lib.require()
+    if g.dim() not in (2, 3):
+        raise ValueError(f"orthogonalize: expected [m, n] or [batch, m, n], got {tuple(g.shape)}")
+    if not g.is_cuda or g.dtype not in (BF16, torch.float32):
+        raise TypeError(f"orthogonalize: expected a bf16 or fp32 GPU tensor, got {g.dtype} on {g.device}")
+    _lib.check_device(g, "orthogonalize")
+    a, b, c = check_newton_schulz(steps, coefficients)
+    if g.numel() == 0:
+        return torch.empty_like(g)
+    g = _aligned(g)
+    batch = g.shape[0] if g.dim() == 3 else 1
+    rows, cols = g.shape[-2:]
+    is16 = g.dtype == BF16
+    prod = 1 if is16 else 3
+    out = torch.empty_like(g)
+    ws = torch.empty(batch * lib.ddl_ns_workspace(rows, cols, prod), dtype=torch.float16, device=g.device)
+    parts = torch.empty(batch * lib.ddl_ns_max_parts(), dtype=torch.float64, device=g.device)
+    check(lib.ddl_orthogonalize(ptr(g), int(is16), ptr(out), ptr(ws), ptr(parts), batch, rows, cols, prod, int(steps),
+                                (C.c_float * 3)(a, b, c), float(eps), stream_ptr()), "orthogonalize")
+    return out

@@ -1,4 +1,5 @@
 from .fused import LARS, FusedAdam, FusedSGD, default_no_decay
 from .lr_scheduler import StepLR, WarmupCosineLR, WarmupPolyLR
+from .muon import Muon
 
-__all__ = ["FusedSGD", "LARS", "FusedAdam", "default_no_decay", "StepLR", "WarmupPolyLR", "WarmupCosineLR"]
+__all__ = ["FusedSGD", "LARS", "FusedAdam", "Muon", "default_no_decay", "StepLR", "WarmupPolyLR", "WarmupCosineLR"]

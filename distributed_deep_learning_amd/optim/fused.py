@@ -135,6 +135,13 @@ class _ArenaOptimizer(torch.optim.Optimizer):
                 return buf[coff + lo - slo:coff + hi - slo]
         raise ValueError(f"optimizer state is sharded and holds nothing for [{lo}, {hi})")
 
+    def state_of(self, p: torch.Tensor, name: str) -> torch.Tensor:
+        """One state buffer of a parameter, as a view with the parameter's shape and strides (unsharded state only)."""
+        if self._shard is not None:
+            raise ValueError("optimizer state is sharded: no rank holds whole tensors")
+        seg = self.arena.segments[p._ddl_segment]                           # noqa: SLF001
+        return torch.as_strided(self.flat_state[name], p.shape, p.stride(), seg.offset)
+
     def state_bytes(self) -> int:
         return sum(v.numel() * v.element_size() for v in self.flat_state.values())
 

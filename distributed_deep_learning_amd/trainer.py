@@ -27,7 +27,7 @@ from .data import synthetic as syn
 from .metrics import (JsonlLogger, PhaseMeter, StepTimer, fmt_test_end, fmt_train_begin, fmt_train_end, fmt_val_end,
                       now_ts)
 from .nn import L1Loss, SoftmaxCrossEntropyLoss
-from .optim import LARS, FusedAdam, FusedSGD, StepLR
+from .optim import LARS, FusedAdam, FusedSGD, Muon, StepLR
 from .parallel import DistributedDataParallel, ParamArena, PipelinedModel, StagedModel
 
 WORKLOADS = {
@@ -164,6 +164,8 @@ class Trainer:
                 o = FusedAdam(a, lr=cfg.lr if cfg.lr != 0.01 else 1e-3, weight_decay=cfg.weight_decay)
             elif opt_kind == "lars":
                 o = LARS(a, lr=cfg.lr, momentum=cfg.momentum, weight_decay=cfg.weight_decay)
+            elif opt_kind == "muon":
+                o = Muon(a, lr=cfg.lr if cfg.lr != 0.01 else 0.02, momentum=cfg.momentum, weight_decay=cfg.weight_decay)
             else:
                 o = FusedSGD(a, lr=cfg.lr, momentum=cfg.momentum, weight_decay=cfg.weight_decay)
             self.optimizers.append(o)

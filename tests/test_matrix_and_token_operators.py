@@ -1,0 +1,630 @@
+"""Orthogonalisation / Muon, the gated feed-forward block and token log probabilities against plain forms in 64 bits.
+
+Tolerances count roundings: half a step is ``eps / 2`` of the type relative to the value (bf16 2^-8, fp16 2^-11, fp32 2^-24)."""
+import math
+
+import pytest
+import torch
+import torch.nn as tnn
+
+from distributed_deep_learning_amd import nn as dnn
+from distributed_deep_learning_amd.config import Config
+from distributed_deep_learning_amd.nn import functional as F
+from distributed_deep_learning_amd.ops import kernels as K
+from distributed_deep_learning_amd.optim import Muon, StepLR
+from distributed_deep_learning_amd.parallel import ParamArena
+
+gpu = pytest.mark.gpu
+B8, H24 = 2.0 ** -8, 2.0 ** -24
+BF = torch.bfloat16
+DT = {"bf16": BF, "fp32": torch.float32}
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _randn(seed, *shape, scale=1.0):
+    return torch.randn(shape, generator=_gen(seed)) * scale
+
+
+# ================================================================================================= orthogonalisation
+def _orth64(g, steps=5, coef=K.NS_COEFFICIENTS, eps=1e-7):
+    a, b, c = coef
+    x = g.double()
+    x = x / (torch.linalg.vector_norm(x, dim=(-2, -1), keepdim=True) + eps)
+    for _ in range(steps):
+        if x.shape[-2] <= x.shape[-1]:
+            s = x @ x.mT
+            x = a * x + (b * s + c * s @ s) @ x
+        else:
+            s = x.mT @ x
+            x = a * x + x @ (b * s + c * s @ s)
+    return x
+
+
+# Relative error of the result's norm.  A step multiplies X by a I + B; rounding the operands of its three products to h relative
+# perturbs that factor by at most 2h in S (twice: S and X X^T's two operands), in S S and in B: below 3 * 2h of a norm that the step keeps
+# near one, five steps: 30 h.  bf16 matrices: h = 2^-11 (fp16 operands) and the rounding of the result; fp32: h = 2^-22 (hi + lo), and sums
+# of up to 5000 products, sqrt(5000) 2^-24 typical, in each of 15 products.
+ORTH_TOL = {"bf16": 30 * 2.0 ** -11 + B8, "fp32": 30 * 2.0 ** -22 + 15 * 71 * H24}
+
+
+def _orth_close(out, g, name, rank=None):
+    """``rank``: of a matrix with empty (or nearly empty) directions.  X is stored with a relative half-step of 2^-22 (hi + lo) before every
+    step; what that leaves in an empty direction grows by a = 3.4445 a step, while |X_j| <= min(a^j, 1.2 sqrt(rank)) from |X_0| = 1:
+    sum_j a^(5-j) |X_j| 2^-22 of the result's norm."""
+    ref = _orth64(g.cpu())
+    err = (out.cpu().double() - ref).norm()
+    a = K.NS_COEFFICIENTS[0]
+    null = 0.0 if rank is None else sum(a ** (5 - j) * min(a ** j, 1.2 * math.sqrt(rank)) for j in range(5)) * 2.0 ** -22
+    assert float(err) <= ORTH_TOL[name] * float(ref.norm()) + null, float(err / ref.norm())
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "fp32"])
+@pytest.mark.parametrize("shape", [(1, 1), (1, 7), (9, 1), (3, 5), (64, 147), (147, 64), (128, 128), (129, 127), (200, 1000), (1000, 136),
+                                   (130, 4100), (3, 65, 70), (2, 300, 129), (5, 32, 32)])
+def test_orthogonalize_matches_64_bits(shape, name):
+    g = (_randn(sum(shape), *shape) * 1e-3).to(DT[name])
+    out = K.orthogonalize(g.cuda())
+    assert out.shape == g.shape and out.dtype == g.dtype
+    for o, x in zip(out.reshape(-1, *shape[-2:]), g.reshape(-1, *shape[-2:])):
+        _orth_close(o, x, name)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "fp32"])
+def test_orthogonalize_of_low_rank_decaying_huge_and_tiny(name):
+    low = _randn(1, 96, 6) @ _randn(2, 6, 200)
+    u, _, v = torch.linalg.svd(_randn(3, 100, 180), full_matrices=False)
+    decay = u @ torch.diag(1.0 / torch.arange(1, 101).float() ** 2) @ v
+    for g, rank in ((low, 6), (decay, 100), (low * 1e30, 6), (low * 1e-6, 6), (low.t().contiguous(), 6)):
+        g = g.to(DT[name])
+        _orth_close(K.orthogonalize(g.cuda()), g, name, rank)
+
+
+@gpu
+def test_orthogonalize_zero_nan_strides_and_empty():
+    g = _randn(4, 4, 40, 70)
+    g[1] = 0.0
+    g[2, 3, 5] = float("nan")
+    out = K.orthogonalize(g.cuda()).cpu()
+    assert torch.equal(out[1], torch.zeros(40, 70)) and torch.isnan(out[2]).all()
+    for i in (0, 3):
+        _orth_close(out[i], g[i], "fp32")
+    big = _randn(5, 81, 203).cuda()
+    view = big[1:, 1:]                                                   # not contiguous; neither base is 16-byte aligned
+    _orth_close(K.orthogonalize(view), view, "fp32")
+    _orth_close(K.orthogonalize(big.t()), big.t(), "fp32")
+    flat = _randn(6, 40 * 72 + 1).cuda()[1:].view(40, 72)                # contiguous, 4-byte aligned
+    _orth_close(K.orthogonalize(flat), flat, "fp32")
+    assert K.orthogonalize(torch.zeros(0, 5, device="cuda")).shape == (0, 5)
+    assert K.orthogonalize(torch.zeros(0, 5, 4, device="cuda")).shape == (0, 5, 4)
+
+
+@gpu
+def test_orthogonalize_captured_replays_and_streams():
+    g = _randn(7, 2, 150, 90).cuda()
+    ref = K.orthogonalize(g)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = K.orthogonalize(g)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(other, ref)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = K.orthogonalize(g)
+    for k in range(3):
+        g.copy_(_randn(70 + k, 2, 150, 90))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, K.orthogonalize(g))                      # fixed order of every sum: bit-equal
+
+
+def test_newton_schulz_refusals():
+    for bad in ((4.0, 1.0, 1.0), (float("nan"), 0.0, 0.0), (20.0, -4.0, 2.0)):
+        with pytest.raises(ValueError):
+            K.check_newton_schulz(5, bad)
+    with pytest.raises(ValueError):
+        K.check_newton_schulz(0, K.NS_COEFFICIENTS)
+    assert K.check_newton_schulz(12, K.NS_COEFFICIENTS) == K.NS_COEFFICIENTS
+    assert K.check_newton_schulz(10, (1.5, -0.5, 0.0)) == (1.5, -0.5, 0.0)
+    if K._lib.available():
+        with pytest.raises(TypeError):
+            K.orthogonalize(torch.zeros(4, 4))                           # not on a GPU
+        with pytest.raises(ValueError):
+            K.orthogonalize(torch.zeros(4))
+
+
+@gpu
+def test_orthogonalize_other_polynomials_and_types():
+    g = _randn(8, 60, 100).cuda()
+    out = K.orthogonalize(g, steps=10, coefficients=(1.5, -0.5, 0.0)).cpu()
+    ref = _orth64(g.cpu(), 10, (1.5, -0.5, 0.0))
+    assert float((out.double() - ref).norm() / ref.norm()) <= 2 * ORTH_TOL["fp32"]
+    with pytest.raises(TypeError):
+        K.orthogonalize(g.half())
+
+
+# ================================================================================================= Muon
+class _Net(tnn.Module):
+    def __init__(self):
+        super().__init__()
+        self.conv = dnn.Conv2d(3, 16, 3)
+        self.tall, self.wide = tnn.Linear(20, 70), tnn.Linear(131, 40, bias=False)
+        self.norm = tnn.LayerNorm(24)
+        self.scalar = tnn.Parameter(torch.tensor(0.5))
+        self.turned = tnn.Parameter(torch.randn(30, 50).t())             # stored transposed
+
+
+def _muon64(state, grads, t, lr, mu, nesterov, wd, adam_lr, betas, eps):
+    b1, b2 = betas
+    for k, (p, m, v) in state.items():
+        g = grads[k].double()
+        if p.dim() >= 2:
+            m.mul_(mu).add_(g)
+            u = (g + mu * m if nesterov else m).reshape(p.shape[0], -1)
+            p.sub_(lr * (max(1.0, u.shape[0] / u.shape[1]) ** 0.5 * _orth64(u).reshape(p.shape) + wd * p))
+        else:
+            m.mul_(b1).add_((1 - b1) * g)
+            v.mul_(b2).add_((1 - b2) * g * g)
+            p.sub_(adam_lr * (m / (1 - b1 ** t)) / ((v / (1 - b2 ** t)).sqrt() + eps))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("nesterov,precision", [(True, "single"), (False, "single"), (True, "half")])
+def test_muon_matches_64_bits(device, nesterov, precision):
+    torch.manual_seed(0)
+    net = _Net().to(device)
+    arena = ParamArena(net.named_parameters())
+    opt = Muon(arena, lr=0.05, momentum=0.9, nesterov=nesterov, weight_decay=0.1, adam_lr=0.01, ns_precision=precision)
+    sched = StepLR(opt, step_size=2, gamma=0.5)
+    state = {n: (p.detach().cpu().double().clone(), torch.zeros(p.shape, dtype=torch.float64), torch.zeros(p.shape, dtype=torch.float64))
+             for n, p in net.named_parameters()}
+    for t in range(1, 4):
+        grads = {n: _randn(100 * t + i, *p.shape) for i, (n, p) in enumerate(net.named_parameters())}
+        for n, p in net.named_parameters():
+            p.grad.copy_(grads[n])
+        lr = opt.lr
+        opt.step()
+        _muon64(state, grads, t, lr, 0.9, nesterov, 0.1, 0.01 * lr / 0.05, (0.9, 0.95), 1e-8)
+        sched.step()
+        assert float(arena.grad.abs().sum()) == 0.0
+        for n, p in net.named_parameters():
+            # update error: the orthogonal factor's, times lr (each of t steps) and the scale; the rest is fp32 arithmetic
+            orth = ORTH_TOL["fp32"] if precision == "single" or device == "cpu" else 30 * 2.0 ** -11
+            rank = min(p.shape[0], p.numel() // max(1, p.shape[0])) if p.dim() >= 2 else 1
+            s = max(1.0, p.shape[0] / (p.numel() / p.shape[0])) ** 0.5 if p.dim() >= 2 else 0.0
+            ref = state[n][0]
+            tol = 1.2 * t * 0.05 * s * orth * math.sqrt(rank) + 64 * H24 * float(ref.norm() + 1)
+            assert float((p.detach().cpu().double() - ref).norm()) <= tol, n
+            assert torch.allclose(opt.state_of(p, "momentum").cpu().double(), state[n][1], rtol=1e-5, atol=1e-6), n
+        if arena.shadow is not None:
+            assert torch.equal(arena.shadow, arena.master.to(BF))
+
+
+def test_muon_refusals_and_state():
+    net = tnn.Sequential(tnn.Linear(8, 16), tnn.Linear(16, 4))
+    arena = ParamArena(net.named_parameters())
+    opt = Muon(arena)
+    with pytest.raises(NotImplementedError):
+        opt.shard_state([(0, 1024)])
+    with pytest.raises(NotImplementedError):
+        opt.step(ranges=[(0, 1024)])
+    with pytest.raises(ValueError):
+        Muon(arena, ns_precision="double")
+    with pytest.raises(ValueError):
+        Muon(arena, ns_coefficients=(9.0, 0.0, 0.0))
+    with pytest.raises(ValueError):
+        Muon(arena, lr=0.0)
+    odd = tnn.Parameter(torch.randn(4, 3, 5).permute(1, 2, 0))
+    with pytest.raises(ValueError):
+        Muon([("odd", odd)])
+    with pytest.raises(ValueError):
+        Config(optimizer="muon", sync="ps").validate()
+    Config(optimizer="muon").validate()
+    opt.flat_state["momentum"].normal_()
+    twin = Muon(ParamArena(tnn.Sequential(tnn.Linear(8, 16), tnn.Linear(16, 4)).named_parameters()))
+    twin.load_state_dict(opt.state_dict())
+    assert torch.equal(twin.flat_state["momentum"], opt.flat_state["momentum"]) and twin.state_of(twin.arena.params[0], "momentum").shape == (16, 8)
+
+
+def test_muon_use_muon_chooses():
+    net = tnn.Sequential(tnn.Linear(8, 16), tnn.Linear(16, 4))
+    opt = Muon(net.named_parameters(), use_muon=lambda n, p: p.dim() == 2 and n.startswith("0"))
+    assert [s.name for s, *_ in opt.matrices] == ["0.weight"]
+
+
+# ================================================================================================= gated feed-forward block
+def _act64(g, act):
+    if act == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s))
+    if act == "gelu":
+        c = 0.5 * (1 + torch.erf(g / math.sqrt(2)))
+        return g * c, c + g * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+    return torch.relu(g), (g > 0).double()
+
+
+def _gated_case(T, D, H, act, seed=0):
+    x, dy = _randn(seed, T, D).to(BF), _randn(seed + 1, T, D, scale=0.1).to(BF)
+    wg, wu = _randn(seed + 2, H, D, scale=D ** -0.5).to(BF), _randn(seed + 3, H, D, scale=D ** -0.5).to(BF)
+    wd = _randn(seed + 4, D, H, scale=H ** -0.5).to(BF)
+    X, DY, G_, U_, W = (t.double() for t in (x, dy, wg, wu, wd))
+    g, u = X @ G_.T, X @ U_.T
+    a, d = _act64(g, act)
+    h = a * u
+    dh = DY @ W
+    dg, du = dh * u * d, dh * a
+    ref = {"y": h @ W.T, "dx": dg @ G_ + du @ U_, "dwg": dg.T @ X, "dwu": du.T @ X, "dwd": DY.T @ h}
+    # roundings on the way: h once; g and u are kept in bf16 for the backward pass (u 2^-8 relative; g moves act' by at most 0.8 |g| 2^-8
+    # and act by at most 1.2 |g| 2^-8), dg and du once; sums of n products n 2^-24 of the magnitudes; the result once
+    ab = torch.abs
+    eh = B8 * ab(h) + 1e-5 * ab(u) * (ab(g) + 1)
+    edg = B8 * (2 * ab(dg) + 0.8 * ab(dh * u * g)) + 1e-6
+    edu = B8 * (ab(du) + 1.2 * ab(dh * g)) + 1e-6
+    n = max(T, D, H) * H24
+    sums = {"y": ab(h) @ ab(W).T, "dx": ab(dg) @ ab(G_) + ab(du) @ ab(U_), "dwg": ab(dg).T @ ab(X), "dwu": ab(du).T @ ab(X), "dwd": ab(DY).T @ ab(h)}
+    err = {"y": eh @ ab(W).T, "dx": edg @ ab(G_) + edu @ ab(U_), "dwg": edg.T @ ab(X), "dwu": edu.T @ ab(X), "dwd": ab(DY).T @ eh}
+    tol = {k: 1.01 * (err[k] + B8 * ab(ref[k]) + n * sums[k]) + 1e-6 for k in ref}
+    return (x, wg, wu, wd, dy), ref, tol
+
+
+def _check(got, ref, tol, what):
+    over = (got.detach().cpu().double() - ref).abs() - tol
+    assert torch.isfinite(got).all() and float(over.max()) <= 0.0, (what, float(over.max()))
+
+
+GATED = [(1, 8, 8, "silu"), (1, 256, 520, "silu"), (3, 72, 136, "gelu"), (17, 64, 200, "relu"), (40, 512, 96, "silu"), (100, 200, 520, "silu"),
+         (129, 136, 264, "gelu"), (257, 328, 128, "silu"), (300, 1000, 1032, "relu"), (64, 100, 77, "silu"), (5, 33, 250, "gelu"), (700, 640, 640, "silu")]
+
+
+@gpu
+@pytest.mark.parametrize("case", GATED)
+def test_gated_mlp_forward_and_gradients(case):
+    T, D, H, act = case
+    (x, wg, wu, wd, dy), ref, tol = _gated_case(T, D, H, act)
+    with torch.no_grad():
+        y0 = F.gated_mlp(*(t.cuda() for t in (x, wg, wu, wd)), activation=act)
+    leaves = [t.cuda().requires_grad_() for t in (x, wg, wu, wd)]
+    y = F.gated_mlp(*leaves, activation=act)
+    assert torch.equal(y0, y) and y.dtype == BF
+    grads = torch.autograd.grad(y, leaves, dy.cuda())
+    for k, t in zip(("y", "dx", "dwg", "dwu", "dwd"), (y, *grads)):
+        assert t.dtype == BF
+        _check(t, ref[k], tol[k], k)
+
+
+@gpu
+def test_gated_mlp_partial_gradients_fp32_and_shapes():
+    (x, wg, wu, wd, dy), ref, tol = _gated_case(24, 64, 136, "silu", seed=9)
+    for needs in ((1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 0, 1), (0, 0, 1, 1)):
+        leaves = [t.cuda().requires_grad_(bool(n)) for t, n in zip((x, wg, wu, wd), needs)]
+        y = F.gated_mlp(*leaves)
+        live = [t for t in leaves if t.requires_grad]
+        grads = iter(torch.autograd.grad(y, live, dy.cuda()))
+        for k, n in zip(("dx", "dwg", "dwu", "dwd"), needs):
+            if n:
+                _check(next(grads), ref[k], tol[k], k)
+    leaves = [t.cuda().float().requires_grad_() for t in (x, wg, wu, wd)]          # fp32 leaves: gradients in fp32
+    y = F.gated_mlp(leaves[0].view(4, 6, 64), *leaves[1:])
+    assert y.shape == (4, 6, 64)
+    grads = torch.autograd.grad(y, leaves, dy.cuda().view(4, 6, 64))
+    for k, t in zip(("dx", "dwg", "dwu", "dwd"), grads):
+        assert t.dtype == torch.float32
+        _check(t, ref[k], tol[k], k)
+    strided = torch.zeros(24, 128, dtype=BF)
+    strided[:, 1:65] = x                                                           # rows not contiguous, not aligned
+    _check(F.gated_mlp(strided.cuda()[:, 1:65], *(t.cuda() for t in (wg, wu, wd))), ref["y"], tol["y"], "strided")
+    wgt = wg.cuda().t().contiguous().t()
+    _check(F.gated_mlp(x.cuda(), wgt, wu.cuda(), wd.cuda()), ref["y"], tol["y"], "transposed weight")
+
+
+@gpu
+def test_gated_mlp_empty_and_rows_do_not_mix():
+    (x, wg, wu, wd, dy), ref, tol = _gated_case(150, 72, 264, "silu", seed=21)
+    leaves = [t.cuda().requires_grad_() for t in (x[:0], wg, wu, wd)]
+    y = F.gated_mlp(*leaves)
+    assert y.shape == (0, 72)
+    for g, t in zip(torch.autograd.grad(y, leaves, y), leaves):
+        assert g.shape == t.shape and float(g.abs().sum()) == 0.0
+    bad = x.clone()
+    bad[7], bad[140] = float("nan"), float("inf")
+    out = F.gated_mlp(*(t.cuda() for t in (bad, wg, wu, wd))).cpu()
+    keep = [i for i in range(150) if i not in (7, 140)]
+    assert torch.isnan(out[7]).all()
+    _check(out[keep], ref["y"][keep], tol["y"][keep], "rows beside a NaN row")
+
+
+def test_gated_mlp_refusals_and_cpu():
+    x, w, wd = torch.randn(3, 16), torch.randn(24, 16), torch.randn(16, 24)
+    with pytest.raises(ValueError):
+        F.gated_mlp(x, w, w, wd, activation="tanh")
+    with pytest.raises(ValueError):
+        F.gated_mlp(x, w, torch.randn(25, 16), wd)
+    with pytest.raises(ValueError):
+        F.gated_mlp(x, w, w, torch.randn(24, 16))
+    with pytest.raises(ValueError):
+        F.gated_mlp(torch.randn(3, 17), w, w, wd)
+    with pytest.raises(ValueError):
+        dnn.GatedMLP(8, 16, activation="tanh")
+    (x, wg, wu, wd, dy), ref, _ = _gated_case(6, 16, 40, "gelu")
+    leaves = [t.double().requires_grad_() for t in (x, wg, wu, wd)]
+    y = F.gated_mlp(*leaves, activation="gelu")
+    for k, t in zip(("y", "dx", "dwg", "dwu", "dwd"), (y, *torch.autograd.grad(y, leaves, dy.double()))):
+        assert torch.allclose(t, ref[k], rtol=1e-10, atol=1e-12), k
+    m = dnn.GatedMLP(16, 40, activation="relu")
+    assert sorted(m.state_dict()) == ["down.weight", "gate.weight", "up.weight"] and m(torch.randn(2, 5, 16)).shape == (2, 5, 16)
+
+
+@gpu
+def test_gated_mlp_module_accumulates_into_the_arena():
+    torch.manual_seed(3)
+    (x, wg, wu, wd, dy), ref, tol = _gated_case(90, 64, 136, "silu", seed=31)
+    m = dnn.GatedMLP(64, 136).cuda()
+    arena = ParamArena(m.named_parameters())
+    with torch.no_grad():
+        for p, w in zip((m.gate.weight, m.up.weight, m.down.weight), (wg, wu, wd)):
+            p.copy_(w)
+    arena.sync_shadow()
+    for n in (1, 2):                                                               # gradients add up over passes
+        xg = x.cuda().requires_grad_()
+        m(xg).backward(dy.cuda())
+        _check(xg.grad, ref["dx"], tol["dx"], "dx")
+        for p, k in zip((m.gate.weight, m.up.weight, m.down.weight), ("dwg", "dwu", "dwd")):
+            assert arena.grad_is_arena_view(p)
+            _check(p.grad, n * ref[k], n * tol[k], k)
+
+
+# ================================================================================================= token log probabilities
+def _logp64(z, tok, top):
+    z = z.double()
+    V = z.shape[1]
+    empty = (z == float("-inf")).all(1)
+    d = z - torch.where(empty, 0.0, z.amax(1))[:, None]                  # first the maximum: far from zero, lse itself loses log s in 64 bits
+    logq = torch.where(empty[:, None], float("-inf"), d - d.exp().sum(1, keepdim=True).log())
+    q = logq.exp()
+    ent = -(torch.where(q > 0, q * logq, 0.0)).sum(1)
+    inside = (tok >= 0) & (tok < V)
+    logp = torch.where(inside, logq.gather(1, tok.clamp(0, V - 1)[:, None])[:, 0], 0.0)
+    idx = torch.sort(z, dim=1, descending=True, stable=True)[1][:, :top]
+    return logp, ent, logq.gather(1, idx), idx, q, logq
+
+
+def _logp_grad64(z, tok, idx, gl, ge, gt):
+    logp, ent, _, _, q, logq = _logp64(z, tok, 0)
+    inside = (tok >= 0) & (tok < z.shape[1])
+    d = torch.zeros_like(q)
+    row = torch.arange(len(tok))
+    if gl is not None:
+        d[row[inside], tok[inside]] += gl.double()[inside]
+    if gt is not None:
+        d.scatter_add_(1, idx, gt.double())
+    dz = d - q * d.sum(1, keepdim=True)
+    if ge is not None:
+        dz = dz - ge.double()[:, None] * torch.where(q > 0, q * (logq + ent[:, None]), 0.0)
+    dz[(z == float("-inf")).all(1)] = 0.0
+    return dz
+
+
+# e^d carries |d| * 1.44 * 2^-24 and a step of the exponential, |d| <= 24 where it matters: 2.2e-6; at most 600 sums in a row: 3.6e-5
+SUM = 4e-5
+
+
+def _check_logp(out, ref):
+    for o, r, scale in zip(out[:3], ref[:3], (1.0, 24.0, 1.0)):
+        o, r = o.detach().cpu().double(), r.detach()
+        fin = torch.isfinite(r)
+        assert torch.equal(torch.isfinite(o), fin) and torch.equal(o[~fin], r[~fin])
+        assert float(((o - r).abs() - (SUM * scale + 4 * H24 * r.abs()))[fin].max().clamp_min(-1) if fin.any() else -1.0) <= 0.0
+    assert torch.equal(out[3].cpu(), ref[3])
+
+
+LOGP = [(1, 1, 1), (1, 7, 7), (3, 33, 5), (2, 255, 64), (5, 1000, 0), (4, 1003, 20), (1, 50257, 20), (2, 8192, 3), (3, 40001, 64), (300, 517, 2),
+        (700, 100, 0), (600, 5000, 8), (2, 70001, 1), (520, 33000, 4)]
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "fp32"])
+@pytest.mark.parametrize("case", LOGP)
+def test_token_logprobs_match_64_bits(case, name):
+    N, V, top = case
+    z = _randn(N + V, N, V, scale=3.0).to(DT[name])
+    tok = torch.randint(0, V, (N,), generator=_gen(V))
+    tok[::5] = torch.tensor([-100, V, 0, V - 1, -1])[torch.arange(len(tok[::5])) % 5]
+    zg = z.cuda().requires_grad_()
+    out = F.token_logprobs(zg, tok.cuda(), top)
+    _check_logp(out, _logp64(z, tok, top))
+    gl, ge, gt = _randn(1, N), _randn(2, N, scale=0.1), _randn(3, N, top)
+    for use in ((1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1)):
+        heads = [(o, g) for o, g, u in zip(out[:3], (gl, ge, gt), use) if u and g.numel()]
+        if not heads:
+            continue
+        (dz,) = torch.autograd.grad([o for o, _ in heads], zg, [g.cuda() for _, g in heads], retain_graph=True)
+        ref = _logp_grad64(z, tok, out[3].cpu(), *(g if u else None for g, u in zip((gl, ge, gt), use)))
+        size = gl.abs() + gt.abs().sum(1) + 24 * ge.abs()
+        # terms of the gradient carry the errors of p (SUM) and of the entropy (24 SUM) times the upstream gradients; one rounding at the end
+        tol = (B8 if name == "bf16" else 8 * H24) * ref.abs() + 4 * SUM * size.double()[:, None] * _logp64(z, tok, 0)[4] + 4 * H24 * size.double()[:, None]
+        assert dz.dtype == z.dtype and float(((dz.cpu().double() - ref).abs() - tol).max()) <= 0.0
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "fp32"])
+def test_token_logprobs_masks_ties_and_extremes(name):
+    dt, inf = DT[name], float("inf")
+    V = 4099
+    z = _randn(11, 10, V, scale=2.0).to(dt)
+    z[0, ::2] = -inf
+    z[1] = -inf                                                          # nothing left
+    z[2] = -inf
+    z[2, 4000] = 3.0                                                     # one token left
+    z[3] = torch.finfo(dt).min                                           # the type's lowest value everywhere: uniform
+    z[4, :] = 1.5                                                        # all equal: indices 0 .. k-1
+    z[5, 10:3000] = 9.0                                                  # a long tie at the top
+    z[6] = z[6] * 1000
+    z[7, 5] = torch.finfo(dt).max
+    z[8, ::3], z[8, 1::3] = 0.0, -0.0                                    # equal zeros of both signs
+    z[8, 2::3] = -1.0
+    tok = torch.tensor([1, 0, 4000, 17, 4098, 5, 3, 5, 0, -100])
+    tok[0] = 0                                                           # a masked token: -inf
+    ref = _logp64(z, tok, 40)
+    zg = z.cuda().requires_grad_()
+    out = F.token_logprobs(zg, tok.cuda(), 40)
+    assert float(out[0][0]) == -inf and float(out[0][1]) == -inf and float(out[1][1]) == 0.0
+    assert torch.equal(out[3][1].cpu(), torch.arange(40)) and torch.equal(out[3][4].cpu(), torch.arange(40))
+    _check_logp(out, ref)
+    gl, ge = torch.ones(10), torch.full((10,), 0.1)
+    gt = _randn(5, 10, 40)
+    (dz,) = torch.autograd.grad(out[:3], zg, [gl.cuda(), ge.cuda(), gt.cuda()])
+    want = _logp_grad64(z, tok, out[3].cpu(), gl, ge, gt)
+    assert torch.isfinite(dz).all() and float(dz[1].abs().sum()) == 0.0
+    tol = 2 * B8 * want.abs() + 2e-3 * ref[4] * (gt.abs().sum(1) + 4).double()[:, None] + 1e-4
+    assert float(((dz.cpu().double() - want).abs() - tol).max()) <= 0.0
+
+
+@gpu
+def test_token_logprobs_nan_and_inf_rows_stay_in_their_rows():
+    z = _randn(12, 4, 3000)
+    z[1, 2999], z[2, 0] = float("nan"), float("inf")
+    tok = torch.tensor([1, 2, 0, 4])
+    zg = z.cuda().requires_grad_()
+    out = F.token_logprobs(zg, tok.cuda(), 3)
+    (dz,) = torch.autograd.grad(out[0].sum() + out[1].sum(), zg)
+    for r in (1, 2):
+        assert torch.isnan(out[0][r]) and torch.isnan(out[1][r]) and torch.isnan(out[2][r]).all() and torch.isnan(dz[r]).all()
+    assert int(out[3][1, 0]) == 2999 and int(out[3][2, 0]) == 0
+    keep = torch.tensor([0, 3])
+    _check_logp([o[keep.cuda()] for o in out], _logp64(z[keep], tok[keep], 3))
+    assert torch.isfinite(dz[keep.cuda()]).all()
+
+
+@gpu
+def test_token_logprobs_shapes_strides_capture():
+    z = _randn(13, 2, 3, 500)
+    tok = torch.randint(0, 500, (2, 3), generator=_gen(13))
+    out = F.token_logprobs(z.cuda(), tok.cuda(), 4)
+    assert [tuple(o.shape) for o in out] == [(2, 3), (2, 3), (2, 3, 4), (2, 3, 4)]
+    wide = torch.zeros(2, 3, 512)
+    wide[..., 3:503] = z
+    again = F.token_logprobs(wide.cuda()[..., 3:503], tok.cuda(), 4)
+    assert all(torch.equal(a, b) for a, b in zip(out, again))
+    flat = torch.cat([torch.zeros(1), z.reshape(-1)]).cuda()[1:].view(6, 500).requires_grad_()      # 4-byte aligned base
+    odd = F.token_logprobs(flat, tok.reshape(-1).cuda(), 4)
+    assert torch.equal(odd[3], out[3].view(6, 4)) and torch.allclose(odd[0], out[0].view(6), atol=SUM)
+    (dz,) = torch.autograd.grad(odd[0].sum(), flat)
+    ref = _logp_grad64(z.reshape(6, 500), tok.reshape(-1), odd[3].cpu(), torch.ones(6), None, None)
+    assert float((dz.cpu().double() - ref).abs().max()) <= 2 * SUM
+    empty = F.token_logprobs(torch.zeros(0, 9, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda"), 2)
+    assert [tuple(o.shape) for o in empty] == [(0,), (0,), (0, 2), (0, 2)]
+    buf, t = z.reshape(6, 500).cuda(), tok.reshape(-1).cuda()
+    F.token_logprobs(buf, t, 5)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cap = F.token_logprobs(buf, t, 5)
+    for k in range(3):
+        buf.copy_(_randn(50 + k, 6, 500))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(cap, F.token_logprobs(buf, t, 5)))
+
+
+def test_token_logprobs_refusals_and_cpu():
+    z, tok = torch.randn(4, 10), torch.tensor([1, -100, 9, 3])
+    for top in (-1, 11):
+        with pytest.raises(ValueError):
+            F.token_logprobs(z, tok, top)
+    with pytest.raises(ValueError):
+        F.token_logprobs(z, tok[:3])
+    with pytest.raises(ValueError):
+        dnn.TokenLogProbs(top=65)
+    if K._lib.available():
+        with pytest.raises(TypeError):
+            K.token_logprobs_fwd(z, tok)                                 # not on a GPU
+        with pytest.raises(TypeError):
+            K.token_logprobs_fwd(z, tok.int())
+        with pytest.raises(TypeError):
+            K.token_logprobs_fwd(z.half(), tok)
+    z[2] = float("-inf")
+    z[3, ::2] = float("-inf")
+    zd = z.clone().requires_grad_()
+    out = dnn.TokenLogProbs(3)(zd, tok)
+    _check_logp(out, _logp64(z, tok, 3))
+    gl, ge = torch.randn(4), torch.randn(4)
+    (dz,) = torch.autograd.grad([out[0], out[1]], zd, [gl, ge])
+    assert torch.allclose(dz.double(), _logp_grad64(z, tok, out[3], gl, ge, None), atol=1e-5)
+
+
+# ================================================================================================= together
+class _Block(tnn.Module):
+    def __init__(self, vocab=301, dim=64, hidden=168):
+        super().__init__()
+        self.inp, self.ff, self.head = dnn.Linear(48, dim), dnn.GatedMLP(dim, hidden), dnn.Linear(dim, vocab)
+
+    def forward(self, x):
+        h = self.inp(x)
+        return self.head(h + self.ff(h))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_block_token_loss_and_muon_step_together(device):
+    torch.manual_seed(5)
+    net = _Block().to(device)
+    opt = Muon(ParamArena(net.named_parameters()), lr=0.02, weight_decay=0.01)
+    x, tok = _randn(40, 88, 48).to(device), torch.randint(0, 301, (88,), generator=_gen(41)).to(device)
+    tok[::9] = -100
+    ref = _Block().double()
+    ref.load_state_dict({k: v.detach().cpu().double() for k, v in net.state_dict().items()})
+    crit = dnn.TokenLogProbs()
+    logp, ent, _, _ = crit(net(x), tok)
+    (-(logp.mean() + 0.01 * ent.mean())).backward()
+    h = ref.inp(x.cpu().double())
+    z = tnn.functional.linear(h + F.gated_mlp(h, ref.ff.gate.weight, ref.ff.up.weight, ref.ff.down.weight), ref.head.weight, ref.head.bias)
+    logq = torch.log_softmax(z, 1)
+    tc = tok.cpu()
+    lp = torch.where(tc >= 0, logq.gather(1, tc.clamp_min(0)[:, None])[:, 0], 0.0)
+    (-(lp.mean() - 0.01 * (logq.exp() * logq).sum(1).mean())).backward()
+    if device == "cuda":
+        torch.cuda.synchronize()
+    for (n, p), (_, q) in zip(net.named_parameters(), ref.named_parameters()):
+        # a chain of about ten bf16 roundings (activations, logits, their gradient, saved projections) on the GPU
+        tol = (10 * B8 if device == "cuda" else 1e-4) * float(q.grad.norm())
+        assert float((p.grad.cpu().double() - q.grad).norm()) <= tol, n
+    before = {n: p.detach().clone() for n, p in net.named_parameters()}
+    opt.step()
+    for n, p in net.named_parameters():
+        assert torch.isfinite(p).all() and not torch.equal(p, before[n]), n
+
+
+@gpu
+def test_muon_in_a_captured_training_step():
+    from distributed_deep_learning_amd.utils.graph import GraphedTrainStep
+    x, y = _randn(60, 32, 48).cuda(), torch.randint(0, 301, (32,), generator=_gen(61)).cuda()
+
+    def make():
+        torch.manual_seed(6)
+        net = _Block().cuda()
+        return net, Muon(ParamArena(net.named_parameters()), lr=0.02)
+
+    net, opt = make()
+    step = GraphedTrainStep(net, dnn.SoftmaxCrossEntropyLoss(), opt, x, y, warmup=1)
+    for _ in range(3):
+        step(x, y)
+    torch.cuda.synchronize()
+    twin, topt = make()
+    crit = dnn.SoftmaxCrossEntropyLoss()
+    for _ in range(4):
+        crit(twin(x), y).backward()
+        topt.step()
+    torch.cuda.synchronize()
+    assert opt.step_count == topt.step_count == 4
+    a, b = opt.arena.master, topt.arena.master
+    assert float((a - b).norm()) <= 1e-3 * float(b.norm())               # split-M sums of the Linear layers may differ in order
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("gpu", marks=gpu)])
+def test_trainer_runs_with_muon(device, tmp_path):
+    from distributed_deep_learning_amd import trainer
+    hist = trainer.run(Config(model="lenet5", optimizer="muon", device=device, epochs=1, batch=16, samples=96, max_steps=3), printer=lambda *a: None)
+    assert math.isfinite(hist[0]["train_loss"])
