@@ -99,8 +99,12 @@ __device__ __forceinline__ void split_store8(unsigned short* hi, long long lo, c
   f16x8 h, l;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    h[e] = (_Float16)v[e];
-    l[e] = (_Float16)(v[e] - (float)h[e]);
+    // The value is pinned in a register first: left to itself the compiler folds the caller's last multiply into the conversion (one
+    // rounding) for the stored hi and not into the one the residual is taken from, and near a tie of fp16 the two differ by a step.
+    float x = v[e];
+    asm("" : "+v"(x));
+    h[e] = (_Float16)x;
+    l[e] = (_Float16)(x - (float)h[e]);
   }
   *reinterpret_cast<f16x8*>(hi) = h;
   *reinterpret_cast<f16x8*>(hi + lo) = l;

@@ -10,6 +10,8 @@ Conventions
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -1328,7 +1330,11 @@ NS_STEPS, NS_EPS = 5, 1e-7
 def check_newton_schulz(steps: int, coefficients) -> tuple:
     """Refuses polynomials whose iterates leave the range the kernels hold (fp16 at 2^12: a few units): every singular value starts
     in [0, 1]; ``x`` after every step and the factor ``b s^2 + c s^4`` must stay below 8.  Returns the coefficients as floats."""
-    a, b, c = (float(v) for v in coefficients)
+    return _newton_schulz_range(int(steps), *(float(v) for v in coefficients))
+
+
+@functools.lru_cache(maxsize=64)
+def _newton_schulz_range(steps: int, a: float, b: float, c: float) -> tuple:
     if steps < 1:
         raise ValueError("orthogonalize: at least one step")
     lim = 1.0

@@ -85,6 +85,17 @@ def test_orthogonalize_of_low_rank_decaying_huge_and_tiny(name):
 
 
 @gpu
+@pytest.mark.parametrize("n", [256, 512])
+def test_orthogonalize_keeps_22_bits_of_every_element(n):
+    """One step of the polynomial X -> X: what comes back is the stored state.  hi + lo is off by half a step of 22 bits, 2^-22 relative, or of
+    fp16's smallest step, 2^-25 at the scale 2^12; the normalisation and the result are three fp32 roundings."""
+    g = _randn(n, n, n)
+    out = K.orthogonalize(g.cuda(), steps=1, coefficients=(1.0, 0.0, 0.0)).cpu().double()
+    x = g.double() / (g.double().norm() + 1e-7)
+    assert float(((out - x).abs() - ((2.0 ** -22 + 3 * H24) * x.abs() + 2.0 ** -37)).max()) <= 0.0
+
+
+@gpu
 def test_orthogonalize_zero_nan_strides_and_empty():
     g = _randn(4, 4, 40, 70)
     g[1] = 0.0
