@@ -7,9 +7,10 @@
 // bound by reading z once.  A row is cut into parts when there are too few rows to fill the chip, and a second launch joins
 // (m, s, q) and the candidate lists of the parts.
 //
-// Top k in the same pass: the part's logits stay in registers (packed as loaded).  The k-th largest of the 256 per-thread maxima is
-// a lower bound of the part's k-th largest value that only a few elements beside the k reach; those are gathered in LDS and ordered by
-// counting.  Rows where very many elements tie with the bound fall back to k rounds of a block-wide maximum.  Candidates are
+// Top k in the same pass: the part's logits stay in registers (packed as loaded).  The threads form k' >= k disjoint groups (k' a power
+// of two); the smallest of the groups' maxima is a bound that at least k elements reach and only about k' ln k' of them, whatever the
+// part's length.  Those are gathered in LDS and ordered by counting.  Where very many elements tie with the bound: k rounds of a
+// block-wide maximum.  Candidates are
 // 64-bit keys, an order-preserving image of the value above the inverted index: equal values go to the lowest index.
 //
 // Masked logits (-inf) have probability zero.  A row without any logit above -inf has logp = top = -inf, entropy 0, gradient 0.  A NaN
@@ -46,6 +47,7 @@ template <> struct Io<float> {
     *reinterpret_cast<f32x4*>(p + 4) = f32x4{f[4], f[5], f[6], f[7]};
   }
   static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+  static __device__ __forceinline__ void pin(Raw& r) { asm volatile("" : "+v"(r.a), "+v"(r.b)); }
 };
 template <> struct Io<bf16_t> {
   static constexpr int ALIGN = 8;
@@ -56,26 +58,29 @@ template <> struct Io<bf16_t> {
   static __device__ __forceinline__ void unpack(const Raw& r, float* f) { unpack8(r, f); }
   static __device__ __forceinline__ void store(bf16_t* p, const float* f) { *reinterpret_cast<u32x4*>(p) = pack8(f); }
   static __device__ __forceinline__ void put(bf16_t* p, float v) { *p = f32_to_bf16(v); }
+  static __device__ __forceinline__ void pin(Raw& r) { asm volatile("" : "+v"(r)); }
 };
 
-// Pieces of 8 elements start on 16-byte boundaries whatever the row's address: piece c holds elements 8c - shift .. 8c - shift + 7.
-template <typename T> __device__ __forceinline__ int shift_of(const T* row) {
-  return (int)(((u64)row / sizeof(T)) & (Io<T>::ALIGN - 1));
+// A row is a run of whole 16-byte aligned pieces of 8 elements, whatever its address, with up to 7 elements in front and behind that belong
+// to part 0: its thread e < 16 holds one of them (e < 8: in front, else behind).
+struct Split { int first, pieces, head, tail; };          // first: element of the first piece;  head, tail: elements in front and behind
+template <typename T> __device__ __forceinline__ Split split_row(const T* row, int V) {
+  const int mis = (int)(((u64)row / sizeof(T)) & (Io<T>::ALIGN - 1));
+  const int first = mis == 0 ? 0 : Io<T>::ALIGN - mis;
+  Split s;
+  s.first = first < V ? first : V;
+  s.pieces = (V - s.first) / 8;
+  s.head = s.first;
+  s.tail = V - s.first - 8 * s.pieces;
+  return s;
 }
-__host__ __device__ inline int pieces_of(int V, int align) { return (V + align - 1 + 7) / 8; }      // for any shift < align
-
-// elements outside the row read as -inf and are marked absent in `valid`
-template <typename T> __device__ __forceinline__ typename Io<T>::Raw load_piece(const T* row, int j0, int V, unsigned& valid) {
-  if (j0 >= 0 && j0 + 8 <= V) { valid = 0xffu; return Io<T>::load(row + j0); }
-  float f[8];
-  valid = 0u;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int j = j0 + e;
-    const bool in = j >= 0 && j < V;
-    f[e] = in ? Io<T>::one(row + j) : -INFINITY;
-    valid |= in ? 1u << e : 0u;
-  }
+__device__ __forceinline__ int edge_element(const Split& s, int tid) {       // -1: none
+  if (tid < s.head) return tid;
+  if (tid >= 8 && tid < 8 + s.tail) return s.first + 8 * s.pieces + tid - 8;
+  return -1;
+}
+template <typename T> __device__ __forceinline__ typename Io<T>::Raw nothing() {
+  const float f[8] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY};
   return Io<T>::pack(f);
 }
 
@@ -87,15 +92,22 @@ __device__ __forceinline__ void stat_rescale(Stat& a, float m) {       // to a m
   a.s = a.s == 0.f ? 0.f : f * a.s;
   a.m = m;
 }
-__device__ __forceinline__ void stat_add8(Stat& a, const float* z) {
-  float mx = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
-  if (mx > a.m) stat_rescale(a, mx);
+__device__ __forceinline__ float max8(const float* z) {                 // ignores NaN
+  return fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
+}
+__device__ __forceinline__ void stat_add8(Stat& a, const float* z) {     // a.m is at least the largest of z
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float d = z[e] - a.m, p = __expf(d);
     a.s += p;                                                            // a NaN (or inf - inf) stays in s
     a.q += p * fmaxf(d, -200.f);                                         // p is zero below about -104: no 0 * inf
   }
+}
+__device__ __forceinline__ void stat_add1(Stat& a, float z) {
+  if (z > a.m) stat_rescale(a, z);
+  const float d = z - a.m, p = __expf(d);
+  a.s += p;
+  a.q += p * fmaxf(d, -200.f);
 }
 __device__ __forceinline__ Stat stat_join(Stat a, Stat b) {
   const float m = fmaxf(a.m, b.m);
@@ -169,26 +181,31 @@ __global__ __launch_bounds__(NT) void logprob_stats_kernel(const T* __restrict__
   const long long r = blockIdx.x / (unsigned)parts;
   const int part = (int)(blockIdx.x - (unsigned)r * (unsigned)parts);
   const T* const row = z + r * V;
-  const int shift = shift_of(row);
-  const int pieces = (V + shift + 7) / 8, c0 = part * per, c1 = min(pieces, c0 + per);
+  const Split sp = split_row(row, V);
+  const T* const body = row + sp.first;
+  const int c0 = part * per, c1 = min(sp.pieces, c0 + per);
   Stat st{-FLT_MAX, 0.f, 0.f};
+  if (part == 0) {
+    const int j = edge_element(sp, threadIdx.x);
+    if (j >= 0) stat_add1(st, Io<T>::one(row + j));
+  }
   int c = c0 + (int)threadIdx.x;
-  for (; c + 3 * NT < c1; c += 4 * NT) {                               // four 16-byte loads in flight
+  for (; c + 3 * NT < c1; c += 4 * NT) {                               // four 16-byte loads in flight, one rescaling for their 32 values
     typename Io<T>::Raw raw[4];
-    unsigned valid;
+    float f[8], mx = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) raw[u] = load_piece(row, (c + u * NT) * 8 - shift, V, valid);
+    for (int u = 0; u < 4; ++u) raw[u] = Io<T>::load(body + (long long)(c + u * NT) * 8);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      float f[8];
-      Io<T>::unpack(raw[u], f);
-      stat_add8(st, f);
-    }
+    for (int u = 0; u < 4; ++u) { Io<T>::unpack(raw[u], f); mx = fmaxf(mx, max8(f)); }
+    if (mx > st.m) stat_rescale(st, mx);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) { Io<T>::unpack(raw[u], f); stat_add8(st, f); }
   }
   for (; c < c1; c += NT) {
-    unsigned valid;
     float f[8];
-    Io<T>::unpack(load_piece(row, c * 8 - shift, V, valid), f);
+    Io<T>::unpack(Io<T>::load(body + (long long)c * 8), f);
+    const float mx = max8(f);
+    if (mx > st.m) stat_rescale(st, mx);
     stat_add8(st, f);
   }
   st = stat_wave(st);
@@ -199,69 +216,86 @@ __global__ __launch_bounds__(NT) void logprob_stats_kernel(const T* __restrict__
   else if (threadIdx.x == 0) pstat[r * parts + part] = st;
 }
 
-// ---- the same with the k largest; at most NCH pieces a thread
+// ---- the same with the k largest; at most NCH pieces a thread, `groups` (a power of two >= k) disjoint sets of threads
 template <typename T, int NCH>
-__global__ __launch_bounds__(NT) void logprob_top_kernel(const T* __restrict__ z, const long long* __restrict__ tokens, int V, int parts,
-                                                         int per, int k, Stat* __restrict__ pstat, u64* __restrict__ ptop, const Outs o) {
+__global__ __launch_bounds__(NT, 4) void logprob_top_kernel(const T* __restrict__ z, const long long* __restrict__ tokens, int V, int parts,
+                                                            int per, int k, int groups, Stat* __restrict__ pstat, u64* __restrict__ ptop,
+                                                            const Outs o) {
   __shared__ Stat red[4];
   __shared__ u64 ured[4];
-  __shared__ u64 tmax[NT];
+  __shared__ float gmax[4][64];
   __shared__ u64 list[CAP];
   __shared__ u64 best[TOP_MAX];
-  __shared__ unsigned bound, count;
+  __shared__ unsigned count;
   const int tid = threadIdx.x;
   const long long r = blockIdx.x / (unsigned)parts;
   const int part = (int)(blockIdx.x - (unsigned)r * (unsigned)parts);
   const T* const row = z + r * V;
-  const int shift = shift_of(row);
-  const int pieces = (V + shift + 7) / 8, c0 = part * per, c1 = min(pieces, c0 + per);
-  Stat st{-FLT_MAX, 0.f, 0.f};
+  const Split sp = split_row(row, V);
+  const T* const body = row + sp.first;
+  const int c0 = part * per, c1 = min(sp.pieces, c0 + per);
+  const int mine = c0 + tid;                                             // this thread's pieces: mine + u * NT
   typename Io<T>::Raw raw[NCH];
-  unsigned valid[NCH];
 #pragma unroll
   for (int u = 0; u < NCH; ++u) {
-    const int c = c0 + tid + u * NT;
-    raw[u] = load_piece(row, c < c1 ? c * 8 - shift : V, V, valid[u]);
+    raw[u] = nothing<T>();
+    if (mine + u * NT < c1) raw[u] = Io<T>::load(body + (long long)(mine + u * NT) * 8);
   }
-  unsigned mk = 0u;                                                      // largest key of this thread
+  const int je = part == 0 ? edge_element(sp, tid) : -1;
+  const float ze = je >= 0 ? Io<T>::one(row + je) : -INFINITY;
+  // (pinned before every pass: else the compiler keeps what one pass unpacked for the next, four times the registers)
+  // the thread's maximum, then sums about it: no rescaling inside the thread
+  Stat st{-FLT_MAX, 0.f, 0.f};
+  float tm = ze;
+  if (tm != tm) tm = -INFINITY;
 #pragma unroll
   for (int u = 0; u < NCH; ++u) {
     float f[8];
+    Io<T>::pin(raw[u]);
     Io<T>::unpack(raw[u], f);
-    if (valid[u] != 0u) stat_add8(st, f);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const unsigned key = (valid[u] >> e) & 1u ? key_of(f[e]) : 0u;
-      mk = key > mk ? key : mk;
-    }
+    tm = fmaxf(tm, max8(f));
   }
+  st.m = fmaxf(tm, -FLT_MAX);
+#pragma unroll
+  for (int u = 0; u < NCH; ++u) {
+    float f[8];
+    Io<T>::pin(raw[u]);
+    Io<T>::unpack(raw[u], f);
+    stat_add8(st, f);
+  }
+  if (je >= 0) stat_add1(st, ze);
+  // a bound that at least k elements reach: the smallest of `groups` maxima over disjoint sets
+  float gm = tm;
+  for (int off = 32; off >= groups; off >>= 1) gm = fmaxf(gm, __shfl_xor(gm, off, 64));
+  gmax[tid >> 6][tid & 63] = gm;
   st = stat_wave(st);
   if ((tid & 63) == 0) red[tid >> 6] = st;
-  tmax[tid] = ((u64)mk << 32) | (u64)(NT - 1 - tid);
   if (tid == 0) count = 0u;
   if (tid < TOP_MAX) best[tid] = 0ull;
   __syncthreads();
   st = stat_join(stat_join(red[0], red[1]), stat_join(red[2], red[3]));
-  {
-    const u64 me = tmax[tid];
-    int rank = 0;
-    for (int i = 0; i < NT; ++i) rank += tmax[i] > me ? 1 : 0;
-    if (rank == k - 1) bound = mk;
-  }
-  __syncthreads();
-  const unsigned lim = bound > 0u ? bound : 1u;
+  float bound = fmaxf(fmaxf(gmax[0][tid & 63], gmax[1][tid & 63]), fmaxf(gmax[2][tid & 63], gmax[3][tid & 63]));
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) bound = fminf(bound, __shfl_xor(bound, off, 64));
+  const bool odd = !(st.s < INFINITY);                                   // a NaN or inf somewhere: no piece may be skipped
 #pragma unroll
   for (int u = 0; u < NCH; ++u) {
     float f[8];
+    Io<T>::pin(raw[u]);
     Io<T>::unpack(raw[u], f);
+    if ((max8(f) >= bound || odd) && mine + u * NT < c1) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const unsigned key = (valid[u] >> e) & 1u ? key_of(f[e]) : 0u;
-      if (key >= lim) {
-        const unsigned at = atomicAdd(&count, 1u);
-        if (at < CAP) list[at] = cand(key, (c0 + tid + u * NT) * 8 - shift + e);
+      for (int e = 0; e < 8; ++e) {
+        if (!(f[e] < bound)) {                                           // a NaN counts as the largest
+          const unsigned at = atomicAdd(&count, 1u);
+          if (at < CAP) list[at] = cand(key_of(f[e]), sp.first + (mine + u * NT) * 8 + e);
+        }
       }
     }
+  }
+  if (je >= 0 && !(ze < bound)) {
+    const unsigned at = atomicAdd(&count, 1u);
+    if (at < CAP) list[at] = cand(key_of(ze), je);
   }
   __syncthreads();
   const unsigned n = count;
@@ -275,17 +309,15 @@ __global__ __launch_bounds__(NT) void logprob_top_kernel(const T* __restrict__ z
   } else {                                                               // many elements tie with the bound
     u64 prev = ~0ull;
     for (int t = 0; t < k; ++t) {
-      u64 mx = 0ull;
-#pragma unroll
-      for (int u = 0; u < NCH; ++u) {
+      u64 mx = je >= 0 ? cand(key_of(ze), je) : 0ull;
+      mx = mx < prev ? mx : 0ull;
+      for (int c = mine; c < c1; c += NT) {                              // read again: rare, and 64-bit keys of registers would spill
         float f[8];
-        Io<T>::unpack(raw[u], f);
+        Io<T>::unpack(Io<T>::load(body + (long long)c * 8), f);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if ((valid[u] >> e) & 1u) {
-            const u64 v = cand(key_of(f[e]), (c0 + tid + u * NT) * 8 - shift + e);
-            mx = v < prev && v > mx ? v : mx;
-          }
+          const u64 v = cand(key_of(f[e]), sp.first + c * 8 + e);
+          mx = v < prev && v > mx ? v : mx;
         }
       }
       prev = block_max(mx, ured);
@@ -339,9 +371,9 @@ __global__ __launch_bounds__(NT) void logprob_bwd_kernel(const T* __restrict__ z
   const int part = (int)(blockIdx.x - (unsigned)r * (unsigned)parts);
   const T* const row = z + r * V;
   T* const drow = dz + r * V;
-  const int shift = shift_of(row);
-  const bool vec = shift_of(drow) == shift;
-  const int pieces = (V + shift + 7) / 8, c0 = part * per, c1 = min(pieces, c0 + per);
+  const Split sp = split_row(row, V);
+  const bool vec = (((u64)(drow + sp.first)) & 15) == 0;
+  const int c0 = part * per, c1 = min(sp.pieces, c0 + per);
   const float mx = norm[2 * r], ls = norm[2 * r + 1], H = ent[r];
   const bool empty = ls == -INFINITY;
   const long long tok = tokens[r];
@@ -354,28 +386,37 @@ __global__ __launch_bounds__(NT) void logprob_bwd_kernel(const T* __restrict__ z
     const float d = (zj - mx) - ls, p = __expf(d);
     return -p * (G + (p == 0.f ? 0.f : gh * (d + H)));
   };
-  for (int c = c0 + (int)threadIdx.x; c < c1; c += NT) {
-    unsigned valid;
+  auto piece = [&](int c, typename Io<T>::Raw raw) {
     float f[8];
-    const int j0 = c * 8 - shift;
-    Io<T>::unpack(load_piece(row, j0, V, valid), f);
+    const int j0 = sp.first + c * 8;
+    Io<T>::unpack(raw, f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = empty ? 0.f : grad(f[e]);
-    if (!empty && (unsigned)(t - j0) < 8u && t >= 0) {
+    if (!empty && t >= j0 && t < j0 + 8) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] += t - j0 == e ? gl : 0.f;
     }
-    if (valid == 0xffu && vec) Io<T>::store(drow + j0, f);
+    if (vec) Io<T>::store(drow + j0, f);
     else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) if ((valid >> e) & 1u) Io<T>::put(drow + j0 + e, f[e]);
+      for (int e = 0; e < 8; ++e) Io<T>::put(drow + j0 + e, f[e]);
     }
+  };
+  const T* const body = row + sp.first;
+  int c = c0 + (int)threadIdx.x;
+  for (; c + NT < c1; c += 2 * NT) {
+    const typename Io<T>::Raw r0 = Io<T>::load(body + (long long)c * 8), r1 = Io<T>::load(body + (long long)(c + NT) * 8);
+    piece(c, r0);
+    piece(c + NT, r1);
   }
+  if (c < c1) piece(c, Io<T>::load(body + (long long)c * 8));
+  const int je = part == 0 ? edge_element(sp, threadIdx.x) : -1;
+  if (je >= 0) Io<T>::put(drow + je, empty ? 0.f : grad(Io<T>::one(row + je)) + (je == t ? gl : 0.f));
   if (gtop == nullptr || empty) return;
   __syncthreads();                                                        // this block's dense values are written: replace the listed ones
   for (int i = threadIdx.x; i < k; i += NT) {
-    const int j = (int)idx[r * k + i], c = (j + shift) / 8;
-    if (c >= c0 && c < c1) {
+    const int j = (int)idx[r * k + i], body_j = j - sp.first, pc = body_j >> 3;
+    if ((body_j >= 0 && pc < sp.pieces) ? (pc >= c0 && pc < c1) : part == 0) {
       float v = grad(Io<T>::one(row + j)) + gtop[r * k + i];
       if (j == t) v += gl;
       Io<T>::put(drow + j, v);
@@ -385,19 +426,28 @@ __global__ __launch_bounds__(NT) void logprob_bwd_kernel(const T* __restrict__ z
 
 // Pieces (of 8 elements) per part.  A block streams a whole row when there are rows enough for two blocks on each of the 256 CUs; fewer
 // rows are cut so that about 512 blocks run, down to one piece a thread.
-int plan(long long rows, int V, int align, int most) {
-  const int pieces = pieces_of(V, align);
+int plan(long long rows, int V, int most) {
+  const int pieces = V / 8;
   long long parts = (512 + rows - 1) / rows;
   if (parts < 1) parts = 1;
   long long per = (pieces + parts - 1) / parts;
   per = (per + NT - 1) / NT * NT;
+  if (per < NT) per = NT;
   if (per > most) per = most;
   return (int)per;
 }
 
+// Rows begin at any alignment: a row has V / 8 pieces at most (fewer behind an unaligned start).
+int parts_of(int V, int per) { const int pieces = V / 8; return pieces == 0 ? 1 : (pieces + per - 1) / per; }
+
+// Most pieces a thread keeps in registers: 64 registers of logits, of the 128 that four waves per SIMD have.
+template <typename T> struct TopPieces { static constexpr int value = sizeof(T) == 2 ? 16 : 8; };
+
 template <typename T, int NCH>
 void launch_top(dim3 grid, hipStream_t st, const T* z, const long long* tokens, int V, int parts, int per, int k, Stat* ps, u64* pt, const Outs& o) {
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_top_kernel<T, NCH>), grid, dim3(NT), 0, st, z, tokens, V, parts, per, k, ps, pt, o);
+  int groups = 1;
+  while (groups < k) groups *= 2;
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_top_kernel<T, NCH>), grid, dim3(NT), 0, st, z, tokens, V, parts, per, k, groups, ps, pt, o);
 }
 
 template <typename T>
@@ -411,19 +461,16 @@ int forward(const T* z, const long long* tokens, long long rows, int V, int k, i
     const int nch = (per + NT - 1) / NT;
     if (nch <= 1) launch_top<T, 1>(grid, st, z, tokens, V, parts, per, k, ps, pt, o);
     else if (nch <= 4) launch_top<T, 4>(grid, st, z, tokens, V, parts, per, k, ps, pt, o);
-    else launch_top<T, 16>(grid, st, z, tokens, V, parts, per, k, ps, pt, o);
+    else launch_top<T, TopPieces<T>::value>(grid, st, z, tokens, V, parts, per, k, ps, pt, o);
   }
   if (parts > 1)
     hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_join_kernel<T>), dim3((unsigned)rows), dim3(NT), 0, st, z, tokens, V, parts, k, ps, pt, o);
   return (int)hipGetLastError();
 }
 
-constexpr int TOP_PIECES = 16 * NT;               // most pieces of a part that keeps its logits in registers
-
 int parts_for(long long rows, int V, int is_bf16, int k, int* per) {
-  const int align = is_bf16 ? 8 : 4;
-  *per = plan(rows, V, align, k > 0 ? TOP_PIECES : 0x7fffff00);
-  return (pieces_of(V, align) + *per - 1) / *per;
+  *per = plan(rows, V, k > 0 ? NT * (is_bf16 ? TopPieces<bf16_t>::value : TopPieces<float>::value) : 0x7fffff00);
+  return parts_of(V, *per);
 }
 
 }  // namespace
@@ -454,8 +501,7 @@ extern "C" int ddl_logprob_fwd(const void* z, int is_bf16, const long long* toke
 extern "C" int ddl_logprob_bwd(const void* z, int is_bf16, const long long* tokens, const float* norm, const float* ent, const float* glogp,
                                const float* gent, const float* gtop, const long long* idx, long long rows, int V, int k, void* dz, void* stream) {
   if (rows <= 0 || V <= 0 || V > 0x7fffff00 || k < 0 || k > TOP_MAX || (gtop != nullptr && idx == nullptr)) return -1;
-  const int align = is_bf16 ? 8 : 4;
-  const int per = plan(rows, V, align, 0x7fffff00), parts = (pieces_of(V, align) + per - 1) / per;
+  const int per = plan(rows, V, 0x7fffff00), parts = parts_of(V, per);
   if (rows * parts > 0x7fffffffll) return -2;
   const dim3 grid((unsigned)(rows * parts));
   hipStream_t st = (hipStream_t)stream;
