@@ -64,27 +64,32 @@ template <int BN> struct PairStager {
     gate = wg + (long long)f0 * ld;
     up = wu + (long long)f0 * ld;
   }
-  __device__ __forceinline__ void issue(unsigned lds, int wid) {
-    const u32x4 rg = gt::make_rsrc(gate, 0xFFFFFFE0ull), ru = gt::make_rsrc(up, 0xFFFFFFE0ull);
-    const unsigned kill = (kdone + 64 > k && kdone + kchunk >= k) ? gt::OOB : 0u;
-#pragma unroll
-    for (int j = 0; j < NP; ++j) gt::dma16(((j / PJ) & 1) ? ru : rg, lds + (unsigned)((j * 4 + wid) * 1024), voff[j] | kill);
-    kdone += 64;
-    gate += 64;
-    up += 64;
+  u32x4 rg, ru;
+  unsigned kill;
+  __device__ __forceinline__ void begin() {
+    rg = gt::make_rsrc(gate, 0xFFFFFFE0ull);
+    ru = gt::make_rsrc(up, 0xFFFFFFE0ull);
+    kill = kdone + kchunk >= k ? gt::OOB : 0u;
   }
+  __device__ __forceinline__ void piece(int j, unsigned lds, int wid) const {
+    gt::dma16(((j / PJ) & 1) ? ru : rg, lds + (unsigned)((j * 4 + wid) * 1024), voff[j] | kill);
+  }
+  __device__ __forceinline__ void end() { kdone += 64; gate += 64; up += 64; }
 };
 
 // Two operands of the same shape one after the other along the reduction.
 template <class S> struct Twice {
+  static constexpr int NP = S::NP;
   S s;
   const unsigned short* second;
-  int left;
-  __device__ __forceinline__ void issue(unsigned lds, int wid) {
+  int left;                                       // stages of the first
+  __device__ __forceinline__ void begin() {
     if (left == 0) { s.base = second; s.kdone = 0; }
     --left;
-    s.issue(lds, wid);
+    s.begin();
   }
+  __device__ __forceinline__ void piece(int j, unsigned lds, int wid) const { s.piece(j, lds, wid); }
+  __device__ __forceinline__ void end() { s.end(); }
 };
 
 struct GatedArgs {
@@ -97,7 +102,7 @@ struct GatedArgs {
 __device__ __forceinline__ void store8(unsigned short* p, const float* v) { *reinterpret_cast<u32x4*>(p) = pack8(v); }
 
 template <int BT, int ACT, bool SAVE>
-__global__ __launch_bounds__(256, 2) void gated_up_kernel(const GatedArgs a) {
+__global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_up_kernel(const GatedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   int ti, tj;
@@ -123,7 +128,7 @@ __global__ __launch_bounds__(256, 2) void gated_up_kernel(const GatedArgs a) {
 }
 
 template <int BT>
-__global__ __launch_bounds__(256, 2) void gated_down_kernel(const GatedArgs a) {
+__global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_down_kernel(const GatedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   int ti, tj;
@@ -142,7 +147,7 @@ __global__ __launch_bounds__(256, 2) void gated_down_kernel(const GatedArgs a) {
 }
 
 template <int BT, int ACT>
-__global__ __launch_bounds__(256, 2) void gated_dh_kernel(const GatedArgs a) {
+__global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_dh_kernel(const GatedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   int ti, tj;
@@ -175,7 +180,7 @@ __global__ __launch_bounds__(256, 2) void gated_dh_kernel(const GatedArgs a) {
 }
 
 template <int BT>
-__global__ __launch_bounds__(256, 2) void gated_dx_kernel(const GatedArgs a) {
+__global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_dx_kernel(const GatedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   int ti, tj;
@@ -198,7 +203,7 @@ __global__ __launch_bounds__(256, 2) void gated_dx_kernel(const GatedArgs a) {
 }
 
 template <int BT>
-__global__ __launch_bounds__(256, 2) void gated_dw_kernel(const GatedArgs a) {
+__global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_dw_kernel(const GatedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int tf = (a.F + BT - 1) / BT, td = (a.D + BT - 1) / BT, per = tf * td, which = (int)blockIdx.x / per;
@@ -233,28 +238,34 @@ __global__ __launch_bounds__(256, 2) void gated_dw_kernel(const GatedArgs a) {
   }, [](int, int, float*) {});
 }
 
-constexpr int BT = 128;
-constexpr int SMEM = gt::Tile<BT, BT>::SMEM;
-
 inline long long tiles(int n, int t) { return ((long long)n + t - 1) / t; }
 
 // one launch of a kernel that takes GatedArgs; opts in to its LDS once per device
-template <auto KERNEL> int launch(long long blocks, const GatedArgs& a, void* stream) {
+template <int BT, auto KERNEL> int launch(long long blocks, const GatedArgs& a, void* stream) {
   static SmemAttrOnce once;
   if (blocks <= 0 || blocks > 0x7fffffffll) return -2;
-  const int rc = once.ensure(reinterpret_cast<const void*>(KERNEL), SMEM);
+  constexpr int smem = gt::Tile<BT, BT>::SMEM;
+  const int rc = once.ensure(reinterpret_cast<const void*>(KERNEL), smem);
   if (rc != 0) return rc;
-  hipLaunchKernelGGL(KERNEL, dim3((unsigned)blocks), dim3(256), SMEM, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(KERNEL, dim3((unsigned)blocks), dim3(256), smem, (hipStream_t)stream, a);
   return (int)hipGetLastError();
 }
 
-template <int ACT> int launch_up(const GatedArgs& a, bool save, void* st) {
+template <int BT, int ACT> int launch_up(const GatedArgs& a, bool save, void* st) {
   const long long nb = tiles(a.M, BT) * tiles(a.F, BT / 2);
-  return save ? launch<&gated_up_kernel<BT, ACT, true>>(nb, a, st) : launch<&gated_up_kernel<BT, ACT, false>>(nb, a, st);
+  return save ? launch<BT, &gated_up_kernel<BT, ACT, true>>(nb, a, st) : launch<BT, &gated_up_kernel<BT, ACT, false>>(nb, a, st);
 }
-template <int ACT> int launch_dh(const GatedArgs& a, void* st) {
-  return launch<&gated_dh_kernel<BT, ACT>>(tiles(a.M, BT) * tiles(a.F, BT), a, st);
+template <int BT> int up_act(const GatedArgs& a, int act, bool save, void* st) {
+  return act == SILU ? launch_up<BT, SILU>(a, save, st) : act == GELU ? launch_up<BT, GELU>(a, save, st) : launch_up<BT, RELU>(a, save, st);
 }
+template <int BT> int dh_act(const GatedArgs& a, int act, void* st) {
+  const long long nb = tiles(a.M, BT) * tiles(a.F, BT);
+  return act == SILU ? launch<BT, &gated_dh_kernel<BT, SILU>>(nb, a, st)
+       : act == GELU ? launch<BT, &gated_dh_kernel<BT, GELU>>(nb, a, st) : launch<BT, &gated_dh_kernel<BT, RELU>>(nb, a, st);
+}
+
+// 256 x 256 tiles where they fill the chip
+bool large(int m, int n) { return tiles(m, 256) * tiles(n, 256) >= 256; }
 
 bool sizes_ok(int M, int D, int F) { return M > 0 && D > 0 && F > 0 && D % 8 == 0 && F % 8 == 0; }
 
@@ -267,10 +278,8 @@ extern "C" int ddl_gated_up(const void* x, const void* wg, const void* wu, void*
   a.x = (const unsigned short*)x; a.wg = (const unsigned short*)wg; a.wu = (const unsigned short*)wu;
   a.h = (unsigned short*)h; a.g = (unsigned short*)g; a.u = (unsigned short*)u;
   a.M = M; a.D = D; a.F = F;
-  if (act == SILU) return launch_up<SILU>(a, g != nullptr, stream);
-  if (act == GELU) return launch_up<GELU>(a, g != nullptr, stream);
-  if (act == RELU) return launch_up<RELU>(a, g != nullptr, stream);
-  return -1;
+  if (act < SILU || act > RELU) return -1;
+  return large(M, 2 * F) ? up_act<256>(a, act, g != nullptr, stream) : up_act<128>(a, act, g != nullptr, stream);
 }
 
 extern "C" int ddl_gated_down(const void* h, const void* wd, void* y, int M, int D, int F, void* stream) {
@@ -278,7 +287,8 @@ extern "C" int ddl_gated_down(const void* h, const void* wd, void* y, int M, int
   GatedArgs a{};
   a.h = (unsigned short*)h; a.wd = (const unsigned short*)wd; a.y = (unsigned short*)y;
   a.M = M; a.D = D; a.F = F;
-  return launch<&gated_down_kernel<BT>>(tiles(M, BT) * tiles(D, BT), a, stream);
+  return large(M, D) ? launch<256, &gated_down_kernel<256>>(tiles(M, 256) * tiles(D, 256), a, stream)
+                     : launch<128, &gated_down_kernel<128>>(tiles(M, 128) * tiles(D, 128), a, stream);
 }
 
 extern "C" int ddl_gated_dh(const void* dy, const void* wd, const void* g, const void* u, void* dg, void* du, int M, int D, int F, int act,
@@ -288,10 +298,8 @@ extern "C" int ddl_gated_dh(const void* dy, const void* wd, const void* g, const
   a.dy = (const unsigned short*)dy; a.wd = (const unsigned short*)wd;
   a.g = (unsigned short*)g; a.u = (unsigned short*)u; a.dg = (unsigned short*)dg; a.du = (unsigned short*)du;
   a.M = M; a.D = D; a.F = F;
-  if (act == SILU) return launch_dh<SILU>(a, stream);
-  if (act == GELU) return launch_dh<GELU>(a, stream);
-  if (act == RELU) return launch_dh<RELU>(a, stream);
-  return -1;
+  if (act < SILU || act > RELU) return -1;
+  return large(M, F) ? dh_act<256>(a, act, stream) : dh_act<128>(a, act, stream);
 }
 
 extern "C" int ddl_gated_dx(const void* dg, const void* du, const void* wg, const void* wu, void* dx, int M, int D, int F, void* stream) {
@@ -300,7 +308,8 @@ extern "C" int ddl_gated_dx(const void* dg, const void* du, const void* wg, cons
   a.dg = (unsigned short*)dg; a.du = (unsigned short*)du; a.wg = (const unsigned short*)wg; a.wu = (const unsigned short*)wu;
   a.dx = (unsigned short*)dx;
   a.M = M; a.D = D; a.F = F;
-  return launch<&gated_dx_kernel<BT>>(tiles(M, BT) * tiles(D, BT), a, stream);
+  return large(M, D) ? launch<256, &gated_dx_kernel<256>>(tiles(M, 256) * tiles(D, 256), a, stream)
+                     : launch<128, &gated_dx_kernel<128>>(tiles(M, 128) * tiles(D, 128), a, stream);
 }
 
 // weight gradients: bf16, written (accumulate 0), or fp32, added to (accumulate 1); a null one is left out
@@ -312,5 +321,6 @@ extern "C" int ddl_gated_dw(const void* x, const void* dy, const void* h, const 
   a.dg = (unsigned short*)dg; a.du = (unsigned short*)du;
   a.dwg = dwg; a.dwu = dwu; a.dwd = dwd;
   a.M = M; a.D = D; a.F = F; a.accumulate = accumulate;
-  return launch<&gated_dw_kernel<BT>>(3 * tiles(F, BT) * tiles(D, BT), a, stream);
+  return large(3 * F, D) ? launch<256, &gated_dw_kernel<256>>(3 * tiles(F, 256) * tiles(D, 256), a, stream)
+                         : launch<128, &gated_dw_kernel<128>>(3 * tiles(F, 128) * tiles(D, 128), a, stream);
 }

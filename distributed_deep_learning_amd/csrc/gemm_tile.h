@@ -31,16 +31,28 @@ namespace gt {
 
 constexpr unsigned OOB = 0xFFFFFFF0u;      // beyond any descriptor: the lane reads zero
 
+// Tied forms (dst == src C, AGPR file) for the large tile, whose loop fills the register file: through the builtin the compiler gives the
+// unrolled products rotating destinations and moves half of the 256 accumulators back at every stage.  The waits for the fragments stay the
+// compiler's (it sees the operands); nothing else touches the accumulators between settle() before and after the loop.
 struct Bf16 {
+  static __device__ __forceinline__ void mfma_tied(const s16x8& a, const s16x8& b, f32x4& c) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  }
   static __device__ __forceinline__ f32x4 mfma(const s16x8 a, const s16x8 b, const f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
 };
 struct Fp16 {
+  static __device__ __forceinline__ void mfma_tied(const s16x8& a, const s16x8& b, f32x4& c) {
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  }
   static __device__ __forceinline__ f32x4 mfma(const s16x8 a, const s16x8 b, const f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
 };
+
+// wait states between a matrix instruction the compiler does not see and other accesses of its registers
+__device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
 __device__ __forceinline__ u32x4 make_rsrc(const void* base, unsigned long long bytes) {
   const unsigned long long a = (unsigned long long)base;
@@ -110,23 +122,34 @@ struct Stager {
   }
   static constexpr int KSTEP = PROD == 3 ? 32 : 64;
 
-  __device__ __forceinline__ void issue(unsigned lds, int wid) {
+  // Staging of one stage: begin, every piece, end.  Stages behind the end of the reduction come out as zeros.
+  u32x4 rsrc;
+  unsigned kill;
+  __device__ __forceinline__ void begin() {
     // bytes the descriptor may reach: K-slow tiles end behind the last reduction step; K-contiguous ones check per chunk
-    u32x4 rsrc;
     if (MODE == SLOW) {
       const int left = k - kdone;
       rsrc = make_rsrc(base, left > 0 ? (unsigned long long)left * (unsigned long long)ld * 2ull : 0ull);
     } else {
       rsrc = make_rsrc(base, 0xFFFFFFE0ull);
     }
-    unsigned kill = 0u;
-    if (MODE == CONTIG && kdone + KSTEP > k) kill = (kdone + kchunk >= k) ? OOB : 0u;
-#pragma unroll
-    for (int j = 0; j < NP; ++j) dma16(rsrc, lds + (unsigned)((j * 4 + wid) * 1024), voff[j] | kill);
+    kill = MODE == CONTIG && kdone + kchunk >= k ? OOB : 0u;
+  }
+  __device__ __forceinline__ void piece(int j, unsigned lds, int wid) const {
+    dma16(rsrc, lds + (unsigned)((j * 4 + wid) * 1024), voff[j] | kill);
+  }
+  __device__ __forceinline__ void end() {
     kdone += KSTEP;
     base += MODE == SLOW ? (long long)KSTEP * ld : 64;
   }
 };
+
+template <class S> __device__ __forceinline__ void issue(S& s, unsigned lds, int wid) {
+  s.begin();
+#pragma unroll
+  for (int j = 0; j < S::NP; ++j) s.piece(j, lds, wid);
+  s.end();
+}
 
 template <int ROWS, int MODE>
 struct Reader {                                    // fragments of a wave's ROWS / 2 rows
@@ -175,21 +198,22 @@ template <int BM, int BN> struct Tile {
   // lands while stage t is multiplied.  SB may be any staging object with issue(); nk stages.
   template <class E, int AM, int BMD, int PROD, class SA, class SB>
   __device__ __forceinline__ void mul(SA& sa, SB& sb, int nk, char* smem, int wid, int lane) {
+    if constexpr (BM == 256) return mul_large<E, AM, BMD, PROD>(sa, sb, nk, smem, wid, lane);
     const unsigned lds = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem;
     Reader<BM, AM> ra;
     Reader<BN, BMD> rb;
     ra.init(wid & 1, lane);
     rb.init(wid >> 1, lane);
-    sa.issue(lds, wid);
-    sb.issue(lds + BM * 128, wid);
+    issue(sa, lds, wid);
+    issue(sb, lds + BM * 128, wid);
     for (int t = 0; t < nk; ++t) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       if (t + 1 < nk) {
         const unsigned nl = lds + (unsigned)(((t + 1) & 1) * STAGE);
-        sa.issue(nl, wid);
-        sb.issue(nl + BM * 128, wid);
+        issue(sa, nl, wid);
+        issue(sb, nl + BM * 128, wid);
       }
       const char* ta = smem + (t & 1) * STAGE;
       const char* tb = ta + BM * 128;
@@ -225,6 +249,97 @@ template <int BM, int BN> struct Tile {
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();                          // every wave has read its last fragments: windows may be written
+    asm volatile("" ::: "memory");
+  }
+
+  // The same for tiles so large that a CU holds one block (256 x 256: 128 KiB of stages, one wave per SIMD, 128 x 128 a wave).  Nothing but
+  // this wave hides its latencies, so the fragments of the next half stage are read between the products of this one, and the one
+  // barrier per stage sits between the halves:  behind it every wave has read all of stage t (its second half is in registers) and all
+  // pieces of stage t+1 have landed;  stage t+2 is then requested into t's place and t+1's first half read.  256 x 256 asks the
+  // L2 -> LDS path for half the bytes per operation of 128 x 128, which sits at that path's ~25 bytes per clock and CU.
+  template <class E, int AM, int BMD, int PROD, class SA, class SB>
+  __device__ __forceinline__ void mul_large(SA& sa, SB& sb, int nk, char* smem, int wid, int lane) {
+    static_assert(FM == 8 && FN == 8 && SA::NP == 8 && SB::NP == 8, "256 x 256 tiles");
+    const unsigned lds = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem;
+    Reader<BM, AM> ra;
+    Reader<BN, BMD> rb;
+    ra.init(wid & 1, lane);
+    rb.init(wid >> 1, lane);
+    issue(sa, lds, wid);
+    issue(sb, lds + BM * 128, wid);
+    issue(sa, lds + STAGE, wid);
+    issue(sb, lds + STAGE + BM * 128, wid);
+    asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    s16x8 a0[FM], b0[FN], a1[FM], b1[FN], b2[FN];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a0[i] = ra.get(smem, i, 0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b0[i] = rb.get(smem + BM * 128, i, 0);
+    settle();
+    for (int t = 0; t < nk; ++t) {
+      const unsigned cur = (unsigned)((t & 1) * STAGE), nxt = STAGE - cur;
+      const char* const ta = smem + cur;
+      const char* const tb = ta + BM * 128;
+      const char* const na = smem + nxt;
+      const char* const nb = na + BM * 128;
+      // first half: hi x hi of split operands
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i < 4) { a1[2 * i] = ra.get(ta, 2 * i, 1); a1[2 * i + 1] = ra.get(ta, 2 * i + 1, 1); }
+        else       { b1[2 * i - 8] = rb.get(tb, 2 * i - 8, 1); b1[2 * i - 7] = rb.get(tb, 2 * i - 7, 1); }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) E::mfma_tied(b0[i], a0[j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      sa.begin();
+      sb.begin();
+      if (PROD == 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (i < 4) {
+            sa.piece(2 * i, lds + cur, wid); sa.piece(2 * i + 1, lds + cur, wid);
+            sb.piece(2 * i, lds + cur + BM * 128, wid); sb.piece(2 * i + 1, lds + cur + BM * 128, wid);
+            a0[2 * i] = ra.get(na, 2 * i, 0); a0[2 * i + 1] = ra.get(na, 2 * i + 1, 0);
+          } else {
+            b0[2 * i - 8] = rb.get(nb, 2 * i - 8, 0); b0[2 * i - 7] = rb.get(nb, 2 * i - 7, 0);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) E::mfma_tied(b1[i], a1[j], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {                      // lo x hi
+          if (i < 4) {
+            sa.piece(2 * i, lds + cur, wid); sa.piece(2 * i + 1, lds + cur, wid);
+            sb.piece(2 * i, lds + cur + BM * 128, wid); sb.piece(2 * i + 1, lds + cur + BM * 128, wid);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) E::mfma_tied(b1[i], a0[j], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {                      // hi x lo; the hi fragments of A are free
+          if (i < 4) { a0[2 * i] = ra.get(na, 2 * i, 0); a0[2 * i + 1] = ra.get(na, 2 * i + 1, 0); }
+          else       { b2[2 * i - 8] = rb.get(nb, 2 * i - 8, 0); b2[2 * i - 7] = rb.get(nb, 2 * i - 7, 0); }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) E::mfma_tied(b0[i], a1[j], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b0[i] = b2[i];
+      }
+      sa.end();
+      sb.end();
+    }
+    settle();
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   }
 

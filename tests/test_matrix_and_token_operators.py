@@ -639,3 +639,26 @@ def test_trainer_runs_with_muon(device, tmp_path):
     from distributed_deep_learning_amd import trainer
     hist = trainer.run(Config(model="lenet5", optimizer="muon", device=device, epochs=1, batch=16, samples=96, max_steps=3), printer=lambda *a: None)
     assert math.isfinite(hist[0]["train_loss"])
+
+
+@gpu
+@pytest.mark.parametrize("T,D,H", [(4100, 1032, 4360), (8192, 2048, 2056)])
+def test_gated_mlp_large_tiles(T, D, H):
+    """Sizes that take 256 x 256 tiles, with ragged edges, against fp32 products on the GPU: their own error (n 2^-24 of the magnitudes) is
+    far below the tolerance, which is that of the small cases per row norm: three roundings to bf16 on the way and one of the result."""
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    r = lambda *s, k=1.0: (torch.randn(s, generator=gen, device="cuda") * k).to(BF)          # noqa: E731
+    leaves = [t.requires_grad_() for t in (r(T, D), r(H, D, k=D ** -0.5), r(H, D, k=D ** -0.5), r(D, H, k=H ** -0.5))]
+    dy = r(T, D, k=0.1)
+    y = F.gated_mlp(*leaves)
+    got = (y, *torch.autograd.grad(y, leaves, dy))
+    x, wg, wu, wd, dyf = (t.detach().float() for t in (*leaves, dy))
+    g, u = x @ wg.t(), x @ wu.t()
+    s = torch.sigmoid(g)
+    a, d = g * s, s * (1 + g * (1 - s))
+    dh = dyf @ wd
+    dg, du = dh * u * d, dh * a
+    ref = ((a * u) @ wd.t(), dg @ wg + du @ wu, dg.t() @ x, du.t() @ x, dyf.t() @ (a * u))
+    for o, q in zip(got, ref):
+        rows = (o.float() - q).norm(dim=1) / q.norm(dim=1)
+        assert torch.isfinite(o).all() and float(rows.max()) <= 4 * B8, float(rows.max())
