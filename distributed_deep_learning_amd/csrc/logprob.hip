@@ -2,8 +2,8 @@
 //
 //   lse = log sum_j exp z_j      logp = z_t - lse      H = lse - sum_j p_j z_j      top: the k largest z_j - lse
 //
-// One pass over the logits: every thread carries the running maximum m, s = sum e^(z - m) and q = sum e^(z - m) (z - m) of what it
-// has seen (a larger maximum m' rescales: s' = f s, q' = f (q + (m - m') s), f = e^(m - m')); H = log s - q / s.  The kernel is
+// One pass over the logits: every thread carries the maximum m, s = sum e^(z - m) and q = sum e^(z - m) (z - m) of what it
+// has seen (joining to a larger m' rescales: s' = f s, q' = f (q + (m - m') s), f = e^(m - m')); H = log s - q / s.  The kernel is
 // bound by reading z once.  A row is cut into parts when there are too few rows to fill the chip, and a second launch joins
 // (m, s, q) and the candidate lists of the parts.
 //
@@ -173,60 +173,22 @@ __device__ __forceinline__ void finish_row(const Stat& st, const T* row, long lo
   }
 }
 
-// ---- one part of one row, nothing but the statistics
-template <typename T>
-__global__ __launch_bounds__(NT) void logprob_stats_kernel(const T* __restrict__ z, const long long* __restrict__ tokens, int V, int parts,
-                                                           int per, Stat* __restrict__ pstat, const Outs o) {
-  __shared__ Stat red[4];
-  const long long r = blockIdx.x / (unsigned)parts;
-  const int part = (int)(blockIdx.x - (unsigned)r * (unsigned)parts);
-  const T* const row = z + r * V;
-  const Split sp = split_row(row, V);
-  const T* const body = row + sp.first;
-  const int c0 = part * per, c1 = min(sp.pieces, c0 + per);
-  Stat st{-FLT_MAX, 0.f, 0.f};
-  if (part == 0) {
-    const int j = edge_element(sp, threadIdx.x);
-    if (j >= 0) stat_add1(st, Io<T>::one(row + j));
+// The k largest of `n` gathered candidates, in order, by counting: list[n] -> best[k].
+__device__ __forceinline__ void order_list(const u64* list, unsigned n, int k, u64* best) {
+  for (unsigned i = threadIdx.x; i < n; i += NT) {
+    const u64 me = list[i];
+    int rank = 0;
+    for (unsigned j = 0; j < n; ++j) rank += list[j] > me ? 1 : 0;
+    if (rank < k) best[rank] = me;
   }
-  int c = c0 + (int)threadIdx.x;
-  for (; c + 3 * NT < c1; c += 4 * NT) {                               // four 16-byte loads in flight, one rescaling for their 32 values
-    typename Io<T>::Raw raw[4];
-    float f[8], mx = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) raw[u] = Io<T>::load(body + (long long)(c + u * NT) * 8);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) { Io<T>::unpack(raw[u], f); mx = fmaxf(mx, max8(f)); }
-    if (mx > st.m) stat_rescale(st, mx);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) { Io<T>::unpack(raw[u], f); stat_add8(st, f); }
-  }
-  for (; c < c1; c += NT) {
-    float f[8];
-    Io<T>::unpack(Io<T>::load(body + (long long)c * 8), f);
-    const float mx = max8(f);
-    if (mx > st.m) stat_rescale(st, mx);
-    stat_add8(st, f);
-  }
-  st = stat_wave(st);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = st;
-  __syncthreads();
-  st = stat_join(stat_join(red[0], red[1]), stat_join(red[2], red[3]));
-  if (parts == 1) finish_row(st, row, tokens[r], V, r, 0, 0ull, o);
-  else if (threadIdx.x == 0) pstat[r * parts + part] = st;
 }
 
-// ---- the same with the k largest; at most NCH pieces a thread, `groups` (a power of two >= k) disjoint sets of threads
-template <typename T, int NCH>
-__global__ __launch_bounds__(NT, 4) void logprob_top_kernel(const T* __restrict__ z, const long long* __restrict__ tokens, int V, int parts,
-                                                            int per, int k, int groups, Stat* __restrict__ pstat, u64* __restrict__ ptop,
-                                                            const Outs o) {
+// ---- one part of one row.  NCH pieces a thread are in registers at a time; without TOP a part may be longer and is taken in turns.
+// `groups`: a power of two >= k, disjoint sets of threads.
+template <typename T, int NCH, bool TOP>
+__global__ __launch_bounds__(NT, 4) void logprob_kernel(const T* __restrict__ z, const long long* __restrict__ tokens, int V, int parts, int per,
+                                                        int k, int groups, Stat* __restrict__ pstat, u64* __restrict__ ptop, const Outs o) {
   __shared__ Stat red[4];
-  __shared__ u64 ured[4];
-  __shared__ float gmax[4][64];
-  __shared__ u64 list[CAP];
-  __shared__ u64 best[TOP_MAX];
-  __shared__ unsigned count;
   const int tid = threadIdx.x;
   const long long r = blockIdx.x / (unsigned)parts;
   const int part = (int)(blockIdx.x - (unsigned)r * (unsigned)parts);
@@ -234,36 +196,52 @@ __global__ __launch_bounds__(NT, 4) void logprob_top_kernel(const T* __restrict_
   const Split sp = split_row(row, V);
   const T* const body = row + sp.first;
   const int c0 = part * per, c1 = min(sp.pieces, c0 + per);
-  const int mine = c0 + tid;                                             // this thread's pieces: mine + u * NT
-  typename Io<T>::Raw raw[NCH];
-#pragma unroll
-  for (int u = 0; u < NCH; ++u) {
-    raw[u] = nothing<T>();
-    if (mine + u * NT < c1) raw[u] = Io<T>::load(body + (long long)(mine + u * NT) * 8);
-  }
   const int je = part == 0 ? edge_element(sp, tid) : -1;
   const float ze = je >= 0 ? Io<T>::one(row + je) : -INFINITY;
-  // (pinned before every pass: else the compiler keeps what one pass unpacked for the next, four times the registers)
-  // the thread's maximum, then sums about it: no rescaling inside the thread
   Stat st{-FLT_MAX, 0.f, 0.f};
-  float tm = ze;
-  if (tm != tm) tm = -INFINITY;
+  typename Io<T>::Raw raw[NCH];
+  float tm = ze == ze ? ze : -INFINITY;                                  // this thread's largest
+  int mine = c0 + tid;                                                   // its pieces: mine + u * NT
+  for (;; mine += NCH * NT) {
 #pragma unroll
-  for (int u = 0; u < NCH; ++u) {
-    float f[8];
-    Io<T>::pin(raw[u]);
-    Io<T>::unpack(raw[u], f);
-    tm = fmaxf(tm, max8(f));
-  }
-  st.m = fmaxf(tm, -FLT_MAX);
+    for (int u = 0; u < NCH; ++u) {
+      raw[u] = nothing<T>();
+      if (mine + u * NT < c1) raw[u] = Io<T>::load(body + (long long)(mine + u * NT) * 8);
+    }
+    // the maximum first, then the sums about it: one rescaling.  (Pinned before every pass: else the compiler keeps what one pass
+    // unpacked for the next, four times the registers.)
 #pragma unroll
-  for (int u = 0; u < NCH; ++u) {
-    float f[8];
-    Io<T>::pin(raw[u]);
-    Io<T>::unpack(raw[u], f);
-    stat_add8(st, f);
+    for (int u = 0; u < NCH; ++u) {
+      float f[8];
+      Io<T>::pin(raw[u]);
+      Io<T>::unpack(raw[u], f);
+      tm = fmaxf(tm, max8(f));
+    }
+    if (tm > st.m) stat_rescale(st, tm);
+#pragma unroll
+    for (int u = 0; u < NCH; ++u) {
+      float f[8];
+      Io<T>::pin(raw[u]);
+      Io<T>::unpack(raw[u], f);
+      stat_add8(st, f);
+    }
+    if (TOP || mine - tid + NCH * NT >= c1) break;
   }
   if (je >= 0) stat_add1(st, ze);
+  if (!TOP) {
+    st = stat_wave(st);
+    if ((tid & 63) == 0) red[tid >> 6] = st;
+    __syncthreads();
+    st = stat_join(stat_join(red[0], red[1]), stat_join(red[2], red[3]));
+    if (parts == 1) finish_row(st, row, tokens[r], V, r, 0, 0ull, o);
+    else if (tid == 0) pstat[r * parts + part] = st;
+    return;
+  }
+  __shared__ u64 ured[4];
+  __shared__ float gmax[4][64];
+  __shared__ u64 list[CAP];
+  __shared__ u64 best[TOP_MAX];
+  __shared__ unsigned count;
   // a bound that at least k elements reach: the smallest of `groups` maxima over disjoint sets
   float gm = tm;
   for (int off = 32; off >= groups; off >>= 1) gm = fmaxf(gm, __shfl_xor(gm, off, 64));
@@ -300,12 +278,7 @@ __global__ __launch_bounds__(NT, 4) void logprob_top_kernel(const T* __restrict_
   __syncthreads();
   const unsigned n = count;
   if (n <= CAP) {
-    for (unsigned i = tid; i < n; i += NT) {
-      const u64 me = list[i];
-      int rank = 0;
-      for (unsigned j = 0; j < n; ++j) rank += list[j] > me ? 1 : 0;
-      if (rank < k) best[rank] = me;
-    }
+    order_list(list, n, k, best);
   } else {                                                               // many elements tie with the bound
     u64 prev = ~0ull;
     for (int t = 0; t < k; ++t) {
@@ -335,10 +308,9 @@ __global__ __launch_bounds__(NT, 4) void logprob_top_kernel(const T* __restrict_
 
 // ---- joins the parts of a row: one block per row
 template <typename T>
-__global__ __launch_bounds__(NT) void logprob_join_kernel(const T* __restrict__ z, const long long* __restrict__ tokens, int V, int parts, int k,
+__global__ __launch_bounds__(NT) void logprob_join_kernel(const T* __restrict__ z, const long long* __restrict__ tokens, int V, int parts, int k, int groups,
                                                           const Stat* __restrict__ pstat, const u64* __restrict__ ptop, const Outs o) {
   __shared__ Stat red[4];
-  __shared__ u64 ured[4];
   const int tid = threadIdx.x;
   const long long r = blockIdx.x;
   Stat st{-FLT_MAX, 0.f, 0.f};
@@ -347,16 +319,49 @@ __global__ __launch_bounds__(NT) void logprob_join_kernel(const T* __restrict__ 
   if ((tid & 63) == 0) red[tid >> 6] = st;
   __syncthreads();
   st = stat_join(stat_join(red[0], red[1]), stat_join(red[2], red[3]));
-  u64 prev = ~0ull, mine = 0ull;
-  for (int t = 0; t < k; ++t) {
-    u64 mx = 0ull;
-    for (int i = tid; i < parts * k; i += NT) {
-      const u64 v = ptop[r * parts * k + i];
-      mx = v < prev && v > mx ? v : mx;
+  if (k == 0) { finish_row(st, z + r * V, tokens[r], V, r, 0, 0ull, o); return; }
+  // the same bound over the parts' lists (keys here: a NaN counts)
+  __shared__ u64 ured[4];
+  __shared__ unsigned gmax[4][64];
+  __shared__ u64 list[CAP];
+  __shared__ u64 best[TOP_MAX];
+  __shared__ unsigned count;
+  const u64* const src = ptop + r * parts * k;
+  const int total = parts * k;
+  unsigned mk = 0u;
+  for (int i = tid; i < total; i += NT) mk = max(mk, (unsigned)(src[i] >> 32));
+  for (int off = 32; off >= groups; off >>= 1) mk = max(mk, (unsigned)__shfl_xor((int)mk, off, 64));
+  gmax[tid >> 6][tid & 63] = mk;
+  if (tid == 0) count = 0u;
+  __syncthreads();
+  unsigned bound = max(max(gmax[0][tid & 63], gmax[1][tid & 63]), max(gmax[2][tid & 63], gmax[3][tid & 63]));
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) bound = min(bound, (unsigned)__shfl_xor((int)bound, off, 64));
+  bound = max(bound, 1u);                                                // 0 marks what a short part left empty
+  for (int i = tid; i < total; i += NT) {
+    const u64 v = src[i];
+    if ((unsigned)(v >> 32) >= bound) {
+      const unsigned at = atomicAdd(&count, 1u);
+      if (at < CAP) list[at] = v;
     }
-    prev = block_max(mx, ured);
-    if (tid == t) mine = prev;
   }
+  __syncthreads();
+  if (count <= CAP) {
+    order_list(list, count, k, best);
+  } else {
+    u64 prev = ~0ull;
+    for (int t = 0; t < k; ++t) {
+      u64 mx = 0ull;
+      for (int i = tid; i < total; i += NT) {
+        const u64 v = src[i];
+        mx = v < prev && v > mx ? v : mx;
+      }
+      prev = block_max(mx, ured);
+      if (tid == 0) best[t] = prev;
+    }
+  }
+  __syncthreads();
+  const u64 mine = tid < k ? best[tid] : 0ull;
   finish_row(st, z + r * V, tokens[r], V, r, k, mine, o);
 }
 
@@ -441,13 +446,13 @@ int plan(long long rows, int V, int most) {
 int parts_of(int V, int per) { const int pieces = V / 8; return pieces == 0 ? 1 : (pieces + per - 1) / per; }
 
 // Most pieces a thread keeps in registers: 64 registers of logits, of the 128 that four waves per SIMD have.
-template <typename T> struct TopPieces { static constexpr int value = sizeof(T) == 2 ? 16 : 8; };
+template <typename T> struct MaxPieces { static constexpr int value = sizeof(T) == 2 ? 16 : 8; };
 
 template <typename T, int NCH>
-void launch_top(dim3 grid, hipStream_t st, const T* z, const long long* tokens, int V, int parts, int per, int k, Stat* ps, u64* pt, const Outs& o) {
-  int groups = 1;
-  while (groups < k) groups *= 2;
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_top_kernel<T, NCH>), grid, dim3(NT), 0, st, z, tokens, V, parts, per, k, groups, ps, pt, o);
+void launch(dim3 grid, hipStream_t st, const T* z, const long long* tokens, int V, int parts, int per, int k, int groups, Stat* ps, u64* pt,
+            const Outs& o) {
+  if (k > 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_kernel<T, NCH, true>), grid, dim3(NT), 0, st, z, tokens, V, parts, per, k, groups, ps, pt, o);
+  else hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_kernel<T, NCH, false>), grid, dim3(NT), 0, st, z, tokens, V, parts, per, k, groups, ps, pt, o);
 }
 
 template <typename T>
@@ -455,21 +460,18 @@ int forward(const T* z, const long long* tokens, long long rows, int V, int k, i
   Stat* const ps = (Stat*)ws;
   u64* const pt = (u64*)((char*)ws + ((size_t)rows * parts * sizeof(Stat) + 15) / 16 * 16);
   const dim3 grid((unsigned)(rows * parts));
-  if (k == 0) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_stats_kernel<T>), grid, dim3(NT), 0, st, z, tokens, V, parts, per, ps, o);
-  } else {
-    const int nch = (per + NT - 1) / NT;
-    if (nch <= 1) launch_top<T, 1>(grid, st, z, tokens, V, parts, per, k, ps, pt, o);
-    else if (nch <= 4) launch_top<T, 4>(grid, st, z, tokens, V, parts, per, k, ps, pt, o);
-    else launch_top<T, TopPieces<T>::value>(grid, st, z, tokens, V, parts, per, k, ps, pt, o);
-  }
+  int groups = 1;
+  while (groups < k) groups *= 2;
+  if (per <= NT) launch<T, 1>(grid, st, z, tokens, V, parts, per, k, groups, ps, pt, o);
+  else if (per <= 4 * NT) launch<T, 4>(grid, st, z, tokens, V, parts, per, k, groups, ps, pt, o);
+  else launch<T, MaxPieces<T>::value>(grid, st, z, tokens, V, parts, per, k, groups, ps, pt, o);
   if (parts > 1)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_join_kernel<T>), dim3((unsigned)rows), dim3(NT), 0, st, z, tokens, V, parts, k, ps, pt, o);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_join_kernel<T>), dim3((unsigned)rows), dim3(NT), 0, st, z, tokens, V, parts, k, groups, ps, pt, o);
   return (int)hipGetLastError();
 }
 
 int parts_for(long long rows, int V, int is_bf16, int k, int* per) {
-  *per = plan(rows, V, k > 0 ? NT * (is_bf16 ? TopPieces<bf16_t>::value : TopPieces<float>::value) : 0x7fffff00);
+  *per = plan(rows, V, k > 0 ? NT * (is_bf16 ? MaxPieces<bf16_t>::value : MaxPieces<float>::value) : 0x7fffff00);
   return parts_of(V, *per);
 }
 

@@ -974,18 +974,18 @@ class GatedMLP(torch.autograd.Function):
             wg, wu, wd = pad(wg, (0, pd, 0, pf)), pad(wu, (0, pd, 0, pf)), pad(wd, (0, pf, 0, pd))
         x16, wg, wu, wd = (K._aligned(t) for t in (x16, wg, wu, wd))
         train = any(ctx.needs_input_grad[:4])
-        h, g, u = K.gated_up(x16, wg, wu, activation, save=train)
+        h, keep = K.gated_up(x16, wg, wu, activation, save=train)
         y = K.gated_down(h, wd)
         if train:
-            ctx.save_for_backward(x16, wg, wu, wd, h, g, u)
-            ctx.meta = (D, F_, activation, x.dtype, (w_gate, w_up, w_down))
+            ctx.save_for_backward(x16, wg, wu, wd, h, *keep)
+            ctx.meta = (D, F_, x.dtype, (w_gate, w_up, w_down))
         return y[:, :D] if pd else y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, wg, wu, wd, h, g, u = ctx.saved_tensors
-        D, F_, activation, x_dtype, weights = ctx.meta
+        x, wg, wu, wd, h, *keep = ctx.saved_tensors
+        D, F_, x_dtype, weights = ctx.meta
         need = ctx.needs_input_grad
         padded = x.shape[1] != D or h.shape[1] != F_
         with device_of(x):
@@ -995,7 +995,7 @@ class GatedMLP(torch.autograd.Function):
             dy = K._aligned(dy)
             dg = du = dx = None
             if need[0] or need[1] or need[2]:
-                dg, du = K.gated_dh(dy, wd, g, u, activation)
+                dg, du = K.gated_dh(dy, wd, keep)
             if need[0]:
                 dx = K.gated_dx(dg, du, wg, wu)
                 dx = (dx[:, :D] if x.shape[1] != D else dx).to(x_dtype)

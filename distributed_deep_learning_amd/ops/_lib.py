@@ -109,7 +109,7 @@ _SIGS = {
     "ddl_muon_step": [_vp] * 14 + [_i, _i, _vp, _f, _i, _vp],
     "ddl_gated_up": [_vp] * 6 + [_i, _i, _i, _i, _vp],
     "ddl_gated_down": [_vp, _vp, _vp, _i, _i, _i, _vp],
-    "ddl_gated_dh": [_vp] * 6 + [_i, _i, _i, _i, _vp],
+    "ddl_gated_dh": [_vp] * 6 + [_i, _i, _i, _vp],
     "ddl_gated_dx": [_vp] * 5 + [_i, _i, _i, _vp],
     "ddl_gated_dw": [_vp] * 8 + [_i, _i, _i, _i, _vp],
     "ddl_logprob_top_max": [],

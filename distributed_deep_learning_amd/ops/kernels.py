@@ -1248,7 +1248,8 @@ def _chk_gated(name: str, **mats):
 
 def gated_up(x, w_gate, w_up, activation: str = "silu", save: bool = False):
     """``h = act(x @ w_gate^T) * (x @ w_up^T)``: ``x`` ``[M, D]``, weights ``[F, D]``, all bf16, ``D`` and ``F`` multiples of 8.
-    Returns ``(h, g, u)``; the projections ``g`` and ``u`` are kept with ``save`` (training), else ``None``."""
+    Returns ``(h, keep)``: with ``save`` (training) ``keep`` is the pair of tensors :func:`gated_dh` takes - the factors ``u act'(g)``
+    and ``act(g)`` in 24 bits, 16 of them in an int16 and 8 in a uint8 tensor ``[2, M, F]`` - else ``None``."""
     lib = _lib.require()
     M, D = x.shape
     F_ = w_gate.shape[0]
@@ -1256,11 +1257,12 @@ def gated_up(x, w_gate, w_up, activation: str = "silu", save: bool = False):
         raise ValueError("gated_up: widths must be multiples of 8")
     _chk_gated("gated_up", x=(x, (M, D)), w_gate=(w_gate, (F_, D)), w_up=(w_up, (F_, D)))
     h = torch.empty((M, F_), dtype=BF16, device=x.device)
-    g, u = (torch.empty_like(h), torch.empty_like(h)) if save else (None, None)
+    keep = (torch.empty((2, M, F_), dtype=torch.int16, device=x.device),
+            torch.empty((2, M, F_), dtype=torch.uint8, device=x.device)) if save else None
     if M > 0:
-        check(lib.ddl_gated_up(ptr(x), ptr(w_gate), ptr(w_up), ptr(h), ptr(g), ptr(u), M, D, F_, GATED_ACTIVATIONS[activation],
-                               stream_ptr()), "gated_up")
-    return h, g, u
+        check(lib.ddl_gated_up(ptr(x), ptr(w_gate), ptr(w_up), ptr(h), ptr(keep[0]) if save else None, ptr(keep[1]) if save else None,
+                               M, D, F_, GATED_ACTIVATIONS[activation], stream_ptr()), "gated_up")
+    return h, keep
 
 
 def gated_down(h, w_down):
@@ -1277,16 +1279,18 @@ def gated_down(h, w_down):
     return y
 
 
-def gated_dh(dy, w_down, g, u, activation: str = "silu"):
-    """``dh = dy @ w_down`` folded straight into ``(dg, du) = (dh u act'(g), dh act(g))``, bf16 ``[M, F]``."""
+def gated_dh(dy, w_down, keep):
+    """``dh = dy @ w_down`` folded straight into ``(dg, du) = (dh u act'(g), dh act(g))``, bf16 ``[M, F]``; ``keep`` from :func:`gated_up`."""
     lib = _lib.require()
     M, D = dy.shape
     F_ = w_down.shape[1]
-    _chk_gated("gated_dh", dy=(dy, (M, D)), w_down=(w_down, (D, F_)), g=(g, (M, F_)), u=(u, (M, F_)))
-    dg, du = torch.empty_like(g), torch.empty_like(g)
+    _chk_gated("gated_dh", dy=(dy, (M, D)), w_down=(w_down, (D, F_)))
+    for t, dt in zip(keep, (torch.int16, torch.uint8)):
+        if tuple(t.shape) != (2, M, F_) or t.dtype != dt or not t.is_contiguous() or t.device != dy.device:
+            raise ValueError("gated_dh: keep must be what gated_up(save=True) returned for these sizes")
+    dg, du = (torch.empty((M, F_), dtype=BF16, device=dy.device) for _ in range(2))
     if M > 0:
-        check(lib.ddl_gated_dh(ptr(dy), ptr(w_down), ptr(g), ptr(u), ptr(dg), ptr(du), M, D, F_, GATED_ACTIVATIONS[activation],
-                               stream_ptr()), "gated_dh")
+        check(lib.ddl_gated_dh(ptr(dy), ptr(w_down), ptr(keep[0]), ptr(keep[1]), ptr(dg), ptr(du), M, D, F_, stream_ptr()), "gated_dh")
     return dg, du
 
 
