@@ -177,13 +177,18 @@ struct Reader {                                    // fragments of a wave's ROWS
   }
 };
 
-template <int BM, int BN> struct Tile {
+template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory"); }
+
+// NST: stages in LDS.  2 (64 KiB for 128 x 128, two blocks on a CU hide each other's latency) or 4 (three stages on their way: for launches
+// of no more blocks than CUs).
+template <int BM, int BN, int NST = 2> struct Tile {
   static constexpr int WM = BM / 2, WN = BN / 2;           // rows / columns of a wave
   static constexpr int FM = WM / 16, FN = WN / 16;
   static constexpr int STAGE = (BM + BN) * 128;
   static constexpr int WPITCH = WN + 4;                    // floats per row of a wave's output window
   static constexpr int WBYTES = 16 * WPITCH * 4;
-  static constexpr int SMEM = 2 * STAGE;
+  static constexpr int SMEM = NST * STAGE;
+  static constexpr int SLAB = FN * FM * 1024;                // floats of a partial tile (all four waves)
   static_assert(4 * WBYTES <= SMEM, "output windows reuse the stages");
   f32x4 acc[FN][FM];
 
@@ -194,28 +199,53 @@ template <int BM, int BN> struct Tile {
       for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // acc += product.  Two stages: stage t+1 is requested as soon as every wave has left stage t-1 (the barrier at the top), and
-  // lands while stage t is multiplied.  SB may be any staging object with issue(); nk stages.
+  // Partial tiles of a split reduction: every lane's accumulators as they are, 16-byte stores that are contiguous over the block.
+  __device__ __forceinline__ void put_slab(float* slab, int tid) const {
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int j = 0; j < FM; ++j) *reinterpret_cast<f32x4*>(slab + ((i * FM + j) * 256 + tid) * 4) = acc[i][j];
+  }
+  // Only the wave's 16-row group j, so that a tile is joined by FM blocks.  In order: the result does not depend on timing.
+  __device__ __forceinline__ void sum_slabs(const float* slab, int n, int j, int tid) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i) acc[i][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+#pragma unroll
+      for (int i = 0; i < FN; ++i) acc[i][0] += *reinterpret_cast<const f32x4*>(slab + (long long)s * SLAB + ((i * FM + j) * 256 + tid) * 4);
+    }
+  }
+
+  // acc += product over nk stages.  The stage NST - 1 ahead is requested as soon as every wave has left the one whose place it takes (the
+  // barrier at the top), and lands while those between are multiplied.
   template <class E, int AM, int BMD, int PROD, class SA, class SB>
   __device__ __forceinline__ void mul(SA& sa, SB& sb, int nk, char* smem, int wid, int lane) {
-    if constexpr (BM == 256) return mul_large<E, AM, BMD, PROD>(sa, sb, nk, smem, wid, lane);
+    if constexpr (BM == 256) {
+      mul_large<E, AM, BMD, PROD>(sa, sb, nk, smem, wid, lane);
+      return;
+    }
     const unsigned lds = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem;
+    constexpr int PER = SA::NP + SB::NP;
     Reader<BM, AM> ra;
     Reader<BN, BMD> rb;
     ra.init(wid & 1, lane);
     rb.init(wid >> 1, lane);
-    issue(sa, lds, wid);
-    issue(sb, lds + BM * 128, wid);
+#pragma unroll
+    for (int q = 0; q < NST - 1; ++q) {
+      issue(sa, lds + q * STAGE, wid);
+      issue(sb, lds + q * STAGE + BM * 128, wid);
+    }
     for (int t = 0; t < nk; ++t) {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      wait_vm<(NST - 2) * PER>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (t + 1 < nk) {
-        const unsigned nl = lds + (unsigned)(((t + 1) & 1) * STAGE);
+      if (NST > 2 || t + 1 < nk) {                           // behind the end: zeros, so that the counted waits stay uniform
+        const unsigned nl = lds + (unsigned)(((t + NST - 1) % NST) * STAGE);
         issue(sa, nl, wid);
         issue(sb, nl + BM * 128, wid);
       }
-      const char* ta = smem + (t & 1) * STAGE;
+      const char* ta = smem + (t % NST) * STAGE;
       const char* tb = ta + BM * 128;
       s16x8 a0[FM], b0[FN];
 #pragma unroll
@@ -247,7 +277,7 @@ template <int BM, int BN> struct Tile {
           for (int j = 0; j < FM; ++j) acc[i][j] = E::mfma(b0[i], a1[j], acc[i][j]);
       }
     }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    wait_vm<0>();
     __builtin_amdgcn_s_barrier();                          // every wave has read its last fragments: windows may be written
     asm volatile("" ::: "memory");
   }
@@ -345,12 +375,13 @@ template <int BM, int BN> struct Tile {
 
   // Rows of the wave's part, 16 at a time through its own window: f(m, n, v[8]) with tile-relative m and n (n a multiple of 8).
   // With COLS the window is also walked down its columns: ft(n, m, v[8]), m a multiple of 8 - the transposed tile.
-  template <bool COLS, class F, class FT>
-  __device__ __forceinline__ void store(char* smem, int wid, int lane, F&& f, FT&& ft) {
+  // NJ = 1: the one group that sum_slabs() left, which is group j0 of the tile.
+  template <bool COLS, int NJ = FM, class F, class FT>
+  __device__ __forceinline__ void store(char* smem, int wid, int lane, F&& f, FT&& ft, int j0 = 0) {
     float* const win = reinterpret_cast<float*>(smem + wid * WBYTES);
-    const int wm0 = (wid & 1) * WM, wn0 = (wid >> 1) * WN;
+    const int wm0 = (wid & 1) * WM + j0 * 16, wn0 = (wid >> 1) * WN;
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
+    for (int j = 0; j < NJ; ++j) {
 #pragma unroll
       for (int i = 0; i < FN; ++i)
         *reinterpret_cast<f32x4*>(win + (lane & 15) * WPITCH + i * 16 + (lane >> 4) * 4) = acc[i][j];

@@ -16,7 +16,7 @@
 // The Frobenius norm is summed in fp64, in a fixed order.
 //
 // Many matrices share every launch: blocks find their matrix through maps of (matrix, block) pairs, so an optimizer step over a whole
-// network is 2 + 3 * steps launches.
+// network is 2 launches and 3 to 6 for every step of the iteration (joins of split reductions, two tile sizes), whatever it has of them.
 #include "common.h"
 #include "host_util.h"
 #include "gemm_tile.h"
@@ -25,14 +25,16 @@
 namespace {
 
 constexpr float SCALE = 4096.f, UNSCALE = 1.f / 4096.f;
-constexpr int MAX_PARTS = 256;                   // partial sums of squares per matrix
+constexpr int MAX_PARTS = 1024;                  // partial sums of squares per matrix
 constexpr int INIT_CHUNKS = 1024;                // 8-element pieces of X0 per block of the init kernel
 
 struct NsMat {                                   // one matrix of a step (device table, or the one of a plain call)
   long long elem;                                // Muon: element offset in the arena;  plain: 0
   long long ws;                                  // fp16 offset of its workspace: X, X', S, B
+  long long slab;                                // float offset of its partial tiles
   int rows, cols, seg;
   float scale;                                   // Muon: factor of the update
+  int gram_splits, square_splits;                // blocks that share the reduction of one tile
 };
 
 struct NsArgs {
@@ -40,8 +42,9 @@ struct NsArgs {
   const int2* map;                               // with a table: (matrix, block) of every block
   int per;                                       // without: blocks per matrix
   NsMat one;
-  long long g_stride, ws_stride;
+  long long g_stride, ws_stride, slab_stride;
   unsigned short* ws;
+  float* slabs;
   double* parts;                                 // [matrix][MAX_PARTS]
   float eps;
   // source / destination
@@ -86,6 +89,7 @@ __device__ __forceinline__ NsMat locate(const NsArgs& a, unsigned bid, int& mat,
   NsMat m = a.one;
   m.elem = (long long)mat * a.g_stride;
   m.ws = (long long)mat * a.ws_stride;
+  m.slab = (long long)mat * a.slab_stride;
   return m;
 }
 
@@ -133,7 +137,6 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const NsArgs a) {
     for (long long i = lo + threadIdx.x * 4; i < hi; i += 1024) {
       const f32x4 g = *reinterpret_cast<const f32x4*>(gp + i);
       f32x4 v = *reinterpret_cast<const f32x4*>(mp + i);
-      float q = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float ge = gs * g[e];
@@ -141,13 +144,33 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const NsArgs a) {
         const float u = muon_update(ge, v[e], mu, nest);
         s += (double)u * (double)u;
       }
-      (void)q;
       *reinterpret_cast<f32x4*>(mp + i) = v;
     }
   } else {
-    for (long long i = lo + threadIdx.x; i < hi; i += 256) {
-      const float g = a.g32 != nullptr ? a.g32[m.elem + i] : bf16_to_f32(a.g16[m.elem + i]);
-      s += (double)g * (double)g;
+    const bool wide = (((unsigned long long)(a.g32 != nullptr ? (const void*)(a.g32 + m.elem) : (const void*)(a.g16 + m.elem))) & 15) == 0;
+    long long i = lo + threadIdx.x * 8;
+    if (wide) {
+      auto piece = [&](long long at, float* v) {
+        if (a.g32 != nullptr) {
+          *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(a.g32 + m.elem + at);
+          *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(a.g32 + m.elem + at + 4);
+        } else {
+          unpack8(*reinterpret_cast<const u32x4*>(a.g16 + m.elem + at), v);
+        }
+      };
+#pragma unroll 4
+      for (; i + 8 <= hi; i += 2048) {
+        float v[8];
+        piece(i, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += (double)v[e] * (double)v[e];
+      }
+    }
+    for (; i < hi; i += 2048) {                             // the last elements, or a matrix of a batch that starts off a 16-byte boundary
+      for (int e = 0; e < 8 && i + e < hi; ++e) {
+        const float g = a.g32 != nullptr ? a.g32[m.elem + i + e] : bf16_to_f32(a.g16[m.elem + i + e]);
+        s += (double)g * (double)g;
+      }
     }
   }
 #pragma unroll
@@ -166,7 +189,8 @@ __global__ __launch_bounds__(256) void ns_init_kernel(const NsArgs a) {
   const Lay<PROD> L(m.rows, m.cols);
   const long long n = (long long)m.rows * m.cols, slice = slice_of(n);
   const int parts = (int)((n + slice - 1) / slice);
-  double s = (int)threadIdx.x < parts ? a.parts[(long long)mat * MAX_PARTS + threadIdx.x] : 0.0;
+  double s = 0.0;
+  for (int i = (int)threadIdx.x; i < parts; i += 256) s += a.parts[(long long)mat * MAX_PARTS + i];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -224,8 +248,11 @@ __global__ __launch_bounds__(256) void ns_init_kernel(const NsArgs a) {
 // ---- the products.  KIND 0: S = X X^T;  1: B = b S + c S S;  2: X' = a X + B X;  3: the same, last step, to the destination.
 enum { GRAM = 0, SQUARE = 1, APPLY = 2, FINAL = 3 };
 
-template <int PROD, int KIND, int BT, bool MUON>
-__global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, const int flip, const float alpha, const float beta) {
+// A tile's reduction may be shared by several blocks (few tiles, long reductions: the gram matrix of a wide X): each leaves its fp32
+// partial tile, and the launch with JOIN adds them in order and does the epilogue.
+template <int PROD, int KIND, int BT, int NST, bool MUON, bool JOIN>
+__global__ __launch_bounds__(256, BT == 256 || NST > 2 ? 1 : 2) void ns_product_kernel(const NsArgs a, const int flip, const float alpha,
+                                                                                        const float beta) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   int mat, idx;
@@ -238,12 +265,16 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
   unsigned short* const S = ws + L.s;
   unsigned short* const B = ws + L.b;
 
-  int ti, tj;
+  using T = gt::Tile<BT, BT, NST>;
+  int ti, tj, split = 0, splits = 1, which = 0;
   if (KIND <= SQUARE) {                                   // lower triangle, row by row
-    ti = (int)((sqrtf(8.f * (float)idx + 1.f) - 1.f) * 0.5f);
-    while ((ti + 1) * (ti + 2) / 2 <= idx) ++ti;
-    while (ti * (ti + 1) / 2 > idx) --ti;
-    tj = idx - ti * (ti + 1) / 2;
+    splits = KIND == GRAM ? m.gram_splits : m.square_splits;
+    if (JOIN) { which = idx / T::FM; split = idx - which * T::FM; }   // split: the row group this block joins
+    else { which = idx / splits; split = idx - which * splits; }
+    ti = (int)((sqrtf(8.f * (float)which + 1.f) - 1.f) * 0.5f);
+    while ((ti + 1) * (ti + 2) / 2 <= which) ++ti;
+    while (ti * (ti + 1) / 2 > which) --ti;
+    tj = which - ti * (ti + 1) / 2;
   } else {
     const int tm = (m.rows + BT - 1) / BT;
     tj = idx / tm;
@@ -251,26 +282,40 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
   }
   const int m0 = ti * BT, n0 = tj * BT;
 
-  gt::Tile<BT, BT> tile;
-  tile.zero();
-  auto run = [&](auto am, auto bm, const unsigned short* pa, long long lda, int ra, const unsigned short* pb, long long ldb, int rb, int k) {
-    constexpr int AM = decltype(am)::value, BMD = decltype(bm)::value;
-    gt::Stager<BT, AM, PROD> sa;
-    gt::Stager<BT, BMD, PROD> sb;
-    sa.init(gt::Operand{pa, lda, m0, ra, k}, wid, lane);
-    sb.init(gt::Operand{pb, ldb, n0, rb, k}, wid, lane);
-    tile.template mul<gt::Fp16, AM, BMD, PROD>(sa, sb, (k + sa.KSTEP - 1) / sa.KSTEP, smem, wid, lane);
-  };
-  struct C { enum { value = gt::CONTIG }; };
-  struct W { enum { value = gt::SLOW }; };
-  if (KIND == GRAM) {
-    if (tall) run(W{}, W{}, X, L.ldx, m.cols, X, L.ldx, m.cols, m.rows);
-    else      run(C{}, C{}, X, L.ldx, m.rows, X, L.ldx, m.rows, m.cols);
-  } else if (KIND == SQUARE) {
-    run(C{}, C{}, S, L.lds, thin, S, L.lds, thin, thin);
+  T tile;
+  float* const slab = a.slabs + m.slab + (long long)which * splits * T::SLAB;
+  if (JOIN) {
+    tile.sum_slabs(slab, splits, split, tid);
   } else {
-    if (tall) run(C{}, C{}, X, L.ldx, m.rows, B, L.lds, thin, thin);
-    else      run(C{}, W{}, B, L.lds, thin, X, L.ldx, m.cols, thin);
+    tile.zero();
+    auto run = [&](auto am, auto bm, const unsigned short* pa, long long lda, int ra, const unsigned short* pb, long long ldb, int rb, int k) {
+      constexpr int AM = decltype(am)::value, BMD = decltype(bm)::value;
+      using SA = gt::Stager<BT, AM, PROD>;
+      using SB = gt::Stager<BT, BMD, PROD>;
+      SA sa;
+      SB sb;
+      if (KIND <= SQUARE && splits > 1) {                 // this block's part of the reduction, whole stages
+        const int per = ((k + SA::KSTEP - 1) / SA::KSTEP + splits - 1) / splits * SA::KSTEP, k0 = min(k, split * per);
+        pa += AM == gt::SLOW ? k0 * lda : (PROD == 3 ? 2 : 1) * k0;
+        pb += BMD == gt::SLOW ? k0 * ldb : (PROD == 3 ? 2 : 1) * k0;
+        k = min(k - k0, per);
+      }
+      sa.init(gt::Operand{pa, lda, m0, ra, k}, wid, lane);
+      sb.init(gt::Operand{pb, ldb, n0, rb, k}, wid, lane);
+      tile.template mul<gt::Fp16, AM, BMD, PROD>(sa, sb, (k + SA::KSTEP - 1) / SA::KSTEP, smem, wid, lane);
+    };
+    struct C { enum { value = gt::CONTIG }; };
+    struct W { enum { value = gt::SLOW }; };
+    if (KIND == GRAM) {
+      if (tall) run(W{}, W{}, X, L.ldx, m.cols, X, L.ldx, m.cols, m.rows);
+      else      run(C{}, C{}, X, L.ldx, m.rows, X, L.ldx, m.rows, m.cols);
+    } else if (KIND == SQUARE) {
+      run(C{}, C{}, S, L.lds, thin, S, L.lds, thin, thin);
+    } else {
+      if (tall) run(C{}, C{}, X, L.ldx, m.rows, B, L.lds, thin, thin);
+      else      run(C{}, W{}, B, L.lds, thin, X, L.ldx, m.cols, thin);
+    }
+    if (KIND <= SQUARE && splits > 1) { tile.put_slab(slab + (long long)split * T::SLAB, tid); return; }
   }
 
   if (KIND <= SQUARE) {
@@ -299,11 +344,13 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
       unsigned short* q = dst + Lay<PROD>::at(r, L.lds, c);
       if (PROD == 3) split_store8(q, 32, v); else f16_store8(q, v);
     };
+    constexpr int NJ = JOIN ? 1 : T::FM;
+    const int j0 = JOIN ? split : 0;
     if (ti != tj)
-      tile.template store<true>(smem, wid, lane, [&](int r, int c, float* v) { put(m0 + r, n0 + c, v); },
-                                [&](int r, int c, float* v) { put(n0 + r, m0 + c, v); });
+      tile.template store<true, NJ>(smem, wid, lane, [&](int r, int c, float* v) { put(m0 + r, n0 + c, v); },
+                                    [&](int r, int c, float* v) { put(n0 + r, m0 + c, v); }, j0);
     else
-      tile.template store<false>(smem, wid, lane, [&](int r, int c, float* v) { put(m0 + r, n0 + c, v); }, [](int, int, float*) {});
+      tile.template store<false, NJ>(smem, wid, lane, [&](int r, int c, float* v) { put(m0 + r, n0 + c, v); }, [](int, int, float*) {}, j0);
   } else {
     unsigned short* const dst = ws + (flip ? L.x0 : L.x1);
     const int ncol = (int)(PROD == 3 ? L.ldx / 2 : L.ldx);
@@ -360,53 +407,115 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
   }
 }
 
-constexpr int BT = 128;
+constexpr int CUS = 256, SLOTS = 2 * CUS;         // two 128 x 128 blocks run on a CU
+constexpr int SLAB = gt::Tile<128, 128>::SLAB;
 
-struct Grids { int norm, init, tri, full; };
+inline int tri(int thin) { const int t = (thin + 127) / 128; return t * (t + 1) / 2; }
+inline int full(int rows, int cols, int bt) { return ((rows + bt - 1) / bt) * ((cols + bt - 1) / bt); }
+inline int stages(int k, int prod) { return prod == 3 ? (k + 31) / 32 : (k + 63) / 64; }
 
-template <int PROD> Grids grids_of(int rows, int cols) {
-  const long long n = (long long)rows * cols, slice = slice_of(n);
-  const Lay<PROD> L(rows, cols);
-  const long long pieces = (long long)rows * ((PROD == 3 ? L.ldx / 2 : L.ldx) / 8);
-  const int thin = rows < cols ? rows : cols, t = (thin + BT - 1) / BT;
-  Grids g;
-  g.norm = (int)((n + slice - 1) / slice);
-  g.init = (int)((pieces + INIT_CHUNKS - 1) / INIT_CHUNKS);
-  g.tri = t * (t + 1) / 2;
-  g.full = ((rows + BT - 1) / BT) * ((cols + BT - 1) / BT);
-  return g;
+// Stages of its reduction that a block does when `tiles` equal tiles have `ks` stages each: the split with the least rounds of blocks times
+// stages.  A partial tile costs 64 KiB written and read, about 6 stages' time beside the block's own start and end; a block alone on its
+// CU runs its stages in 0.6 of the time it needs beside another.
+inline int chunk_for(long long tiles, int ks) {
+  int best = ks;
+  double least = 1e30;
+  for (int s = 1; s == 1 || s <= ks / 8; ++s) {
+    const long long blocks = tiles * s;
+    const int per = (ks + s - 1) / s;
+    const double t = (double)((blocks + SLOTS - 1) / SLOTS) * (per + 6) * (blocks <= CUS ? 0.6 : 1.0) + (s > 1 ? 6.0 + 0.5 * s : 0.0);
+    if (t < least) { least = t; best = per; }
+  }
+  return best;
 }
+// X' = a X + B X in 256 x 256 tiles (half the staged bytes per operation) where they alone fill the chip and the reduction is long enough for
+// one block on a CU to hide its ends: 8192 x 2048 fp32 164 us against 183;  8 x 512 x 4608 bf16 (8 stages) 70 us against 44.
+inline bool large_apply(int rows, int cols, long long batch) { return min(rows, cols) >= 1024 && full(rows, cols, 256) * batch >= CUS; }
 
-template <int PROD, int KIND, bool MUON>
+template <int PROD, int KIND, int BT, int NST, bool MUON, bool JOIN>
 int launch_product(const NsArgs& a, int blocks, int flip, float alpha, float beta, hipStream_t st) {
+  if (blocks == 0) return 0;
   static SmemAttrOnce once;
-  auto* fn = &ns_product_kernel<PROD, KIND, BT, MUON>;
-  const int smem = gt::Tile<BT, BT>::SMEM;
+  auto* fn = &ns_product_kernel<PROD, KIND, BT, NST, MUON, JOIN>;
+  const int smem = gt::Tile<BT, BT, NST>::SMEM;
   const int rc = once.ensure(reinterpret_cast<const void*>(fn), smem);
   if (rc != 0) return rc;
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_product_kernel<PROD, KIND, BT, MUON>), dim3(blocks), dim3(256), smem, st, a, flip, alpha, beta);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_product_kernel<PROD, KIND, BT, NST, MUON, JOIN>), dim3(blocks), dim3(256), smem, st, a, flip, alpha, beta);
   return (int)hipGetLastError();
 }
 
-// blocks[4]: norm, init, triangle, full;  maps[4] likewise (null for a plain call)
+// Launches: 0 norm, 1 init, 2 gram, 3 square, 4 joining gram, 5 joining square, 6 apply in 128 x 128, 7 apply in 256 x 256 tiles
+enum { LAUNCHES = 8 };
+
+template <int PROD, int KIND, bool MUON>
+int symmetric(const NsArgs& a, const NsArgs& join, int blocks, int joins, int flip, float alpha, float beta, hipStream_t st) {
+  int rc = blocks <= CUS ? launch_product<PROD, KIND, 128, 4, MUON, false>(a, blocks, flip, alpha, beta, st)
+                         : launch_product<PROD, KIND, 128, 2, MUON, false>(a, blocks, flip, alpha, beta, st);
+  if (rc == 0) rc = launch_product<PROD, KIND, 128, 2, MUON, true>(join, joins, flip, alpha, beta, st);
+  return rc;
+}
+template <int PROD, int KIND, bool MUON>
+int apply(const NsArgs& small, const NsArgs& big, int nsmall, int nbig, int flip, float alpha, float beta, hipStream_t st) {
+  int rc = launch_product<PROD, KIND, 256, 2, MUON, false>(big, nbig, flip, alpha, beta, st);
+  if (rc == 0)
+    rc = nsmall <= CUS ? launch_product<PROD, KIND, 128, 4, MUON, false>(small, nsmall, flip, alpha, beta, st)
+                       : launch_product<PROD, KIND, 128, 2, MUON, false>(small, nsmall, flip, alpha, beta, st);
+  return rc;
+}
+
+// blocks of every launch;  maps likewise (null for a plain call: `per` blocks a matrix)
 template <int PROD, bool MUON>
 int run_steps(NsArgs a, const int* blocks, const int2* const* maps, const int* per, int steps, const float* abc, hipStream_t st) {
   auto with = [&](int i) { a.map = maps != nullptr ? maps[i] : nullptr; a.per = per != nullptr ? per[i] : 1; return a; };
   hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_norm_kernel<MUON>), dim3(blocks[0]), dim3(256), 0, st, with(0));
   hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_init_kernel<PROD, MUON>), dim3(blocks[1]), dim3(256), 0, st, with(1));
   int rc = (int)hipGetLastError();
-  if (rc != 0) return rc;
-  for (int s = 0; s < steps; ++s) {
+  for (int s = 0; s < steps && rc == 0; ++s) {
     const float ca = abc[0], cb = abc[1], cc = abc[2];
-    rc = launch_product<PROD, GRAM, MUON>(with(2), blocks[2], s & 1, UNSCALE, 0.f, st);
-    if (rc == 0) rc = launch_product<PROD, SQUARE, MUON>(with(2), blocks[2], s & 1, cc * UNSCALE, cb, st);
-    if (rc != 0) return rc;
-    rc = s + 1 < steps ? launch_product<PROD, APPLY, MUON>(with(3), blocks[3], s & 1, UNSCALE, ca, st)
-                       : launch_product<PROD, FINAL, MUON>(with(3), blocks[3], s & 1, UNSCALE, ca, st);
-    if (rc != 0) return rc;
+    rc = symmetric<PROD, GRAM, MUON>(with(2), with(4), blocks[2], blocks[4], s & 1, UNSCALE, 0.f, st);
+    if (rc == 0) rc = symmetric<PROD, SQUARE, MUON>(with(3), with(5), blocks[3], blocks[5], s & 1, cc * UNSCALE, cb, st);
+    if (rc == 0)
+      rc = s + 1 < steps ? apply<PROD, APPLY, MUON>(with(6), with(7), blocks[6], blocks[7], s & 1, UNSCALE, ca, st)
+                         : apply<PROD, FINAL, MUON>(with(6), with(7), blocks[6], blocks[7], s & 1, UNSCALE, ca, st);
   }
-  return 0;
+  return rc;
 }
+
+// One matrix of `batch` like it, with the stages a block does of its gram and of its square product: its splits and the blocks of every launch.
+struct Shape { int gram_splits, square_splits, blocks[LAUNCHES]; long long slabs; };
+template <int PROD> Shape shape_of(int rows, int cols, long long batch, int gram_chunk, int square_chunk) {
+  const long long n = (long long)rows * cols, slice = slice_of(n);
+  const Lay<PROD> L(rows, cols);
+  const long long pieces = (long long)rows * ((PROD == 3 ? L.ldx / 2 : L.ldx) / 8);
+  const int thin = rows < cols ? rows : cols, wide = rows < cols ? cols : rows, t = tri(thin);
+  Shape h{};
+  auto splits = [](int ks, int chunk) { return (ks + chunk - 1) / chunk; };
+  h.gram_splits = splits(stages(wide, PROD), gram_chunk);
+  h.square_splits = splits(stages(thin, PROD), square_chunk);
+  h.blocks[0] = (int)((n + slice - 1) / slice);
+  h.blocks[1] = (int)((pieces + INIT_CHUNKS - 1) / INIT_CHUNKS);
+  h.blocks[2] = t * h.gram_splits;
+  h.blocks[3] = t * h.square_splits;
+  h.blocks[4] = h.gram_splits > 1 ? t * gt::Tile<128, 128>::FM : 0;
+  h.blocks[5] = h.square_splits > 1 ? t * gt::Tile<128, 128>::FM : 0;
+  const bool big = large_apply(rows, cols, batch);
+  h.blocks[6] = big ? 0 : full(rows, cols, 128);
+  h.blocks[7] = big ? full(rows, cols, 256) : 0;
+  const int most = h.gram_splits > h.square_splits ? h.gram_splits : h.square_splits;
+  h.slabs = most > 1 ? (long long)t * most * SLAB : 0;
+  return h;
+}
+
+Shape shape_of(int rows, int cols, int prod, long long batch, int gram_chunk, int square_chunk) {
+  return prod == 3 ? shape_of<3>(rows, cols, batch, gram_chunk, square_chunk) : shape_of<1>(rows, cols, batch, gram_chunk, square_chunk);
+}
+Shape shape_of_batch(int rows, int cols, int prod, int batch) {
+  const int thin = rows < cols ? rows : cols, wide = rows < cols ? cols : rows;
+  const long long tiles = (long long)batch * tri(thin);
+  return shape_of(rows, cols, prod, batch, chunk_for(tiles, stages(wide, prod)), chunk_for(tiles, stages(thin, prod)));
+}
+// Sets of different matrices: a block does at most a 1024th of all stages (two rounds of blocks, the long ones first), and at least 8
+inline int set_chunk(long long work) { const long long c = (work + 2 * SLOTS - 1) / (2 * SLOTS); return c < 8 ? 8 : (int)(c > 1 << 30 ? 1 << 30 : c); }
 
 }  // namespace
 
@@ -418,53 +527,70 @@ extern "C" long long ddl_ns_workspace(int rows, int cols, int prod) {
 
 extern "C" int ddl_ns_max_parts() { return MAX_PARTS; }
 
-// blocks of one matrix in the four launches: norm, init, triangle, full
-extern "C" int ddl_ns_blocks(int rows, int cols, int prod, int* out) {
+// stages of all tiles of a matrix: of its gram and of its square product
+extern "C" long long ddl_ns_work(int rows, int cols, int prod, int square) {
   if (rows <= 0 || cols <= 0 || (prod != 1 && prod != 3)) return -1;
-  const Grids g = prod == 3 ? grids_of<3>(rows, cols) : grids_of<1>(rows, cols);
-  out[0] = g.norm; out[1] = g.init; out[2] = g.tri; out[3] = g.full;
-  return 0;
+  const int thin = rows < cols ? rows : cols, wide = rows < cols ? cols : rows;
+  return (long long)tri(thin) * stages(square ? thin : wide, prod);
+}
+
+// For one of `batch` equal matrices (gram_work 0), or one of a set of matrices with gram_work and square_work stages in all (batch 1): out[0..1]
+// the splits of the gram and of the square product, out[2..9] blocks of every launch; returns the floats of partial tiles it needs.
+extern "C" long long ddl_ns_shape(int rows, int cols, int prod, int batch, long long gram_work, long long square_work, int* out) {
+  if (rows <= 0 || cols <= 0 || batch <= 0 || gram_work < 0 || square_work < 0 || (prod != 1 && prod != 3)) return -1;
+  const Shape h = gram_work == 0 ? shape_of_batch(rows, cols, prod, batch)
+                                 : shape_of(rows, cols, prod, 1, set_chunk(gram_work), set_chunk(square_work));
+  out[0] = h.gram_splits;
+  out[1] = h.square_splits;
+  for (int i = 0; i < LAUNCHES; ++i) out[2 + i] = h.blocks[i];
+  return h.slabs;
 }
 
 extern "C" int ddl_ns_mat_bytes() { return (int)sizeof(NsMat); }
 
-// g, out: [batch][rows][cols], bf16 or fp32;  ws: batch * ddl_ns_workspace fp16;  parts: batch * MAX_PARTS doubles;  abc on the host
-extern "C" int ddl_orthogonalize(const void* g, int is_bf16, void* out, void* ws, double* parts, int batch, int rows, int cols,
+// g, out: [batch][rows][cols], bf16 or fp32;  ws: batch * ddl_ns_workspace fp16;  parts: batch * MAX_PARTS doubles;  slabs: batch times what
+// ddl_ns_shape(.., batch, 0, 0, ..) returns, floats;  abc on the host
+extern "C" int ddl_orthogonalize(const void* g, int is_bf16, void* out, void* ws, double* parts, float* slabs, int batch, int rows, int cols,
                                  int prod, int steps, const float* abc, float eps, void* stream) {
   if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || (prod != 1 && prod != 3)) return -1;
+  const Shape h = shape_of_batch(rows, cols, prod, batch);
   NsArgs a{};
   a.one.rows = rows; a.one.cols = cols;
+  a.one.gram_splits = h.gram_splits; a.one.square_splits = h.square_splits;
   a.g_stride = (long long)rows * cols;
   a.ws_stride = ddl_ns_workspace(rows, cols, prod);
+  a.slab_stride = h.slabs;
   a.ws = (unsigned short*)ws;
+  a.slabs = slabs;
   a.parts = parts;
   a.eps = eps;
   if (is_bf16) { a.g16 = (const bf16_t*)g; a.out16 = (bf16_t*)out; } else { a.g32 = (const float*)g; a.out32 = (float*)out; }
-  int per[4], blocks[4];
-  ddl_ns_blocks(rows, cols, prod, per);
-  for (int i = 0; i < 4; ++i) {
-    if ((long long)per[i] * batch > 0x7fffffffll) return -2;
-    blocks[i] = per[i] * batch;
+  int blocks[LAUNCHES];
+  for (int i = 0; i < LAUNCHES; ++i) {
+    if ((long long)h.blocks[i] * batch > 0x7fffffffll) return -2;
+    blocks[i] = h.blocks[i] * batch;
   }
-  return prod == 3 ? run_steps<3, false>(a, blocks, nullptr, per, steps, abc, (hipStream_t)stream)
-                   : run_steps<1, false>(a, blocks, nullptr, per, steps, abc, (hipStream_t)stream);
+  return prod == 3 ? run_steps<3, false>(a, blocks, nullptr, h.blocks, steps, abc, (hipStream_t)stream)
+                   : run_steps<1, false>(a, blocks, nullptr, h.blocks, steps, abc, (hipStream_t)stream);
 }
 
-// Muon over the matrices of an arena.  table: NsMat[] and maps: int2[] on the device, blocks[4] on the host.
+// Muon over the matrices of an arena.  table: NsMat[], maps: one int2[] after the other for the 8 launches, on the device;  blocks[8] on the host.
 // hyper (device): [0] lr [1] momentum [2] nesterov [4] gradient scale.
-extern "C" int ddl_muon_step(const void* table, const void* map0, const void* map1, const void* map2, const void* map3,
-                             const int* blocks, float* master, float* grad, float* mom, void* shadow, const float* seg_wd,
-                             const float* hyper, void* ws, double* parts, int prod, int steps, const float* abc, float eps,
-                             int zero_grad, void* stream) {
+extern "C" int ddl_muon_step(const void* table, const void* maps, const int* blocks, float* master, float* grad, float* mom, void* shadow,
+                             const float* seg_wd, const float* hyper, void* ws, double* parts, float* slabs, int prod, int steps, const float* abc,
+                             float eps, int zero_grad, void* stream) {
   if (steps <= 0 || (prod != 1 && prod != 3)) return -1;
   NsArgs a{};
   a.table = (const NsMat*)table;
   a.ws = (unsigned short*)ws;
+  a.slabs = slabs;
   a.parts = parts;
   a.eps = eps;
   a.grad = grad; a.mom = mom; a.master = master; a.shadow = (bf16_t*)shadow; a.seg_wd = seg_wd; a.hyper = hyper;
   a.zero_grad = zero_grad;
-  const int2* maps[4] = {(const int2*)map0, (const int2*)map1, (const int2*)map2, (const int2*)map3};
-  return prod == 3 ? run_steps<3, true>(a, blocks, maps, nullptr, steps, abc, (hipStream_t)stream)
-                   : run_steps<1, true>(a, blocks, maps, nullptr, steps, abc, (hipStream_t)stream);
+  const int2* list[LAUNCHES];
+  const int2* at = (const int2*)maps;
+  for (int i = 0; i < LAUNCHES; ++i) { list[i] = at; at += blocks[i]; }
+  return prod == 3 ? run_steps<3, true>(a, blocks, list, nullptr, steps, abc, (hipStream_t)stream)
+                   : run_steps<1, true>(a, blocks, list, nullptr, steps, abc, (hipStream_t)stream);
 }

@@ -104,9 +104,10 @@ _SIGS = {
     "ddl_ns_workspace": [_i, _i, _i],
     "ddl_ns_max_parts": [],
     "ddl_ns_mat_bytes": [],
-    "ddl_ns_blocks": [_i, _i, _i, _vp],
-    "ddl_orthogonalize": [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _f, _vp],
-    "ddl_muon_step": [_vp] * 14 + [_i, _i, _vp, _f, _i, _vp],
+    "ddl_ns_work": [_i, _i, _i, _i],
+    "ddl_ns_shape": [_i, _i, _i, _i, _ll, _ll, _vp],
+    "ddl_orthogonalize": [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _f, _vp],
+    "ddl_muon_step": [_vp] * 12 + [_i, _i, _vp, _f, _i, _vp],
     "ddl_gated_up": [_vp] * 6 + [_i, _i, _i, _i, _vp],
     "ddl_gated_down": [_vp, _vp, _vp, _i, _i, _i, _vp],
     "ddl_gated_dh": [_vp] * 6 + [_i, _i, _i, _vp],
@@ -120,7 +121,7 @@ _SIGS = {
 
 
 _LONG_RESULT = {"ddl_conv_wgrad_plan", "ddl_conv_c64_launches", "ddl_wgrad_halo_launches", "ddl_ns_workspace",
-                "ddl_logprob_workspace"}
+                "ddl_ns_shape", "ddl_ns_work", "ddl_logprob_workspace"}
 
 
 def _load():

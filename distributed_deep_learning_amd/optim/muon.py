@@ -6,7 +6,7 @@ For every weight that is a matrix (convolution filters flattened to ``[out, in *
 
 Everything else (biases, norm parameters, whatever ``use_muon`` declines) is updated by Adam with its own learning rate.
 
-GPU path: ``csrc/ortho.hip``, all matrices of the arena in shared launches (2 + 3 per Newton-Schulz step): the momentum update is fused with
+GPU path: ``csrc/ortho.hip``, all matrices of the arena in shared launches (2, and 3 to 6 for every Newton-Schulz step): the momentum update is fused with
 the sums of squares, the weight update with the last product, and the bf16 shadow and the cleared gradient are written along.
 CPU path: the same mathematics with torch ops.
 """
@@ -79,28 +79,34 @@ class Muon(_ArenaOptimizer):
             self._plan = self._build_plan()
 
     def _build_plan(self):
-        """Device tables of the shared launches: one record per matrix, and for each of the four launch shapes (norm, init, symmetric
-        product, full product) which block works on which part of which matrix."""
+        """Device tables of the shared launches: one record per matrix, and for each launch which block works on which part of which
+        matrix."""
         lib = _lib.require()
         prod = 3 if self.ns_precision == "single" else 1
-        rec = np.dtype([("elem", "<i8"), ("ws", "<i8"), ("rows", "<i4"), ("cols", "<i4"), ("seg", "<i4"), ("scale", "<f4")])
+        rec = np.dtype([("elem", "<i8"), ("ws", "<i8"), ("slab", "<i8"), ("rows", "<i4"), ("cols", "<i4"), ("seg", "<i4"), ("scale", "<f4"),
+                        ("gram_splits", "<i4"), ("square_splits", "<i4")])
         if rec.itemsize != lib.ddl_ns_mat_bytes():
             raise RuntimeError("Muon: matrix record does not match the kernel library")
-        table, maps, ws, out = np.zeros(len(self.matrices), dtype=rec), [[], [], [], []], 0, (C.c_int * 4)()
+        table, launches = np.zeros(len(self.matrices), dtype=rec), [[] for _ in range(8)]
+        ws, slabs, out = 0, 0, (C.c_int * 10)()
+        work = [sum(lib.ddl_ns_work(rows, cols, prod, square) for _, rows, cols, _ in self.matrices) for square in (0, 1)]
         # long reductions first: the blocks that run longest start first
-        order = sorted(range(len(self.matrices)), key=lambda i: -max(self.matrices[i][1], self.matrices[i][2]))
-        for i, (s, rows, cols, scale) in enumerate(self.matrices):
-            table[i] = (s.offset, ws, rows, cols, s.index, scale)
+        for i in sorted(range(len(self.matrices)), key=lambda i: -max(self.matrices[i][1], self.matrices[i][2])):
+            s, rows, cols, scale = self.matrices[i]
+            need = lib.ddl_ns_shape(rows, cols, prod, 1, *work, out)
+            if need < 0:
+                raise RuntimeError(f"Muon: no plan for a {rows} x {cols} matrix")
+            table[i] = (s.offset, ws, slabs, rows, cols, s.index, scale, out[0], out[1])
             ws += lib.ddl_ns_workspace(rows, cols, prod)
-        for i in order:
-            _lib.check(lib.ddl_ns_blocks(self.matrices[i][1], self.matrices[i][2], prod, out), "ns_blocks")
-            for m, n in zip(maps, out):
+            slabs += need
+            for m, n in zip(launches, out[2:10]):
                 m.append(np.stack([np.full(n, i, dtype=np.int32), np.arange(n, dtype=np.int32)], 1))
         dev = self.arena.device
-        maps = [torch.from_numpy(np.ascontiguousarray(np.concatenate(m))).to(dev) for m in maps]
-        return {"table": torch.from_numpy(table.view(np.uint8).copy()).to(dev), "maps": maps, "prod": prod,
-                "blocks": (C.c_int * 4)(*(len(m) for m in maps)), "coef": (C.c_float * 3)(*self.ns_coefficients),
-                "ws": torch.empty(ws, dtype=torch.float16, device=dev),
+        maps = np.concatenate([np.concatenate(m) for m in launches])
+        return {"table": torch.from_numpy(table.view(np.uint8).copy()).to(dev), "maps": torch.from_numpy(np.ascontiguousarray(maps)).to(dev),
+                "blocks": (C.c_int * 8)(*(sum(len(x) for x in m) for m in launches)), "prod": prod,
+                "coef": (C.c_float * 3)(*self.ns_coefficients), "ws": torch.empty(ws, dtype=torch.float16, device=dev),
+                "slabs": torch.empty(max(slabs, 4), dtype=torch.float32, device=dev),
                 "parts": torch.empty(len(self.matrices) * lib.ddl_ns_max_parts(), dtype=torch.float64, device=dev)}
 
     def shard_state(self, ranges, gather=None) -> None:
@@ -127,11 +133,11 @@ class Muon(_ArenaOptimizer):
         st = self.flat_state
         if self._plan is not None:
             p = self._plan
-            _lib.check(lib.ddl_muon_step(p["table"].data_ptr(), *(m.data_ptr() for m in p["maps"]), p["blocks"], a.master.data_ptr(),
-                                         a.grad.data_ptr(), st["momentum"].data_ptr(),
-                                         a.shadow.data_ptr() if a.shadow is not None else None, self.seg_wd.data_ptr(),
-                                         self.hyper.data_ptr(), p["ws"].data_ptr(), p["parts"].data_ptr(), p["prod"], self.ns_steps,
-                                         p["coef"], self.ns_eps, int(zero_grad), _lib.stream_ptr()), "muon_step")
+            _lib.check(lib.ddl_muon_step(p["table"].data_ptr(), p["maps"].data_ptr(), p["blocks"], a.master.data_ptr(), a.grad.data_ptr(),
+                                         st["momentum"].data_ptr(), a.shadow.data_ptr() if a.shadow is not None else None,
+                                         self.seg_wd.data_ptr(), self.hyper.data_ptr(), p["ws"].data_ptr(), p["parts"].data_ptr(),
+                                         p["slabs"].data_ptr(), p["prod"], self.ns_steps, p["coef"], self.ns_eps, int(zero_grad),
+                                         _lib.stream_ptr()), "muon_step")
         if self._adam_seg is not None:
             _lib.check(lib.ddl_flat_adam(a.master.data_ptr(), a.grad.data_ptr(), st["momentum"].data_ptr(),
                                          st["exp_avg_sq"].data_ptr(), a.shadow.data_ptr() if a.shadow is not None else None,

@@ -96,6 +96,19 @@ def test_orthogonalize_keeps_22_bits_of_every_element(n):
 
 
 @gpu
+@pytest.mark.parametrize("name", ["bf16", "fp32"])
+@pytest.mark.parametrize("shape", [(512, 4608), (4608, 520), (8, 512, 2304), (1025, 1100), (4100, 4160), (2056, 8200), (8200, 2050)])
+def test_orthogonalize_split_reductions_and_large_tiles(shape, name):
+    """Against 64 bits on the GPU: reductions shared by blocks, deep staging, 256 x 256 tiles, ragged edges of all of them."""
+    gen = torch.Generator(device="cuda").manual_seed(sum(shape))
+    g = torch.randn(shape, generator=gen, device="cuda").to(DT[name])
+    out, ref = K.orthogonalize(g).double(), _orth64(g)
+    err = torch.linalg.vector_norm(out - ref, dim=(-2, -1)) / torch.linalg.vector_norm(ref, dim=(-2, -1))
+    assert float(err.max()) <= ORTH_TOL[name]
+    assert torch.equal(K.orthogonalize(g).double(), out)                 # split sums are added in a fixed order
+
+
+@gpu
 def test_orthogonalize_zero_nan_strides_and_empty():
     g = _randn(4, 4, 40, 70)
     g[1] = 0.0
