@@ -56,9 +56,13 @@ template <int N> __device__ __forceinline__ void keep24(unsigned short* hi, unsi
     *reinterpret_cast<unsigned*>(lo) = l[0];
   }
 }
-__device__ __forceinline__ void get24(const unsigned short* hi, const unsigned char* lo, float* v) {
-  const u32x4 h = *reinterpret_cast<const u32x4*>(hi);
-  const u32x2 l = *reinterpret_cast<const u32x2*>(lo);
+struct Kept { u32x4 h; u32x2 l; };
+__device__ __forceinline__ Kept load24(const unsigned short* hi, const unsigned char* lo) {
+  return Kept{*reinterpret_cast<const u32x4*>(hi), *reinterpret_cast<const u32x2*>(lo)};
+}
+__device__ __forceinline__ void get24(const Kept& k, float* v) {
+  const u32x4 h = k.h;
+  const u32x2 l = k.l;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const unsigned top = (e & 1) ? h[e / 2] & 0xffff0000u : h[e / 2] << 16;
@@ -178,7 +182,7 @@ __global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_down_kernel(cons
   sa.init(gt::Operand{a.h, a.F, m0, a.M, a.F}, wid, lane);
   sb.init(gt::Operand{a.wd, a.F, n0, a.D, a.F}, wid, lane);
   tile.template mul<gt::Bf16, gt::CONTIG, gt::CONTIG, 1>(sa, sb, (a.F + 63) / 64, smem, wid, lane);
-  tile.template store<false>(smem, wid, lane, [&](int r, int c, const float* v) {
+  tile.template store<false>(smem, wid, lane, gt::NoLoad{}, [&](int r, int c, const float* v, gt::None) {
     r += m0; c += n0;
     if (r < a.M && c < a.D) store8(a.y + (long long)r * a.D + c, v);
   }, [](int, int, float*) {});
@@ -198,14 +202,22 @@ __global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_dh_kernel(const 
   sa.init(gt::Operand{a.dy, a.D, m0, a.M, a.D}, wid, lane);
   sb.init(gt::Operand{a.wd, a.F, n0, a.F, a.D}, wid, lane);
   tile.template mul<gt::Bf16, gt::CONTIG, gt::SLOW, 1>(sa, sb, (a.D + 63) / 64, smem, wid, lane);
-  tile.template store<false>(smem, wid, lane, [&](int r, int c, const float* v) {
+  const long long plane = (long long)a.M * a.F;
+  struct Factors { Kept p, q; };
+  auto load = [&](int r, int c) {
+    r += m0; c += n0;
+    const long long o = (long long)r * a.F + c;
+    Factors k{};
+    if (r < a.M && c < a.F) { k.p = load24(a.keep16 + o, a.keep8 + o); k.q = load24(a.keep16 + plane + o, a.keep8 + plane + o); }
+    return k;
+  };
+  tile.template store<false>(smem, wid, lane, load, [&](int r, int c, const float* v, const Factors& k) {
     r += m0; c += n0;
     if (r >= a.M || c >= a.F) return;
     const long long o = (long long)r * a.F + c;
-    const long long plane = (long long)a.M * a.F;
     float p[8], q[8], dg[8], du[8];
-    get24(a.keep16 + o, a.keep8 + o, p);
-    get24(a.keep16 + plane + o, a.keep8 + plane + o, q);
+    get24(k.p, p);
+    get24(k.q, q);
 #pragma unroll
     for (int e = 0; e < 8; ++e) { dg[e] = v[e] * p[e]; du[e] = v[e] * q[e]; }
     store8(a.dg + o, dg);
@@ -230,7 +242,7 @@ __global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_dx_kernel(const 
   sb.second = a.wu;
   sa.left = sb.left = nk;
   tile.template mul<gt::Bf16, gt::CONTIG, gt::SLOW, 1>(sa, sb, 2 * nk, smem, wid, lane);
-  tile.template store<false>(smem, wid, lane, [&](int r, int c, const float* v) {
+  tile.template store<false>(smem, wid, lane, gt::NoLoad{}, [&](int r, int c, const float* v, gt::None) {
     r += m0; c += n0;
     if (r < a.M && c < a.D) store8(a.dx + (long long)r * a.D + c, v);
   }, [](int, int, float*) {});
@@ -255,17 +267,24 @@ __global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_dw_kernel(const 
   sa.init(gt::Operand{pa, rows, m0, rows, a.M}, wid, lane);
   sb.init(gt::Operand{pb, cols, n0, cols, a.M}, wid, lane);
   tile.template mul<gt::Bf16, gt::SLOW, gt::SLOW, 1>(sa, sb, (a.M + 63) / 64, smem, wid, lane);
-  tile.template store<false>(smem, wid, lane, [&](int r, int c, const float* v) {
+  struct Sum { f32x4 lo, hi; };
+  auto load = [&](int r, int c) {
+    r += m0; c += n0;
+    Sum q{};
+    if (a.accumulate && r < rows && c < cols) {
+      const float* const p = (const float*)out + (long long)r * cols + c;
+      q = Sum{*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 4)};
+    }
+    return q;
+  };
+  tile.template store<false>(smem, wid, lane, load, [&](int r, int c, const float* v, const Sum& q) {
     r += m0; c += n0;
     if (r >= rows || c >= cols) return;
     const long long o = (long long)r * cols + c;
     if (a.accumulate) {
       float* const p = (float*)out + o;
-      f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) { lo[e] += v[e]; hi[e] += v[4 + e]; }
-      *reinterpret_cast<f32x4*>(p) = lo;
-      *reinterpret_cast<f32x4*>(p + 4) = hi;
+      *reinterpret_cast<f32x4*>(p) = f32x4{q.lo[0] + v[0], q.lo[1] + v[1], q.lo[2] + v[2], q.lo[3] + v[3]};
+      *reinterpret_cast<f32x4*>(p + 4) = f32x4{q.hi[0] + v[4], q.hi[1] + v[5], q.hi[2] + v[6], q.hi[3] + v[7]};
     } else {
       store8((unsigned short*)out + o, v);
     }

@@ -31,8 +31,8 @@ namespace gt {
 
 constexpr unsigned OOB = 0xFFFFFFF0u;      // beyond any descriptor: the lane reads zero
 
-// Tied forms (dst == src C, AGPR file) for the large tile, whose loop fills the register file: through the builtin the compiler gives the
-// unrolled products rotating destinations and moves half of the 256 accumulators back at every stage.  The waits for the fragments stay the
+// Tied forms (dst == src C, AGPR file): through the builtin the compiler gives the unrolled products rotating destinations and, for the large
+// tile, moves half of the 256 accumulators back at every stage.  The waits for the fragments stay the
 // compiler's (it sees the operands); nothing else touches the accumulators between settle() before and after the loop.
 struct Bf16 {
   static __device__ __forceinline__ void mfma_tied(const s16x8& a, const s16x8& b, f32x4& c) {
@@ -177,10 +177,14 @@ struct Reader {                                    // fragments of a wave's ROWS
   }
 };
 
+struct None {};                                    // epilogues that read nothing
+struct NoLoad { __device__ __forceinline__ None operator()(int, int) const { return None{}; } };
+
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory"); }
 
-// NST: stages in LDS.  2 (64 KiB for 128 x 128, two blocks on a CU hide each other's latency) or 4 (three stages on their way: for launches
-// of no more blocks than CUs).
+// 128 x 128 with NST = 2 stages: 64 KiB of LDS, two blocks on a CU; with NST = 4: one block, three stages on their way, for launches of no more
+// blocks than CUs.  256 x 256 (NST = 2, 128 KiB, one wave per SIMD, 128 x 128 a wave) asks the L2 -> LDS path, which sits at its ~25 bytes per
+// clock and CU with 128 x 128, for half the bytes per operation.
 template <int BM, int BN, int NST = 2> struct Tile {
   static constexpr int WM = BM / 2, WN = BN / 2;           // rows / columns of a wave
   static constexpr int FM = WM / 16, FN = WN / 16;
@@ -217,186 +221,134 @@ template <int BM, int BN, int NST = 2> struct Tile {
     }
   }
 
-  // acc += product over nk stages.  The stage NST - 1 ahead is requested as soon as every wave has left the one whose place it takes (the
-  // barrier at the top), and lands while those between are multiplied.
+  // acc += product over nk stages.
+  //
+  // A wave reads the fragments of the next half stage between the products of this one (a[0], b[0]: first halves; a[1], b[1]: second), and there
+  // is one barrier per stage, between the halves: behind it every wave has read all of stage t (its second half is in registers) and all
+  // pieces of stage t+1 have landed; stage t+NST is then requested into t's place and the first half of t+1 is read.
   template <class E, int AM, int BMD, int PROD, class SA, class SB>
   __device__ __forceinline__ void mul(SA& sa, SB& sb, int nk, char* smem, int wid, int lane) {
-    if constexpr (BM == 256) {
-      mul_large<E, AM, BMD, PROD>(sa, sb, nk, smem, wid, lane);
-      return;
-    }
+    static_assert(FM == FN && SA::NP == FM && SB::NP == FN, "square tiles of a 2 x 2 block of waves");
+    constexpr int H = FN / 2, PER = SA::NP + SB::NP, BOFF = BM * 128;
     const unsigned lds = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem;
-    constexpr int PER = SA::NP + SB::NP;
     Reader<BM, AM> ra;
     Reader<BN, BMD> rb;
     ra.init(wid & 1, lane);
     rb.init(wid >> 1, lane);
 #pragma unroll
-    for (int q = 0; q < NST - 1; ++q) {
+    for (int q = 0; q < NST; ++q) {                        // behind the end: zeros, so that the counted waits stay uniform
       issue(sa, lds + q * STAGE, wid);
-      issue(sb, lds + q * STAGE + BM * 128, wid);
+      issue(sb, lds + q * STAGE + BOFF, wid);
     }
+    wait_vm<(NST - 1) * PER>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    s16x8 a0[FM], b0[FN], a1[FM], b1[FN], b2[FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) a0[i] = ra.get(smem, i, 0);
+#pragma unroll
+    for (int i = 0; i < FN; ++i) b0[i] = rb.get(smem + BOFF, i, 0);
+    settle();
+    int cur = 0;
     for (int t = 0; t < nk; ++t) {
+      const int nxt = cur + STAGE == SMEM ? 0 : cur + STAGE;
+      const char* const ta = smem + cur;
+      const char* const tb = ta + BOFF;
+      const char* const na = smem + nxt;
+      const char* const nb = na + BOFF;
+      const unsigned refill = lds + (unsigned)cur;
+      // first half: hi x hi of split operands
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        if (i < H) { a1[2 * i] = ra.get(ta, 2 * i, 1); a1[2 * i + 1] = ra.get(ta, 2 * i + 1, 1); }
+        else       { b1[2 * (i - H)] = rb.get(tb, 2 * (i - H), 1); b1[2 * (i - H) + 1] = rb.get(tb, 2 * (i - H) + 1, 1); }
+#pragma unroll
+        for (int j = 0; j < FM; ++j) E::mfma_tied(b0[i], a0[j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       wait_vm<(NST - 2) * PER>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (NST > 2 || t + 1 < nk) {                           // behind the end: zeros, so that the counted waits stay uniform
-        const unsigned nl = lds + (unsigned)(((t + NST - 1) % NST) * STAGE);
-        issue(sa, nl, wid);
-        issue(sb, nl + BM * 128, wid);
+      sa.begin();
+      sb.begin();
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {                       // second half;  split operands: lo x hi
+        if (i < H) {
+          sa.piece(2 * i, refill, wid); sa.piece(2 * i + 1, refill, wid);
+          sb.piece(2 * i, refill + BOFF, wid); sb.piece(2 * i + 1, refill + BOFF, wid);
+          if (PROD == 1) { a0[2 * i] = ra.get(na, 2 * i, 0); a0[2 * i + 1] = ra.get(na, 2 * i + 1, 0); }
+        } else if (PROD == 1) {
+          b0[2 * (i - H)] = rb.get(nb, 2 * (i - H), 0); b0[2 * (i - H) + 1] = rb.get(nb, 2 * (i - H) + 1, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+          if (PROD == 1) E::mfma_tied(b1[i], a1[j], acc[i][j]);
+          else           E::mfma_tied(b1[i], a0[j], acc[i][j]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      const char* ta = smem + (t % NST) * STAGE;
-      const char* tb = ta + BM * 128;
-      s16x8 a0[FM], b0[FN];
+      if (PROD == 3) {
 #pragma unroll
-      for (int j = 0; j < FM; ++j) a0[j] = ra.get(ta, j, 0);
+        for (int i = 0; i < FN; ++i) {                     // hi x lo;  the hi fragments of A are free, those of B are not yet
+          if (i < H) { a0[2 * i] = ra.get(na, 2 * i, 0); a0[2 * i + 1] = ra.get(na, 2 * i + 1, 0); }
+          else       { b2[2 * (i - H)] = rb.get(nb, 2 * (i - H), 0); b2[2 * (i - H) + 1] = rb.get(nb, 2 * (i - H) + 1, 0); }
 #pragma unroll
-      for (int i = 0; i < FN; ++i) b0[i] = rb.get(tb, i, 0);
+          for (int j = 0; j < FM; ++j) E::mfma_tied(b0[i], a1[j], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j) acc[i][j] = E::mfma(b0[i], a0[j], acc[i][j]);
-      s16x8 a1[FM], b1[FN];
-#pragma unroll
-      for (int j = 0; j < FM; ++j) a1[j] = ra.get(ta, j, 1);
-#pragma unroll
-      for (int i = 0; i < FN; ++i) b1[i] = rb.get(tb, i, 1);
-      if (PROD == 1) {
-#pragma unroll
-        for (int i = 0; i < FN; ++i)
-#pragma unroll
-          for (int j = 0; j < FM; ++j) acc[i][j] = E::mfma(b1[i], a1[j], acc[i][j]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < FN; ++i)
-#pragma unroll
-          for (int j = 0; j < FM; ++j) acc[i][j] = E::mfma(b1[i], a0[j], acc[i][j]);
-#pragma unroll
-        for (int i = 0; i < FN; ++i)
-#pragma unroll
-          for (int j = 0; j < FM; ++j) acc[i][j] = E::mfma(b0[i], a1[j], acc[i][j]);
+        for (int i = 0; i < FN; ++i) b0[i] = b2[i];
       }
+      sa.end();
+      sb.end();
+      cur = nxt;
     }
+    settle();
     wait_vm<0>();
     __builtin_amdgcn_s_barrier();                          // every wave has read its last fragments: windows may be written
     asm volatile("" ::: "memory");
   }
 
-  // The same for tiles so large that a CU holds one block (256 x 256: 128 KiB of stages, one wave per SIMD, 128 x 128 a wave).  Nothing but
-  // this wave hides its latencies, so the fragments of the next half stage are read between the products of this one, and the one
-  // barrier per stage sits between the halves:  behind it every wave has read all of stage t (its second half is in registers) and all
-  // pieces of stage t+1 have landed;  stage t+2 is then requested into t's place and t+1's first half read.  256 x 256 asks the
-  // L2 -> LDS path for half the bytes per operation of 128 x 128, which sits at that path's ~25 bytes per clock and CU.
-  template <class E, int AM, int BMD, int PROD, class SA, class SB>
-  __device__ __forceinline__ void mul_large(SA& sa, SB& sb, int nk, char* smem, int wid, int lane) {
-    static_assert(FM == 8 && FN == 8 && SA::NP == 8 && SB::NP == 8, "256 x 256 tiles");
-    const unsigned lds = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem;
-    Reader<BM, AM> ra;
-    Reader<BN, BMD> rb;
-    ra.init(wid & 1, lane);
-    rb.init(wid >> 1, lane);
-    issue(sa, lds, wid);
-    issue(sb, lds + BM * 128, wid);
-    issue(sa, lds + STAGE, wid);
-    issue(sb, lds + STAGE + BM * 128, wid);
-    asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    s16x8 a0[FM], b0[FN], a1[FM], b1[FN], b2[FN];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a0[i] = ra.get(smem, i, 0);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) b0[i] = rb.get(smem + BM * 128, i, 0);
-    settle();
-    for (int t = 0; t < nk; ++t) {
-      const unsigned cur = (unsigned)((t & 1) * STAGE), nxt = STAGE - cur;
-      const char* const ta = smem + cur;
-      const char* const tb = ta + BM * 128;
-      const char* const na = smem + nxt;
-      const char* const nb = na + BM * 128;
-      // first half: hi x hi of split operands
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i < 4) { a1[2 * i] = ra.get(ta, 2 * i, 1); a1[2 * i + 1] = ra.get(ta, 2 * i + 1, 1); }
-        else       { b1[2 * i - 8] = rb.get(tb, 2 * i - 8, 1); b1[2 * i - 7] = rb.get(tb, 2 * i - 7, 1); }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) E::mfma_tied(b0[i], a0[j], acc[i][j]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      sa.begin();
-      sb.begin();
-      if (PROD == 1) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (i < 4) {
-            sa.piece(2 * i, lds + cur, wid); sa.piece(2 * i + 1, lds + cur, wid);
-            sb.piece(2 * i, lds + cur + BM * 128, wid); sb.piece(2 * i + 1, lds + cur + BM * 128, wid);
-            a0[2 * i] = ra.get(na, 2 * i, 0); a0[2 * i + 1] = ra.get(na, 2 * i + 1, 0);
-          } else {
-            b0[2 * i - 8] = rb.get(nb, 2 * i - 8, 0); b0[2 * i - 7] = rb.get(nb, 2 * i - 7, 0);
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) E::mfma_tied(b1[i], a1[j], acc[i][j]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {                      // lo x hi
-          if (i < 4) {
-            sa.piece(2 * i, lds + cur, wid); sa.piece(2 * i + 1, lds + cur, wid);
-            sb.piece(2 * i, lds + cur + BM * 128, wid); sb.piece(2 * i + 1, lds + cur + BM * 128, wid);
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) E::mfma_tied(b1[i], a0[j], acc[i][j]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {                      // hi x lo; the hi fragments of A are free
-          if (i < 4) { a0[2 * i] = ra.get(na, 2 * i, 0); a0[2 * i + 1] = ra.get(na, 2 * i + 1, 0); }
-          else       { b2[2 * i - 8] = rb.get(nb, 2 * i - 8, 0); b2[2 * i - 7] = rb.get(nb, 2 * i - 7, 0); }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) E::mfma_tied(b0[i], a1[j], acc[i][j]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) b0[i] = b2[i];
-      }
-      sa.end();
-      sb.end();
-    }
-    settle();
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-  }
-
-  // Rows of the wave's part, 16 at a time through its own window: f(m, n, v[8]) with tile-relative m and n (n a multiple of 8).
-  // With COLS the window is also walked down its columns: ft(n, m, v[8]), m a multiple of 8 - the transposed tile.
+  // Rows of the wave's part, 16 at a time through its own window: f(m, n, v[8], aux) with tile-relative m and n (n a multiple of 8), where
+  // aux = load(m, n) was requested one row group earlier (what an epilogue reads would otherwise cost a memory latency per group).
+  // With COLS the window gets f's values back and is walked down its columns: ft(n, m, v[8]), m a multiple of 8 - the transposed tile.
   // NJ = 1: the one group that sum_slabs() left, which is group j0 of the tile.
-  template <bool COLS, int NJ = FM, class F, class FT>
-  __device__ __forceinline__ void store(char* smem, int wid, int lane, F&& f, FT&& ft, int j0 = 0) {
+  template <bool COLS, int NJ = FM, class LD, class F, class FT>
+  __device__ __forceinline__ void store(char* smem, int wid, int lane, LD&& load, F&& f, FT&& ft, int j0 = 0) {
+    constexpr int NC = WN / 32;
     float* const win = reinterpret_cast<float*>(smem + wid * WBYTES);
     const int wm0 = (wid & 1) * WM + j0 * 16, wn0 = (wid >> 1) * WN;
+    auto row = [&](int c) { return (c * 64 + lane) / (WN / 8); };
+    auto chunk = [&](int c) { return (c * 64 + lane) % (WN / 8) * 8; };
+    decltype(load(0, 0)) aux[2][NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) aux[0][c] = load(wm0 + row(c), wn0 + chunk(c));
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
+      if (j + 1 < NJ) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) aux[(j + 1) & 1][c] = load(wm0 + (j + 1) * 16 + row(c), wn0 + chunk(c));
+      }
 #pragma unroll
       for (int i = 0; i < FN; ++i)
         *reinterpret_cast<f32x4*>(win + (lane & 15) * WPITCH + i * 16 + (lane >> 4) * 4) = acc[i][j];
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-      for (int c = 0; c < WN / 32; ++c) {
-        const int idx = c * 64 + lane, row = idx / (WN / 8), ch = idx % (WN / 8);
+      for (int c = 0; c < NC; ++c) {
+        float* const at = win + row(c) * WPITCH + chunk(c);
         float v[8];
-        *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(win + row * WPITCH + ch * 8);
-        *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(win + row * WPITCH + ch * 8 + 4);
-        f(wm0 + j * 16 + row, wn0 + ch * 8, v);
+        *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(at);
+        *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(at + 4);
+        f(wm0 + j * 16 + row(c), wn0 + chunk(c), v, aux[j & 1][c]);
+        if (COLS) {
+          *reinterpret_cast<f32x4*>(at) = *reinterpret_cast<const f32x4*>(v);
+          *reinterpret_cast<f32x4*>(at + 4) = *reinterpret_cast<const f32x4*>(v + 4);
+        }
       }
       if (COLS) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-        for (int c = 0; c < WN / 32; ++c) {
+        for (int c = 0; c < NC; ++c) {
           const int idx = c * 64 + lane, col = idx >> 1, half = idx & 1;
           float v[8];
 #pragma unroll

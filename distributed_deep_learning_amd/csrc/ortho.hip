@@ -320,50 +320,61 @@ __global__ __launch_bounds__(256, BT == 256 || NST > 2 ? 1 : 2) void ns_product_
 
   if (KIND <= SQUARE) {
     unsigned short* const dst = KIND == GRAM ? S : B;
-    auto value = [&](int r, int c, float* v) {            // v <- alpha v + beta S(r, c), 8 columns
-      if (KIND == SQUARE) {
-        const unsigned short* q = S + Lay<PROD>::at(r, L.lds, c);
-        const f16x8 h = *reinterpret_cast<const f16x8*>(q);
-        if (PROD == 3) {
-          const f16x8 l = *reinterpret_cast<const f16x8*>(q + 32);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = alpha * v[e] + beta * ((float)h[e] + (float)l[e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = alpha * v[e] + beta * (float)h[e];
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= alpha;
-      }
-    };
     const int ncol = (int)(PROD == 3 ? L.lds / 2 : L.lds);
-    auto put = [&](int r, int c, float* v) {
+    struct Old { f16x8 h, l; };
+    auto load = [&](int r, int c) {                       // S(r, c), 8 columns, for B = beta S + alpha S S
+      Old o{};
+      r += m0; c += n0;
+      if (KIND == SQUARE && r < thin && c < ncol) {
+        const unsigned short* q = S + Lay<PROD>::at(r, L.lds, c);
+        o.h = *reinterpret_cast<const f16x8*>(q);
+        if (PROD == 3) o.l = *reinterpret_cast<const f16x8*>(q + 32);
+      }
+      return o;
+    };
+    auto put = [&](int r, int c, const float* v) {
       if (r >= thin || c >= ncol) return;
-      value(r, c, v);
       unsigned short* q = dst + Lay<PROD>::at(r, L.lds, c);
       if (PROD == 3) split_store8(q, 32, v); else f16_store8(q, v);
+    };
+    auto straight = [&](int r, int c, float* v, const Old& o) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = KIND == SQUARE ? alpha * v[e] + beta * (PROD == 3 ? (float)o.h[e] + (float)o.l[e] : (float)o.h[e]) : alpha * v[e];
+      put(m0 + r, n0 + c, v);
     };
     constexpr int NJ = JOIN ? 1 : T::FM;
     const int j0 = JOIN ? split : 0;
     if (ti != tj)
-      tile.template store<true, NJ>(smem, wid, lane, [&](int r, int c, float* v) { put(m0 + r, n0 + c, v); },
-                                    [&](int r, int c, float* v) { put(n0 + r, m0 + c, v); }, j0);
+      tile.template store<true, NJ>(smem, wid, lane, load, straight, [&](int r, int c, const float* v) { put(n0 + r, m0 + c, v); }, j0);
     else
-      tile.template store<false, NJ>(smem, wid, lane, [&](int r, int c, float* v) { put(m0 + r, n0 + c, v); }, [](int, int, float*) {}, j0);
+      tile.template store<false, NJ>(smem, wid, lane, load, straight, [](int, int, float*) {}, j0);
   } else {
     unsigned short* const dst = ws + (flip ? L.x0 : L.x1);
     const int ncol = (int)(PROD == 3 ? L.ldx / 2 : L.ldx);
     float lr = 0.f, wd = 0.f;
     if (KIND == FINAL && MUON) { lr = a.hyper[0]; wd = a.seg_wd[m.seg]; }
     const bool wide8 = (m.cols & 7) == 0;
-    tile.template store<false>(smem, wid, lane, [&](int r, int c, float* v) {
+    struct Old { f16x8 h, l; f32x4 w[2]; };
+    auto load = [&](int r, int c) {                       // X(r, c), 8 columns; Muon's last step: the weights too
+      Old q{};
+      r += m0; c += n0;
+      if (r >= m.rows || c >= (KIND == FINAL ? m.cols : ncol)) return q;
+      const long long at = Lay<PROD>::at(r, L.ldx, c);
+      q.h = *reinterpret_cast<const f16x8*>(X + at);
+      q.l = *reinterpret_cast<const f16x8*>(X + at + L.lo);
+      if (KIND == FINAL && MUON && wide8) {
+        const float* const wp = a.master + m.elem + (long long)r * m.cols + c;
+        q.w[0] = *reinterpret_cast<const f32x4*>(wp);
+        q.w[1] = *reinterpret_cast<const f32x4*>(wp + 4);
+      }
+      return q;
+    };
+    tile.template store<false>(smem, wid, lane, load, [&](int r, int c, float* v, const Old& q) {
       r += m0; c += n0;
       if (r >= m.rows || c >= (KIND == FINAL ? m.cols : ncol)) return;
       const long long at = Lay<PROD>::at(r, L.ldx, c);
-      const f16x8 h = *reinterpret_cast<const f16x8*>(X + at), l = *reinterpret_cast<const f16x8*>(X + at + L.lo);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = alpha * v[e] + beta * ((float)h[e] + (float)l[e]);
+      for (int e = 0; e < 8; ++e) v[e] = alpha * v[e] + beta * ((float)q.h[e] + (float)q.l[e]);
       if (KIND == APPLY) { split_store8(dst + at, L.lo, v); return; }
       const long long o = m.elem + (long long)r * m.cols + c;
 #pragma unroll
@@ -372,8 +383,8 @@ __global__ __launch_bounds__(256, BT == 256 || NST > 2 ? 1 : 2) void ns_product_
         float* const wp = a.master + o;
         if (wide8) {
           float w[8];
-          *reinterpret_cast<f32x4*>(w) = *reinterpret_cast<const f32x4*>(wp);
-          *reinterpret_cast<f32x4*>(w + 4) = *reinterpret_cast<const f32x4*>(wp + 4);
+          *reinterpret_cast<f32x4*>(w) = q.w[0];
+          *reinterpret_cast<f32x4*>(w + 4) = q.w[1];
 #pragma unroll
           for (int e = 0; e < 8; ++e) w[e] -= lr * (m.scale * v[e] + wd * w[e]);
           *reinterpret_cast<f32x4*>(wp) = *reinterpret_cast<const f32x4*>(w);
@@ -405,6 +416,227 @@ __global__ __launch_bounds__(256, BT == 256 || NST > 2 ? 1 : 2) void ns_product_
       }
     }, [](int, int, float*) {});
   }
+}
+
+// ---- matrices that fit one CU: thin side <= 128, wide side <= NT * 128.  One block of eight waves does everything in one launch: X stays in
+// registers in fp32 (every lane holds fragments of all NT column tiles in the layout of the products' results), S, B and one tile of X at a
+// time are in LDS as operands.  Such matrices are bound by latency: 17 launches of about 5 us each take longer than all their products.
+// X is taken as [thin][wide] (a tall matrix is read and written transposed).
+template <int PROD> struct Solo {
+  static constexpr int KSTAGES = PROD == 3 ? 4 : 2, BUF = KSTAGES * 16384;      // a 128 x 128 operand
+  static constexpr int SMEM = 2 * BUF;
+  // Byte offset of the elements (row, col .. col + 3) of an operand, for a lane's first fragment; its other fragments are 16 rows (ROWS16 or
+  // SLOW16(j)) and 16 columns (^ COL16) away.  The lo part of split operands is half a row (^ 64) or 32 rows (+ 8192) away.
+  static constexpr int ROWS16 = 2048, COL16 = 32;
+  static __device__ __forceinline__ int contig(int row, int col) {
+    const int st = PROD == 3 ? col >> 5 : col >> 6, c = PROD == 3 ? (col & 31) >> 3 : (col & 63) >> 3;
+    return st * 16384 + row * 128 + ((c ^ ((row >> 1) & 7)) << 4) + (col & 7) * 2;
+  }
+  static __device__ __forceinline__ int slow(int row, int col) {
+    const int st = PROD == 3 ? row >> 5 : row >> 6, r = PROD == 3 ? row & 31 : row & 63;
+    return st * 16384 + r * 256 + (((col >> 3) ^ (((r & 3) << 2) | ((r >> 2) & 3))) << 4) + (col & 7) * 2;
+  }
+  static constexpr int SLOW16(int j) { return PROD == 3 ? (j >> 1) * 16384 + (j & 1) * 4096 : j * 4096; }
+};
+
+template <int PROD> __device__ __forceinline__ void solo_put(char* buf, int off, int lo, const f32x4& v) {
+  f16x4 h, l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float x = v[e];
+    asm("" : "+v"(x));                                                  // one rounding for both parts (split_store8)
+    h[e] = (_Float16)x;
+    l[e] = (_Float16)(x - (float)h[e]);
+  }
+  *reinterpret_cast<f16x4*>(buf + off) = h;
+  if (PROD == 3) *reinterpret_cast<f16x4*>(buf + lo) = l;
+}
+
+template <int PROD, int NT, bool MUON>
+__global__ __launch_bounds__(512, 2) void ns_solo_kernel(const NsArgs a, const int steps, const float ca, const float cb, const float cc) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ double red[8];
+  using L = Solo<PROD>;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wid & 1, wn = wid >> 1;                                // 64 rows x 32 columns of a tile: 4 x 2 fragments
+  int mat, idx;
+  const NsMat m = locate(a, blockIdx.x, mat, idx);
+  const bool tall = m.rows > m.cols;
+  const int thin = tall ? m.cols : m.rows, wide = tall ? m.rows : m.cols;
+  const int row0 = wm * 64 + (lane & 15), col0 = wn * 32 + (lane >> 4) * 4;
+  auto at = [&](int r, int c) { return m.elem + (tall ? (long long)c * m.cols + r : (long long)r * m.cols + c); };
+  float mu = 0.f, nest = 0.f, gs = 1.f;
+  if (MUON) { mu = a.hyper[1]; nest = a.hyper[2]; gs = a.hyper[4]; }
+
+  f32x4 x[NT][4][2];
+  double sq = 0.0;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = row0 + j * 16, c = t * 128 + col0 + i * 16;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float v = 0.f;
+          if (r < thin && c + e < wide) {
+            const long long o = at(r, c + e);
+            if (MUON) {
+              const float g = gs * a.grad[o], mm = mu * a.mom[o] + g;
+              a.mom[o] = mm;
+              if (a.zero_grad) a.grad[o] = 0.f;
+              v = muon_update(g, mm, mu, nest);
+            } else {
+              v = a.g32 != nullptr ? a.g32[o] : bf16_to_f32(a.g16[o]);
+            }
+          }
+          x[t][j][i][e] = v;
+          sq += (double)v * (double)v;
+        }
+      }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sq += __shfl_xor(sq, o, 64);
+  if (lane == 0) red[wid] = sq;
+  __syncthreads();
+  sq = 0.0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) sq += red[w];
+  const float inv = (float)((double)SCALE / (sqrt(sq) + (double)a.eps));
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) x[t][j][i] *= inv;
+
+  char* const buf0 = smem;
+  char* const buf1 = smem + L::BUF;
+  gt::Reader<128, gt::CONTIG> ra;                                       // 64 rows of the first operand
+  gt::Reader<64, gt::CONTIG> rb;                                        // 32 rows of the second
+  gt::Reader<64, gt::SLOW> rs;
+  ra.init(wm, lane);
+  rb.init(wn, lane);
+  rs.init(wn, lane);
+  f32x4 acc[4][2];
+  auto clear = [&]() {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  };
+  auto mul = [&](const char* pa, const char* pb, auto slow) {
+#pragma unroll 1
+    for (int st = 0; st < L::KSTAGES; ++st, pa += 16384, pb += 16384) {
+      s16x8 fa[4], fb[2][2];
+      auto load_a = [&](int h) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fa[j] = ra.get(pa, j, h);
+      };
+      auto load_b = [&](int h) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) fb[h][i] = decltype(slow)::value ? rs.get(pb, i, h) : rb.get(pb, i, h);
+      };
+      auto go = [&](int h) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j][i] = gt::Fp16::mfma(fb[h][i], fa[j], acc[j][i]);
+      };
+      load_a(0); load_b(0); load_b(1);
+      go(0);
+      if (PROD == 3) go(1);
+      load_a(1);
+      go(PROD == 3 ? 0 : 1);
+    }
+  };
+  const int off_c = L::contig(row0, col0), off_s = L::slow(row0, col0);
+  auto put_contig = [&](char* buf, const f32x4 (*v)[2]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int off = off_c ^ (i * L::COL16);
+        solo_put<PROD>(buf + j * L::ROWS16, off, off ^ 64, v[j][i]);
+      }
+  };
+  auto put_slow = [&](char* buf, const f32x4 (*v)[2]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int off = off_s ^ (i * L::COL16);
+        solo_put<PROD>(buf + L::SLOW16(j), off, off + 8192, v[j][i]);
+      }
+  };
+  struct No { enum { value = 0 }; };
+  struct Yes { enum { value = 1 }; };
+
+  for (int s = 0; s < steps; ++s) {
+    clear();
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {                                      // S = X X^T
+      put_contig(t & 1 ? buf1 : buf0, x[t]);
+      __syncthreads();                                                  // the other buffer's readers passed the previous barrier
+      mul(t & 1 ? buf1 : buf0, t & 1 ? buf1 : buf0, No{});
+    }
+    f32x4 sv[4][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sv[j][i] = acc[j][i] * UNSCALE;
+    char* const bs = NT & 1 ? buf1 : buf0;                              // not read since the last barrier
+    char* const bb = NT & 1 ? buf0 : buf1;
+    put_contig(bs, sv);
+    __syncthreads();
+    clear();
+    mul(bs, bs, No{});                                                  // B = b S + c S S
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sv[j][i] = sv[j][i] * cb + acc[j][i] * (cc * UNSCALE);
+    put_contig(bb, sv);
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {                                      // X = a X + B X
+      put_slow(bs, x[t]);
+      __syncthreads();
+      clear();
+      mul(bb, bs, Yes{});
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x[t][j][i] = x[t][j][i] * ca + acc[j][i] * UNSCALE;
+      __syncthreads();
+    }
+  }
+
+  float lr = 0.f, wd = 0.f;
+  if (MUON) { lr = a.hyper[0]; wd = a.seg_wd[m.seg]; }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = row0 + j * 16, c = t * 128 + col0 + i * 16;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (r < thin && c + e < wide) {
+            const long long o = at(r, c + e);
+            const float v = x[t][j][i][e] * UNSCALE;
+            if (MUON) {
+              const float w = a.master[o] - lr * (m.scale * v + wd * a.master[o]);
+              a.master[o] = w;
+              if (a.shadow != nullptr) a.shadow[o] = f32_to_bf16(w);
+            } else if (a.out32 != nullptr) {
+              a.out32[o] = v;
+            } else {
+              a.out16[o] = f32_to_bf16(v);
+            }
+          }
+        }
+      }
 }
 
 constexpr int CUS = 256, SLOTS = 2 * CUS;         // two 128 x 128 blocks run on a CU
@@ -461,6 +693,23 @@ int apply(const NsArgs& small, const NsArgs& big, int nsmall, int nbig, int flip
     rc = nsmall <= CUS ? launch_product<PROD, KIND, 128, 4, MUON, false>(small, nsmall, flip, alpha, beta, st)
                        : launch_product<PROD, KIND, 128, 2, MUON, false>(small, nsmall, flip, alpha, beta, st);
   return rc;
+}
+
+// Measured: 64 x 147 bf16 41 us against 92 in 17 launches.  Four tiles (120 x 400 fp32) spill and run 257 us against 150: two at most.
+constexpr int SOLO_TILES = 2;
+inline bool solo(int rows, int cols) { return min(rows, cols) <= 128 && max(rows, cols) <= SOLO_TILES * 128; }
+
+template <int PROD, int NT, bool MUON> int launch_solo_t(const NsArgs& a, int mats, int steps, const float* abc, hipStream_t st) {
+  static SmemAttrOnce once;
+  auto* fn = &ns_solo_kernel<PROD, NT, MUON>;
+  const int smem = Solo<PROD>::SMEM, rc = once.ensure(reinterpret_cast<const void*>(fn), smem);
+  if (rc != 0) return rc;
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_solo_kernel<PROD, NT, MUON>), dim3(mats), dim3(512), smem, st, a, steps, abc[0], abc[1], abc[2]);
+  return (int)hipGetLastError();
+}
+// wide: the widest matrix
+template <int PROD, bool MUON> int launch_solo(const NsArgs& a, int mats, int wide, int steps, const float* abc, hipStream_t st) {
+  return wide <= 128 ? launch_solo_t<PROD, 1, MUON>(a, mats, steps, abc, st) : launch_solo_t<PROD, 2, MUON>(a, mats, steps, abc, st);
 }
 
 // blocks of every launch;  maps likewise (null for a plain call: `per` blocks a matrix)
@@ -525,6 +774,9 @@ extern "C" long long ddl_ns_workspace(int rows, int cols, int prod) {
   return prod == 3 ? Lay<3>(rows, cols).size : Lay<1>(rows, cols).size;
 }
 
+// 1: one block does the whole matrix in one launch, which needs no workspace
+extern "C" int ddl_ns_solo(int rows, int cols) { return rows > 0 && cols > 0 && solo(rows, cols) ? 1 : 0; }
+
 extern "C" int ddl_ns_max_parts() { return MAX_PARTS; }
 
 // stages of all tiles of a matrix: of its gram and of its square product
@@ -565,6 +817,12 @@ extern "C" int ddl_orthogonalize(const void* g, int is_bf16, void* out, void* ws
   a.parts = parts;
   a.eps = eps;
   if (is_bf16) { a.g16 = (const bf16_t*)g; a.out16 = (bf16_t*)out; } else { a.g32 = (const float*)g; a.out32 = (float*)out; }
+  if (solo(rows, cols)) {
+    a.per = 1;
+    const int wide = max(rows, cols);
+    return prod == 3 ? launch_solo<3, false>(a, batch, wide, steps, abc, (hipStream_t)stream)
+                     : launch_solo<1, false>(a, batch, wide, steps, abc, (hipStream_t)stream);
+  }
   int blocks[LAUNCHES];
   for (int i = 0; i < LAUNCHES; ++i) {
     if ((long long)h.blocks[i] * batch > 0x7fffffffll) return -2;
@@ -575,10 +833,11 @@ extern "C" int ddl_orthogonalize(const void* g, int is_bf16, void* out, void* ws
 }
 
 // Muon over the matrices of an arena.  table: NsMat[], maps: one int2[] after the other for the 8 launches, on the device;  blocks[8] on the host.
-// hyper (device): [0] lr [1] momentum [2] nesterov [4] gradient scale.
+// hyper (device): [0] lr [1] momentum [2] nesterov [4] gradient scale.  solo_wide > 0: every matrix is a ddl_ns_solo one, the widest has this many
+// columns (rows, if tall), blocks[0] is the number of matrices and maps[] names each once.
 extern "C" int ddl_muon_step(const void* table, const void* maps, const int* blocks, float* master, float* grad, float* mom, void* shadow,
                              const float* seg_wd, const float* hyper, void* ws, double* parts, float* slabs, int prod, int steps, const float* abc,
-                             float eps, int zero_grad, void* stream) {
+                             float eps, int zero_grad, int solo_wide, void* stream) {
   if (steps <= 0 || (prod != 1 && prod != 3)) return -1;
   NsArgs a{};
   a.table = (const NsMat*)table;
@@ -588,6 +847,11 @@ extern "C" int ddl_muon_step(const void* table, const void* maps, const int* blo
   a.eps = eps;
   a.grad = grad; a.mom = mom; a.master = master; a.shadow = (bf16_t*)shadow; a.seg_wd = seg_wd; a.hyper = hyper;
   a.zero_grad = zero_grad;
+  if (solo_wide > 0) {
+    a.map = (const int2*)maps;
+    return prod == 3 ? launch_solo<3, true>(a, blocks[0], solo_wide, steps, abc, (hipStream_t)stream)
+                     : launch_solo<1, true>(a, blocks[0], solo_wide, steps, abc, (hipStream_t)stream);
+  }
   const int2* list[LAUNCHES];
   const int2* at = (const int2*)maps;
   for (int i = 0; i < LAUNCHES; ++i) { list[i] = at; at += blocks[i]; }

@@ -1372,10 +1372,12 @@ def orthogonalize(g: torch.Tensor, steps: int = NS_STEPS, coefficients=NS_COEFFI
     is16 = g.dtype == BF16
     prod = 1 if is16 else 3
     out = torch.empty_like(g)
-    slabs = lib.ddl_ns_shape(rows, cols, prod, batch, 0, 0, (C.c_int * 10)())
-    slabs = torch.empty(batch * slabs, dtype=torch.float32, device=g.device) if slabs else None
-    ws = torch.empty(batch * lib.ddl_ns_workspace(rows, cols, prod), dtype=torch.float16, device=g.device)
-    parts = torch.empty(batch * lib.ddl_ns_max_parts(), dtype=torch.float64, device=g.device)
+    ws = parts = slabs = None
+    if not lib.ddl_ns_solo(rows, cols):
+        slabs = lib.ddl_ns_shape(rows, cols, prod, batch, 0, 0, (C.c_int * 10)())
+        slabs = torch.empty(batch * slabs, dtype=torch.float32, device=g.device) if slabs else None
+        ws = torch.empty(batch * lib.ddl_ns_workspace(rows, cols, prod), dtype=torch.float16, device=g.device)
+        parts = torch.empty(batch * lib.ddl_ns_max_parts(), dtype=torch.float64, device=g.device)
     check(lib.ddl_orthogonalize(ptr(g), int(is16), ptr(out), ptr(ws), ptr(parts), ptr(slabs), batch, rows, cols, prod, int(steps),
                                 (C.c_float * 3)(a, b, c), float(eps), stream_ptr()), "orthogonalize")
     return out

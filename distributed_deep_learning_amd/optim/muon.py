@@ -6,7 +6,8 @@ For every weight that is a matrix (convolution filters flattened to ``[out, in *
 
 Everything else (biases, norm parameters, whatever ``use_muon`` declines) is updated by Adam with its own learning rate.
 
-GPU path: ``csrc/ortho.hip``, all matrices of the arena in shared launches (2, and 3 to 6 for every Newton-Schulz step): the momentum update is fused with
+GPU path: ``csrc/ortho.hip``, all matrices of the arena in shared launches (2, and 3 to 6 for every Newton-Schulz step; one in all when
+every matrix fits a CU): the momentum update is fused with
 the sums of squares, the weight update with the last product, and the bf16 shadow and the cleared gradient are written along.
 CPU path: the same mathematics with torch ops.
 """
@@ -89,6 +90,7 @@ class Muon(_ArenaOptimizer):
             raise RuntimeError("Muon: matrix record does not match the kernel library")
         table, launches = np.zeros(len(self.matrices), dtype=rec), [[] for _ in range(8)]
         ws, slabs, out = 0, 0, (C.c_int * 10)()
+        solo = all(lib.ddl_ns_solo(rows, cols) for _, rows, cols, _ in self.matrices)        # every matrix fits a CU: one launch for all
         work = [sum(lib.ddl_ns_work(rows, cols, prod, square) for _, rows, cols, _ in self.matrices) for square in (0, 1)]
         # long reductions first: the blocks that run longest start first
         for i in sorted(range(len(self.matrices)), key=lambda i: -max(self.matrices[i][1], self.matrices[i][2])):
@@ -97,15 +99,16 @@ class Muon(_ArenaOptimizer):
             if need < 0:
                 raise RuntimeError(f"Muon: no plan for a {rows} x {cols} matrix")
             table[i] = (s.offset, ws, slabs, rows, cols, s.index, scale, out[0], out[1])
-            ws += lib.ddl_ns_workspace(rows, cols, prod)
-            slabs += need
-            for m, n in zip(launches, out[2:10]):
+            if not solo:
+                ws += lib.ddl_ns_workspace(rows, cols, prod)
+                slabs += need
+            for m, n in zip(launches, [1] + [0] * 7 if solo else out[2:10]):
                 m.append(np.stack([np.full(n, i, dtype=np.int32), np.arange(n, dtype=np.int32)], 1))
         dev = self.arena.device
         maps = np.concatenate([np.concatenate(m) for m in launches])
         return {"table": torch.from_numpy(table.view(np.uint8).copy()).to(dev), "maps": torch.from_numpy(np.ascontiguousarray(maps)).to(dev),
                 "blocks": (C.c_int * 8)(*(sum(len(x) for x in m) for m in launches)), "prod": prod,
-                "coef": (C.c_float * 3)(*self.ns_coefficients), "ws": torch.empty(ws, dtype=torch.float16, device=dev),
+                "solo": max(max(rows, cols) for _, rows, cols, _ in self.matrices) if solo else 0, "coef": (C.c_float * 3)(*self.ns_coefficients), "ws": torch.empty(max(ws, 8), dtype=torch.float16, device=dev),
                 "slabs": torch.empty(max(slabs, 4), dtype=torch.float32, device=dev),
                 "parts": torch.empty(len(self.matrices) * lib.ddl_ns_max_parts(), dtype=torch.float64, device=dev)}
 
@@ -137,7 +140,7 @@ class Muon(_ArenaOptimizer):
                                          st["momentum"].data_ptr(), a.shadow.data_ptr() if a.shadow is not None else None,
                                          self.seg_wd.data_ptr(), self.hyper.data_ptr(), p["ws"].data_ptr(), p["parts"].data_ptr(),
                                          p["slabs"].data_ptr(), p["prod"], self.ns_steps, p["coef"], self.ns_eps, int(zero_grad),
-                                         _lib.stream_ptr()), "muon_step")
+                                         p["solo"], _lib.stream_ptr()), "muon_step")
         if self._adam_seg is not None:
             _lib.check(lib.ddl_flat_adam(a.master.data_ptr(), a.grad.data_ptr(), st["momentum"].data_ptr(),
                                          st["exp_avg_sq"].data_ptr(), a.shadow.data_ptr() if a.shadow is not None else None,

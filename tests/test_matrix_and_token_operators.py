@@ -64,7 +64,8 @@ def _orth_close(out, g, name, rank=None):
 @gpu
 @pytest.mark.parametrize("name", ["bf16", "fp32"])
 @pytest.mark.parametrize("shape", [(1, 1), (1, 7), (9, 1), (3, 5), (64, 147), (147, 64), (128, 128), (129, 127), (200, 1000), (1000, 136),
-                                   (130, 4100), (3, 65, 70), (2, 300, 129), (5, 32, 32)])
+                                   (130, 4100), (3, 65, 70), (2, 300, 129), (5, 32, 32), (6, 25), (120, 400), (128, 512), (512, 128), (3, 257, 100), (128, 513),
+                                   (129, 512)])
 def test_orthogonalize_matches_64_bits(shape, name):
     g = (_randn(sum(shape), *shape) * 1e-3).to(DT[name])
     out = K.orthogonalize(g.cuda())
@@ -253,6 +254,25 @@ def test_muon_refusals_and_state():
     twin = Muon(ParamArena(tnn.Sequential(tnn.Linear(8, 16), tnn.Linear(16, 4)).named_parameters()))
     twin.load_state_dict(opt.state_dict())
     assert torch.equal(twin.flat_state["momentum"], opt.flat_state["momentum"]) and twin.state_of(twin.arena.params[0], "momentum").shape == (16, 8)
+
+
+@gpu
+@pytest.mark.parametrize("shapes", [[(6, 25), (120, 400), (16, 1, 5, 5), (9,)], [(6, 25), (130, 400), (300, 40)], [(700, 650), (5, 4)]])
+def test_muon_same_result_in_one_and_in_many_launches(shapes):
+    """Sets whose matrices all fit a CU take one launch, others the shared launches; either way zero_grad=False leaves the gradients."""
+    params = [torch.nn.Parameter(_randn(i, *s).cuda()) for i, s in enumerate(shapes)]
+    opt = Muon([(f"p{i}", p) for i, p in enumerate(params)], lr=0.1, momentum=0.9, adam_lr=0.1)
+    for i, p in enumerate(params):
+        p.grad.copy_(_randn(50 + i, *p.shape))
+    before = [p.detach().cpu().double() for p in params]
+    opt.step(zero_grad=False)
+    for i, (p, b) in enumerate(zip(params, before)):
+        g = _randn(50 + i, *p.shape)
+        assert torch.equal(p.grad.cpu(), g)
+        if p.dim() > 1:
+            rows, cols = p.shape[0], p.numel() // p.shape[0]
+            ref = b - 0.1 * max(1.0, rows / cols) ** 0.5 * _orth64(1.9 * g.reshape(rows, cols)).reshape(p.shape)
+            assert float((p.detach().cpu().double() - ref).norm()) <= 0.1 * max(1.0, rows / cols) ** 0.5 * ORTH_TOL["fp32"] * min(rows, cols) ** 0.5 * 1.2 + 8 * H24 * float(ref.norm())
 
 
 def test_muon_use_muon_chooses():
