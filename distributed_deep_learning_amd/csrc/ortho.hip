@@ -5,6 +5,12 @@
 // computed, half mirrored: m^2 n) + 2 m^3 (S S, likewise m^3) + 2 m^2 n operations, m the thin side: all of it matrix products,
 // run on the tiles of gemm_tile.h.  A tall X is never transposed: its gram matrix takes both operands K-slow, its update is X B.
 //
+// Chains.  All factors P_i = a I + b S_i + c S_i S_i are polynomials of the first S and commute, and S_(i+1) = P_i S_i P_i, so up to three
+// steps can be taken on m x m matrices before X is touched again:  X <- (P_2 P_1 P_0) X.  Five steps then cost 6 m^2 n + 14 m^3 (3 + 2 steps)
+// instead of 15 m^2 n + 5 m^3.  What the first S has lost of a small singular value is not found again inside a chain; with 22-bit
+// operands chains of three leave the result as exact as single steps (a chain of five does not: 1e-4 on a spectrum that falls like 1/k^2),
+// with 11-bit operands they do not, so PROD = 1 takes single steps.  Chosen for wide matrices (use_chains below).
+//
 // Numbers.  The polynomial has slope a = 3.4 at zero, so five steps amplify what a rounding leaves in a small singular direction
 // by up to a^5 = 485.  Therefore
 //   * all values are scaled by 2^12 and held in fp16, whose 11 bits cost the same matrix rate as bf16's 8: the entries of X, S
@@ -59,18 +65,21 @@ __host__ __device__ constexpr long long up(long long n, long long m) { return (n
 // Layout of one matrix's workspace (fp16 elements).  PROD 1: X is a hi plane and a lo plane of [rows][ld], S and B are hi planes.
 // PROD 3: rows of interleaved groups (32 hi, 32 lo).
 template <int PROD> struct Lay {
-  long long ldx, lds, x0, x1, s, b, size, lo;    // lo: distance from a hi value to its lo value
+  enum { MATS = PROD == 3 ? 5 : 2 };             // m x m matrices: S, P (or B = P - a I); chains also T = P S and two for the product of the P
+  long long ldx, lds, x0, x1, s, size, lo;       // lo: distance from a hi value to its lo value
+  long long mat;                                 // size of an m x m matrix, S the first
   __host__ __device__ Lay(int rows, int cols) {
     const int thin = rows < cols ? rows : cols;
     if (PROD == 3) {
       ldx = 2 * up(cols, 32); lds = 2 * up(thin, 32);
-      x0 = 0; x1 = (long long)rows * ldx; s = 2 * x1; b = s + (long long)thin * lds; size = up(b + (long long)thin * lds, 64);
+      x0 = 0; x1 = (long long)rows * ldx; s = 2 * x1;
       lo = 32;
     } else {
       ldx = up(cols, 64); lds = up(thin, 64);
-      x0 = 0; lo = (long long)rows * ldx; x1 = 2 * lo; s = 4 * lo; b = s + (long long)thin * lds;
-      size = up(b + (long long)thin * lds, 64);
+      x0 = 0; lo = (long long)rows * ldx; x1 = 2 * lo; s = 4 * lo;
     }
+    mat = (long long)thin * lds;
+    size = s + MATS * mat;
   }
   __host__ __device__ static long long at(long long row, long long ld, int col) {
     return PROD == 3 ? row * ld + (col >> 5) * 64 + (col & 31) : row * ld + col;
@@ -245,14 +254,19 @@ __global__ __launch_bounds__(256) void ns_init_kernel(const NsArgs a) {
   }
 }
 
-// ---- the products.  KIND 0: S = X X^T;  1: B = b S + c S S;  2: X' = a X + B X;  3: the same, last step, to the destination.
+// ---- the products.  KIND 0: S = X X^T;  1: an m x m product;  2: X' = beta X + F X;  3: the same, last step, to the destination.
+enum { MAT_S = 0, MAT_P = 1, MAT_T = 2, MAT_Q = 3, MAT_R = 4 };
+struct Op {
+  int a, b, dst;                                 // SQUARE: mats[dst] = alpha mats[a] mats[b] + beta mats[a] + diag I;  APPLY: F = mats[a]
+  int flip;                                      // X is in the second of its two places
+  float alpha, beta, diag;
+};
 enum { GRAM = 0, SQUARE = 1, APPLY = 2, FINAL = 3 };
 
 // A tile's reduction may be shared by several blocks (few tiles, long reductions: the gram matrix of a wide X): each leaves its fp32
 // partial tile, and the launch with JOIN adds them in order and does the epilogue.
 template <int PROD, int KIND, int BT, int NST, bool MUON, bool JOIN>
-__global__ __launch_bounds__(256, BT == 256 || NST > 2 ? 1 : 2) void ns_product_kernel(const NsArgs a, const int flip, const float alpha,
-                                                                                        const float beta) {
+__global__ __launch_bounds__(256, BT == 256 || NST > 2 ? 1 : 2) void ns_product_kernel(const NsArgs a, const Op op) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   int mat, idx;
@@ -261,9 +275,9 @@ __global__ __launch_bounds__(256, BT == 256 || NST > 2 ? 1 : 2) void ns_product_
   const bool tall = m.rows > m.cols;
   const int thin = tall ? m.cols : m.rows;
   unsigned short* const ws = a.ws + m.ws;
-  unsigned short* const X = ws + (flip ? L.x1 : L.x0);
-  unsigned short* const S = ws + L.s;
-  unsigned short* const B = ws + L.b;
+  unsigned short* const X = ws + (op.flip ? L.x1 : L.x0);
+  unsigned short* const A = ws + L.s + op.a * L.mat;
+  unsigned short* const B = ws + L.s + op.b * L.mat;
 
   using T = gt::Tile<BT, BT, NST>;
   int ti, tj, split = 0, splits = 1, which = 0;
@@ -310,23 +324,23 @@ __global__ __launch_bounds__(256, BT == 256 || NST > 2 ? 1 : 2) void ns_product_
       if (tall) run(W{}, W{}, X, L.ldx, m.cols, X, L.ldx, m.cols, m.rows);
       else      run(C{}, C{}, X, L.ldx, m.rows, X, L.ldx, m.rows, m.cols);
     } else if (KIND == SQUARE) {
-      run(C{}, C{}, S, L.lds, thin, S, L.lds, thin, thin);
+      run(C{}, C{}, A, L.lds, thin, B, L.lds, thin, thin);
     } else {
-      if (tall) run(C{}, C{}, X, L.ldx, m.rows, B, L.lds, thin, thin);
-      else      run(C{}, W{}, B, L.lds, thin, X, L.ldx, m.cols, thin);
+      if (tall) run(C{}, C{}, X, L.ldx, m.rows, A, L.lds, thin, thin);
+      else      run(C{}, W{}, A, L.lds, thin, X, L.ldx, m.cols, thin);
     }
     if (KIND <= SQUARE && splits > 1) { tile.put_slab(slab + (long long)split * T::SLAB, tid); return; }
   }
 
   if (KIND <= SQUARE) {
-    unsigned short* const dst = KIND == GRAM ? S : B;
+    unsigned short* const dst = ws + L.s + op.dst * L.mat;
     const int ncol = (int)(PROD == 3 ? L.lds / 2 : L.lds);
     struct Old { f16x8 h, l; };
-    auto load = [&](int r, int c) {                       // S(r, c), 8 columns, for B = beta S + alpha S S
+    auto load = [&](int r, int c) {                       // A(r, c), 8 columns
       Old o{};
       r += m0; c += n0;
-      if (KIND == SQUARE && r < thin && c < ncol) {
-        const unsigned short* q = S + Lay<PROD>::at(r, L.lds, c);
+      if (KIND == SQUARE && op.beta != 0.f && r < thin && c < ncol) {
+        const unsigned short* q = A + Lay<PROD>::at(r, L.lds, c);
         o.h = *reinterpret_cast<const f16x8*>(q);
         if (PROD == 3) o.l = *reinterpret_cast<const f16x8*>(q + 32);
       }
@@ -339,7 +353,10 @@ __global__ __launch_bounds__(256, BT == 256 || NST > 2 ? 1 : 2) void ns_product_
     };
     auto straight = [&](int r, int c, float* v, const Old& o) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = KIND == SQUARE ? alpha * v[e] + beta * (PROD == 3 ? (float)o.h[e] + (float)o.l[e] : (float)o.h[e]) : alpha * v[e];
+      for (int e = 0; e < 8; ++e) {
+        v[e] *= op.alpha;
+        if (KIND == SQUARE) v[e] += op.beta * (PROD == 3 ? (float)o.h[e] + (float)o.l[e] : (float)o.h[e]) + (m0 + r == n0 + c + e ? op.diag : 0.f);
+      }
       put(m0 + r, n0 + c, v);
     };
     constexpr int NJ = JOIN ? 1 : T::FM;
@@ -349,7 +366,7 @@ __global__ __launch_bounds__(256, BT == 256 || NST > 2 ? 1 : 2) void ns_product_
     else
       tile.template store<false, NJ>(smem, wid, lane, load, straight, [](int, int, float*) {}, j0);
   } else {
-    unsigned short* const dst = ws + (flip ? L.x0 : L.x1);
+    unsigned short* const dst = ws + (op.flip ? L.x0 : L.x1);
     const int ncol = (int)(PROD == 3 ? L.ldx / 2 : L.ldx);
     float lr = 0.f, wd = 0.f;
     if (KIND == FINAL && MUON) { lr = a.hyper[0]; wd = a.seg_wd[m.seg]; }
@@ -360,8 +377,10 @@ __global__ __launch_bounds__(256, BT == 256 || NST > 2 ? 1 : 2) void ns_product_
       r += m0; c += n0;
       if (r >= m.rows || c >= (KIND == FINAL ? m.cols : ncol)) return q;
       const long long at = Lay<PROD>::at(r, L.ldx, c);
-      q.h = *reinterpret_cast<const f16x8*>(X + at);
-      q.l = *reinterpret_cast<const f16x8*>(X + at + L.lo);
+      if (op.beta != 0.f) {
+        q.h = *reinterpret_cast<const f16x8*>(X + at);
+        q.l = *reinterpret_cast<const f16x8*>(X + at + L.lo);
+      }
       if (KIND == FINAL && MUON && wide8) {
         const float* const wp = a.master + m.elem + (long long)r * m.cols + c;
         q.w[0] = *reinterpret_cast<const f32x4*>(wp);
@@ -374,7 +393,7 @@ __global__ __launch_bounds__(256, BT == 256 || NST > 2 ? 1 : 2) void ns_product_
       if (r >= m.rows || c >= (KIND == FINAL ? m.cols : ncol)) return;
       const long long at = Lay<PROD>::at(r, L.ldx, c);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = alpha * v[e] + beta * ((float)q.h[e] + (float)q.l[e]);
+      for (int e = 0; e < 8; ++e) v[e] = op.alpha * v[e] + op.beta * ((float)q.h[e] + (float)q.l[e]);
       if (KIND == APPLY) { split_store8(dst + at, L.lo, v); return; }
       const long long o = m.elem + (long long)r * m.cols + c;
 #pragma unroll
@@ -665,14 +684,14 @@ inline int chunk_for(long long tiles, int ks) {
 inline bool large_apply(int rows, int cols, long long batch) { return min(rows, cols) >= 1024 && full(rows, cols, 256) * batch >= CUS; }
 
 template <int PROD, int KIND, int BT, int NST, bool MUON, bool JOIN>
-int launch_product(const NsArgs& a, int blocks, int flip, float alpha, float beta, hipStream_t st) {
+int launch_product(const NsArgs& a, int blocks, const Op& op, hipStream_t st) {
   if (blocks == 0) return 0;
   static SmemAttrOnce once;
   auto* fn = &ns_product_kernel<PROD, KIND, BT, NST, MUON, JOIN>;
   const int smem = gt::Tile<BT, BT, NST>::SMEM;
   const int rc = once.ensure(reinterpret_cast<const void*>(fn), smem);
   if (rc != 0) return rc;
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_product_kernel<PROD, KIND, BT, NST, MUON, JOIN>), dim3(blocks), dim3(256), smem, st, a, flip, alpha, beta);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_product_kernel<PROD, KIND, BT, NST, MUON, JOIN>), dim3(blocks), dim3(256), smem, st, a, op);
   return (int)hipGetLastError();
 }
 
@@ -680,20 +699,42 @@ int launch_product(const NsArgs& a, int blocks, int flip, float alpha, float bet
 enum { LAUNCHES = 8 };
 
 template <int PROD, int KIND, bool MUON>
-int symmetric(const NsArgs& a, const NsArgs& join, int blocks, int joins, int flip, float alpha, float beta, hipStream_t st) {
-  int rc = blocks <= CUS ? launch_product<PROD, KIND, 128, 4, MUON, false>(a, blocks, flip, alpha, beta, st)
-                         : launch_product<PROD, KIND, 128, 2, MUON, false>(a, blocks, flip, alpha, beta, st);
-  if (rc == 0) rc = launch_product<PROD, KIND, 128, 2, MUON, true>(join, joins, flip, alpha, beta, st);
+int symmetric(const NsArgs& a, const NsArgs& join, int blocks, int joins, const Op& op, hipStream_t st) {
+  int rc = blocks <= CUS ? launch_product<PROD, KIND, 128, 4, MUON, false>(a, blocks, op, st)
+                         : launch_product<PROD, KIND, 128, 2, MUON, false>(a, blocks, op, st);
+  if (rc == 0) rc = launch_product<PROD, KIND, 128, 2, MUON, true>(join, joins, op, st);
   return rc;
 }
 template <int PROD, int KIND, bool MUON>
-int apply(const NsArgs& small, const NsArgs& big, int nsmall, int nbig, int flip, float alpha, float beta, hipStream_t st) {
-  int rc = launch_product<PROD, KIND, 256, 2, MUON, false>(big, nbig, flip, alpha, beta, st);
+int apply(const NsArgs& small, const NsArgs& big, int nsmall, int nbig, const Op& op, hipStream_t st) {
+  int rc = launch_product<PROD, KIND, 256, 2, MUON, false>(big, nbig, op, st);
   if (rc == 0)
-    rc = nsmall <= CUS ? launch_product<PROD, KIND, 128, 4, MUON, false>(small, nsmall, flip, alpha, beta, st)
-                       : launch_product<PROD, KIND, 128, 2, MUON, false>(small, nsmall, flip, alpha, beta, st);
+    rc = nsmall <= CUS ? launch_product<PROD, KIND, 128, 4, MUON, false>(small, nsmall, op, st)
+                       : launch_product<PROD, KIND, 128, 2, MUON, false>(small, nsmall, op, st);
   return rc;
 }
+
+// The largest value of |a + b t + c t^2| over squared singular values (which the checked polynomial keeps below 1.6), with a little to spare
+inline float factor_bound(const float* abc) {
+  float f = 0.f;
+  for (int i = 0; i <= 160; ++i) {
+    const float t = 0.01f * (float)i, v = fabsf(abc[0] + abc[1] * t + abc[2] * t * t);
+    f = v > f ? v : f;
+  }
+  return 1.05f * f;
+}
+// Scale of products of up to three factors in fp16 (4096 for the usual matrices): a power of two that keeps them in range.  0: out of range
+inline float chain_scale(const float* abc) {
+  const float f = factor_bound(abc);
+  float q = 4096.f;
+  while (q >= 256.f && f * f * f * q > 60000.f) q *= 0.5f;
+  return f * 4096.f < 60000.f && q >= 256.f ? q : 0.f;
+}
+// A set of matrices: operations in chains (6 m^2 n + 14 m^3 each) against single steps (15 m^2 n + 5 m^3).  Chains are 18 launches instead of 15
+// and their m x m products fill the chip less.
+inline bool use_chains(double chained, double single) { return chained <= 0.8 * single; }
+inline double chained_work(double thin, double wide) { return 6 * thin * thin * wide + 14 * thin * thin * thin; }
+inline double single_work(double thin, double wide) { return 15 * thin * thin * wide + 5 * thin * thin * thin; }
 
 // Measured: 64 x 147 bf16 41 us against 92 in 17 launches.  Four tiles (120 x 400 fp32) spill and run 257 us against 150: two at most.
 constexpr int SOLO_TILES = 2;
@@ -712,20 +753,56 @@ template <int PROD, bool MUON> int launch_solo(const NsArgs& a, int mats, int wi
   return wide <= 128 ? launch_solo_t<PROD, 1, MUON>(a, mats, steps, abc, st) : launch_solo_t<PROD, 2, MUON>(a, mats, steps, abc, st);
 }
 
-// blocks of every launch;  maps likewise (null for a plain call: `per` blocks a matrix)
+// blocks of every launch;  maps likewise (null for a plain call: `per` blocks a matrix);  chains: only with PROD = 3
 template <int PROD, bool MUON>
-int run_steps(NsArgs a, const int* blocks, const int2* const* maps, const int* per, int steps, const float* abc, hipStream_t st) {
+int run_steps(NsArgs a, const int* blocks, const int2* const* maps, const int* per, int steps, const float* abc, bool chains, hipStream_t st) {
   auto with = [&](int i) { a.map = maps != nullptr ? maps[i] : nullptr; a.per = per != nullptr ? per[i] : 1; return a; };
   hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_norm_kernel<MUON>), dim3(blocks[0]), dim3(256), 0, st, with(0));
   hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_init_kernel<PROD, MUON>), dim3(blocks[1]), dim3(256), 0, st, with(1));
   int rc = (int)hipGetLastError();
-  for (int s = 0; s < steps && rc == 0; ++s) {
-    const float ca = abc[0], cb = abc[1], cc = abc[2];
-    rc = symmetric<PROD, GRAM, MUON>(with(2), with(4), blocks[2], blocks[4], s & 1, UNSCALE, 0.f, st);
-    if (rc == 0) rc = symmetric<PROD, SQUARE, MUON>(with(3), with(5), blocks[3], blocks[5], s & 1, cc * UNSCALE, cb, st);
+  const float ca = abc[0], cb = abc[1], cc = abc[2];
+  int flip = 0;
+  auto gram = [&]() {
+    if (rc == 0) rc = symmetric<PROD, GRAM, MUON>(with(2), with(4), blocks[2], blocks[4], Op{0, 0, MAT_S, flip, UNSCALE, 0.f, 0.f}, st);
+  };
+  auto mats = [&](int x, int y, int dst, float alpha, float beta, float diag) {
+    if (rc == 0) rc = symmetric<PROD, SQUARE, MUON>(with(3), with(5), blocks[3], blocks[5], Op{x, y, dst, flip, alpha, beta, diag}, st);
+  };
+  auto applied = [&](int f, float alpha, float beta, bool last) {
+    const Op op{f, f, 0, flip, alpha, beta, 0.f};
     if (rc == 0)
-      rc = s + 1 < steps ? apply<PROD, APPLY, MUON>(with(6), with(7), blocks[6], blocks[7], s & 1, UNSCALE, ca, st)
-                         : apply<PROD, FINAL, MUON>(with(6), with(7), blocks[6], blocks[7], s & 1, UNSCALE, ca, st);
+      rc = last ? apply<PROD, FINAL, MUON>(with(6), with(7), blocks[6], blocks[7], op, st) : apply<PROD, APPLY, MUON>(with(6), with(7), blocks[6], blocks[7], op, st);
+    flip ^= 1;
+  };
+  const float q = chain_scale(abc);
+  if (!chains || q == 0.f) {
+    for (int s = 0; s < steps; ++s) {                     // B = b S + c S S;  X <- a X + B X
+      gram();
+      mats(MAT_S, MAT_S, MAT_P, cc * UNSCALE, cb, 0.f);
+      applied(MAT_P, UNSCALE, ca, s + 1 == steps);
+    }
+    return rc;
+  }
+  for (int done = 0; done < steps;) {
+    const int rest = steps - done, len = rest == 4 ? 2 : rest < 3 ? rest : 3;
+    int f = MAT_Q, free = MAT_R;                          // where the product of the chain's factors is; the other place
+    float scale = SCALE;
+    gram();
+    for (int i = 0; i < len; ++i) {
+      const int p = i == 0 ? f : MAT_P;
+      mats(MAT_S, MAT_S, p, cc * UNSCALE, cb, ca * SCALE);                     // P
+      if (i > 0) {                                                             // product so far <- P times it, at scale q
+        mats(MAT_P, f, free, q / (SCALE * scale), 0.f, 0.f);
+        const int t = f; f = free; free = t;
+        scale = q;
+      }
+      if (i + 1 < len) {                                                       // S <- P (P S)
+        mats(p, MAT_S, MAT_T, UNSCALE, 0.f, 0.f);
+        mats(p, MAT_T, MAT_S, UNSCALE, 0.f, 0.f);
+      }
+    }
+    done += len;
+    applied(f, 1.f / scale, 0.f, done == steps);
   }
   return rc;
 }
@@ -798,6 +875,16 @@ extern "C" long long ddl_ns_shape(int rows, int cols, int prod, int batch, long 
   return h.slabs;
 }
 
+// 1: matrices with these thin and wide sides take their steps in chains
+extern "C" int ddl_ns_chains(const int* thin, const int* wide, int n) {
+  double chained = 0.0, single = 0.0;
+  for (int i = 0; i < n; ++i) {
+    chained += chained_work(thin[i], wide[i]);
+    single += single_work(thin[i], wide[i]);
+  }
+  return use_chains(chained, single) ? 1 : 0;
+}
+
 extern "C" int ddl_ns_mat_bytes() { return (int)sizeof(NsMat); }
 
 // g, out: [batch][rows][cols], bf16 or fp32;  ws: batch * ddl_ns_workspace fp16;  parts: batch * MAX_PARTS doubles;  slabs: batch times what
@@ -828,16 +915,17 @@ extern "C" int ddl_orthogonalize(const void* g, int is_bf16, void* out, void* ws
     if ((long long)h.blocks[i] * batch > 0x7fffffffll) return -2;
     blocks[i] = h.blocks[i] * batch;
   }
-  return prod == 3 ? run_steps<3, false>(a, blocks, nullptr, h.blocks, steps, abc, (hipStream_t)stream)
-                   : run_steps<1, false>(a, blocks, nullptr, h.blocks, steps, abc, (hipStream_t)stream);
+  const double thin = min(rows, cols), wide = max(rows, cols);
+  return prod == 3 ? run_steps<3, false>(a, blocks, nullptr, h.blocks, steps, abc, use_chains(chained_work(thin, wide), single_work(thin, wide)), (hipStream_t)stream)
+                   : run_steps<1, false>(a, blocks, nullptr, h.blocks, steps, abc, false, (hipStream_t)stream);
 }
 
 // Muon over the matrices of an arena.  table: NsMat[], maps: one int2[] after the other for the 8 launches, on the device;  blocks[8] on the host.
 // hyper (device): [0] lr [1] momentum [2] nesterov [4] gradient scale.  solo_wide > 0: every matrix is a ddl_ns_solo one, the widest has this many
-// columns (rows, if tall), blocks[0] is the number of matrices and maps[] names each once.
+// columns (rows, if tall), blocks[0] is the number of matrices and maps[] names each once.  chains: ddl_ns_chains of the set.
 extern "C" int ddl_muon_step(const void* table, const void* maps, const int* blocks, float* master, float* grad, float* mom, void* shadow,
                              const float* seg_wd, const float* hyper, void* ws, double* parts, float* slabs, int prod, int steps, const float* abc,
-                             float eps, int zero_grad, int solo_wide, void* stream) {
+                             float eps, int zero_grad, int solo_wide, int chains, void* stream) {
   if (steps <= 0 || (prod != 1 && prod != 3)) return -1;
   NsArgs a{};
   a.table = (const NsMat*)table;
@@ -855,6 +943,6 @@ extern "C" int ddl_muon_step(const void* table, const void* maps, const int* blo
   const int2* list[LAUNCHES];
   const int2* at = (const int2*)maps;
   for (int i = 0; i < LAUNCHES; ++i) { list[i] = at; at += blocks[i]; }
-  return prod == 3 ? run_steps<3, true>(a, blocks, list, nullptr, steps, abc, (hipStream_t)stream)
-                   : run_steps<1, true>(a, blocks, list, nullptr, steps, abc, (hipStream_t)stream);
+  return prod == 3 ? run_steps<3, true>(a, blocks, list, nullptr, steps, abc, chains != 0, (hipStream_t)stream)
+                   : run_steps<1, true>(a, blocks, list, nullptr, steps, abc, false, (hipStream_t)stream);
 }

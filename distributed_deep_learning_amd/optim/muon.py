@@ -104,11 +104,14 @@ class Muon(_ArenaOptimizer):
                 slabs += need
             for m, n in zip(launches, [1] + [0] * 7 if solo else out[2:10]):
                 m.append(np.stack([np.full(n, i, dtype=np.int32), np.arange(n, dtype=np.int32)], 1))
+        sides = [(C.c_int * len(self.matrices))(*(f(rows, cols) for _, rows, cols, _ in self.matrices)) for f in (min, max)]
         dev = self.arena.device
         maps = np.concatenate([np.concatenate(m) for m in launches])
         return {"table": torch.from_numpy(table.view(np.uint8).copy()).to(dev), "maps": torch.from_numpy(np.ascontiguousarray(maps)).to(dev),
                 "blocks": (C.c_int * 8)(*(sum(len(x) for x in m) for m in launches)), "prod": prod,
-                "solo": max(max(rows, cols) for _, rows, cols, _ in self.matrices) if solo else 0, "coef": (C.c_float * 3)(*self.ns_coefficients), "ws": torch.empty(max(ws, 8), dtype=torch.float16, device=dev),
+                "chains": lib.ddl_ns_chains(*sides, len(self.matrices)),
+                "solo": max(max(rows, cols) for _, rows, cols, _ in self.matrices) if solo else 0,
+                "coef": (C.c_float * 3)(*self.ns_coefficients), "ws": torch.empty(max(ws, 8), dtype=torch.float16, device=dev),
                 "slabs": torch.empty(max(slabs, 4), dtype=torch.float32, device=dev),
                 "parts": torch.empty(len(self.matrices) * lib.ddl_ns_max_parts(), dtype=torch.float64, device=dev)}
 
@@ -140,7 +143,7 @@ class Muon(_ArenaOptimizer):
                                          st["momentum"].data_ptr(), a.shadow.data_ptr() if a.shadow is not None else None,
                                          self.seg_wd.data_ptr(), self.hyper.data_ptr(), p["ws"].data_ptr(), p["parts"].data_ptr(),
                                          p["slabs"].data_ptr(), p["prod"], self.ns_steps, p["coef"], self.ns_eps, int(zero_grad),
-                                         p["solo"], _lib.stream_ptr()), "muon_step")
+                                         p["solo"], p["chains"], _lib.stream_ptr()), "muon_step")
         if self._adam_seg is not None:
             _lib.check(lib.ddl_flat_adam(a.master.data_ptr(), a.grad.data_ptr(), st["momentum"].data_ptr(),
                                          st["exp_avg_sq"].data_ptr(), a.shadow.data_ptr() if a.shadow is not None else None,
