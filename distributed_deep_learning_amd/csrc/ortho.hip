@@ -442,7 +442,7 @@ __global__ __launch_bounds__(256, BT == 256 || NST > 2 ? 1 : 2) void ns_product_
 // time are in LDS as operands.  Such matrices are bound by latency: 17 launches of about 5 us each take longer than all their products.
 // X is taken as [thin][wide] (a tall matrix is read and written transposed).
 template <int PROD> struct Solo {
-  static constexpr int KSTAGES = PROD == 3 ? 4 : 2, BUF = KSTAGES * 16384;      // a 128 x 128 operand
+  static constexpr int KSTAGES = PROD == 3 ? 4 : 2, KSTEP = 128 / KSTAGES, BUF = KSTAGES * 16384;      // a 128 x 128 operand
   static constexpr int SMEM = 2 * BUF;
   // Byte offset of the elements (row, col .. col + 3) of an operand, for a lane's first fragment; its other fragments are 16 rows (ROWS16 or
   // SLOW16(j)) and 16 columns (^ COL16) away.  The lo part of split operands is half a row (^ 64) or 32 rows (+ 8192) away.
@@ -544,9 +544,11 @@ __global__ __launch_bounds__(512, 2) void ns_solo_kernel(const NsArgs a, const i
 #pragma unroll
       for (int i = 0; i < 2; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   };
-  auto mul = [&](const char* pa, const char* pb, auto slow) {
+  // k: length of the reduction;  cols: of the result.  A wave whose part of the result is all padding keeps its zeros.
+  auto mul = [&](const char* pa, const char* pb, auto slow, int k, int cols) {
+    if (wm * 64 >= thin || wn * 32 >= cols) return;
 #pragma unroll 1
-    for (int st = 0; st < L::KSTAGES; ++st, pa += 16384, pb += 16384) {
+    for (int st = 0; st * L::KSTEP < k && st < L::KSTAGES; ++st, pa += 16384, pb += 16384) {
       s16x8 fa[4], fb[2][2];
       auto load_a = [&](int h) {
 #pragma unroll
@@ -597,7 +599,7 @@ __global__ __launch_bounds__(512, 2) void ns_solo_kernel(const NsArgs a, const i
     for (int t = 0; t < NT; ++t) {                                      // S = X X^T
       put_contig(t & 1 ? buf1 : buf0, x[t]);
       __syncthreads();                                                  // the other buffer's readers passed the previous barrier
-      mul(t & 1 ? buf1 : buf0, t & 1 ? buf1 : buf0, No{});
+      mul(t & 1 ? buf1 : buf0, t & 1 ? buf1 : buf0, No{}, wide - t * 128, thin);
     }
     f32x4 sv[4][2];
 #pragma unroll
@@ -609,7 +611,7 @@ __global__ __launch_bounds__(512, 2) void ns_solo_kernel(const NsArgs a, const i
     put_contig(bs, sv);
     __syncthreads();
     clear();
-    mul(bs, bs, No{});                                                  // B = b S + c S S
+    mul(bs, bs, No{}, thin, thin);                                                  // B = b S + c S S
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -621,7 +623,7 @@ __global__ __launch_bounds__(512, 2) void ns_solo_kernel(const NsArgs a, const i
       put_slow(bs, x[t]);
       __syncthreads();
       clear();
-      mul(bb, bs, Yes{});
+      mul(bb, bs, Yes{}, thin, wide - t * 128);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -736,7 +738,7 @@ inline bool use_chains(double chained, double single) { return chained <= 0.8 * 
 inline double chained_work(double thin, double wide) { return 6 * thin * thin * wide + 14 * thin * thin * thin; }
 inline double single_work(double thin, double wide) { return 15 * thin * thin * wide + 5 * thin * thin * thin; }
 
-// Measured: 64 x 147 bf16 41 us against 92 in 17 launches.  Four tiles (120 x 400 fp32) spill and run 257 us against 150: two at most.
+// Measured: 128 x 256 94 us against about 170 in 17 launches.  Four tiles (120 x 400 fp32) spill and run 257 us against 150: two at most.
 constexpr int SOLO_TILES = 2;
 inline bool solo(int rows, int cols) { return min(rows, cols) <= 128 && max(rows, cols) <= SOLO_TILES * 128; }
 
@@ -850,6 +852,10 @@ extern "C" long long ddl_ns_workspace(int rows, int cols, int prod) {
   if (rows <= 0 || cols <= 0 || (prod != 1 && prod != 3)) return -1;
   return prod == 3 ? Lay<3>(rows, cols).size : Lay<1>(rows, cols).size;
 }
+
+// Products of a plain call.  bf16 results need no more than 11-bit operands in large matrices (relative error of the result 0.0018 to 0.0021,
+// of which its rounding is 0.0017), but few products average less: 0.0023 to 0.0032 at thin sides of 128 to 16, 0.0017 with PROD = 3.
+extern "C" int ddl_ns_prod(int rows, int cols, int is_bf16) { return is_bf16 && min(rows, cols) > 128 ? 1 : 3; }
 
 // 1: one block does the whole matrix in one launch, which needs no workspace
 extern "C" int ddl_ns_solo(int rows, int cols) { return rows > 0 && cols > 0 && solo(rows, cols) ? 1 : 0; }

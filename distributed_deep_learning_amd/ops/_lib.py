@@ -106,6 +106,7 @@ _SIGS = {
     "ddl_ns_mat_bytes": [],
     "ddl_ns_work": [_i, _i, _i, _i],
     "ddl_ns_solo": [_i, _i],
+    "ddl_ns_prod": [_i, _i, _i],
     "ddl_ns_chains": [_vp, _vp, _i],
     "ddl_ns_shape": [_i, _i, _i, _i, _ll, _ll, _vp],
     "ddl_orthogonalize": [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _f, _vp],

@@ -1355,7 +1355,8 @@ def _newton_schulz_range(steps: int, a: float, b: float, c: float) -> tuple:
 def orthogonalize(g: torch.Tensor, steps: int = NS_STEPS, coefficients=NS_COEFFICIENTS, eps: float = NS_EPS) -> torch.Tensor:
     """The orthogonal factor of every matrix in ``g`` (``[m, n]`` or ``[batch, m, n]``, bf16 or fp32), approximately: ``steps``
     Newton-Schulz steps ``X <- a X + (b S + c S S) X``, ``S = X X^T``, from ``X = G / (|G|_F + eps)`` (``csrc/ortho.hip``).  The result has
-    ``g``'s shape and dtype; fp32 matrices are multiplied to fp32's accuracy, bf16 ones with 11-bit operands."""
+    ``g``'s shape and dtype; fp32 matrices are multiplied to fp32's accuracy, so are bf16 ones of up to 128 rows or
+    columns; larger ones with 11-bit operands, which adds little to the rounding of the result."""
     import ctypes as C
     lib = _lib.require()
     if g.dim() not in (2, 3):
@@ -1370,7 +1371,7 @@ def orthogonalize(g: torch.Tensor, steps: int = NS_STEPS, coefficients=NS_COEFFI
     batch = g.shape[0] if g.dim() == 3 else 1
     rows, cols = g.shape[-2:]
     is16 = g.dtype == BF16
-    prod = 1 if is16 else 3
+    prod = lib.ddl_ns_prod(rows, cols, int(is16))
     out = torch.empty_like(g)
     ws = parts = slabs = None
     if not lib.ddl_ns_solo(rows, cols):
