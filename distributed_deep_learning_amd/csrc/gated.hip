@@ -70,9 +70,9 @@ __device__ __forceinline__ void get24(const Kept& k, float* v) {
   }
 }
 
-// Tile order: XCD-contiguous runs that sweep 8 tile rows column by column, so that the operand panels a run shares stay in that L2.
-__device__ __forceinline__ void tile_of(unsigned bid, unsigned nwg, int tm, int tn, int& i, int& j) {
-  const unsigned t = xcd_remap(bid, nwg);
+// Tile order: XCD-contiguous runs (t counts blocks that way) that sweep 8 tile rows column by column, so that the operand panels a run shares
+// stay in that L2.
+__device__ __forceinline__ void tile_of(unsigned t, int tm, int tn, int& i, int& j) {
   const unsigned per = 8u * (unsigned)tn, grp = t / per, in = t - grp * per;
   const unsigned rows = min(8u, (unsigned)tm - grp * 8u);
   j = (int)(in / rows);
@@ -107,6 +107,10 @@ template <int BN> struct PairStager {
     gt::dma16(((j / PJ) & 1) ? ru : rg, lds + (unsigned)((j * 4 + wid) * 1024), voff[j] | kill);
   }
   __device__ __forceinline__ void end() { kdone += 64; gate += 64; up += 64; }
+  __device__ __forceinline__ void part(int first, int n) {
+    kdone = first * 64; gate += kdone; up += kdone;
+    k = min(k, (first + n) * 64);
+  }
 };
 
 // Two operands of the same shape one after the other along the reduction.
@@ -115,6 +119,16 @@ template <class S> struct Twice {
   S s;
   const unsigned short* second;
   int left;                                       // stages of the first
+  __device__ __forceinline__ void part(int first, int) {
+    if (first < left) {
+      s.part(first, left - first);
+      left -= first;
+    } else {
+      s.base = second;
+      s.part(first - left, left);
+      left = -1;
+    }
+  }
   __device__ __forceinline__ void begin() {
     if (left == 0) { s.base = second; s.kdone = 0; }
     --left;
@@ -126,32 +140,86 @@ template <class S> struct Twice {
 
 struct GatedArgs {
   const unsigned short *x, *wg, *wu, *wd, *dy;
-  unsigned short *h, *dg, *du, *y, *dx;
-  unsigned short* keep16; unsigned char* keep8;    // P then Q, [2][M][F]
+  unsigned short *h, *dg, *du, *y;
+  void* dx;
+  unsigned short* keep16; unsigned char* keep8;    // P then Q, [2][M][Fp]
   void *dwg, *dwu, *dwd;
-  int M, D, F, accumulate;                        // accumulate: weight gradients are fp32 and added to
+  float* slabs;
+  int M, D, F, Dp, Fp;                            // Dp, Fp: D and F padded to 8, the row lengths of all operands (the padding is zero)
+  int dx32, dw;                                   // dx fp32 instead of bf16;  weight gradients: 0 bf16, 1 fp32 added to, 2 fp32
+  int splits, per;                                // blocks that share the reduction of a tile, stages of each
 };
 
 __device__ __forceinline__ void store8(unsigned short* p, const float* v) { *reinterpret_cast<u32x4*>(p) = pack8(v); }
+// results have rows of their own length n: columns c .. c + 7 of row r
+__device__ __forceinline__ void result16(unsigned short* p, long long r, int c, int n, const float* v) {
+  p += r * n + c;
+  if ((n & 7) == 0) { store8(p, v); return; }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) if (c + e < n) p[e] = f32_to_bf16(v[e]);
+}
+__device__ __forceinline__ void result32(float* p, long long r, int c, int n, const float* v) {
+  p += r * n + c;
+  if ((n & 7) == 0) {
+    *reinterpret_cast<f32x4*>(p) = *reinterpret_cast<const f32x4*>(v);
+    *reinterpret_cast<f32x4*>(p + 4) = *reinterpret_cast<const f32x4*>(v + 4);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) if (c + e < n) p[e] = v[e];
+}
 
-template <int BT, int ACT, bool SAVE>
-__global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_up_kernel(const GatedArgs a) {
+// What a block of a product does.  The reduction of a tile may be shared by several blocks (few tiles, long reductions): each leaves its fp32
+// partial tile in a slab, and the launch with JOIN adds them in order, a block per 16-row group, and does the epilogue.
+template <int BT, int NST, bool JOIN> struct Block {
+  using T = gt::Tile<BT, BT, NST>;
+  static constexpr int NJ = JOIN ? 1 : T::FM;
+  static constexpr bool SPLIT = BT == 128 && !JOIN;
+  T tile;
+  int tid, lane, wid, t, part;                    // t: the tile;  part: of its reduction (JOIN: its row group)
+  __device__ __forceinline__ void begin(const GatedArgs& a) {
+    tid = threadIdx.x; lane = tid & 63; wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    t = (int)xcd_remap(blockIdx.x, gridDim.x); part = 0;
+    if (JOIN) { part = t % T::FM; t /= T::FM; }
+    else if (SPLIT && a.splits > 1) { part = t % a.splits; t /= a.splits; }
+  }
+  // true: the tile's epilogue is this block's
+  template <int AM, int BMD, class SA, class SB> __device__ __forceinline__ bool product(const GatedArgs& a, SA& sa, SB& sb, int nk, char* smem) {
+    float* const slab = a.slabs + (long long)t * a.splits * T::SLAB;
+    if (JOIN) { tile.sum_slabs(slab, a.splits, part, tid); return true; }
+    if (SPLIT && a.splits > 1) {
+      const int first = part * a.per;
+      nk = min(a.per, nk - first);
+      sa.part(first, nk);
+      sb.part(first, nk);
+    }
+    tile.zero();
+    tile.template mul<gt::Bf16, AM, BMD, 1>(sa, sb, nk, smem, wid, lane);
+    if (SPLIT && a.splits > 1) { tile.put_slab(slab + (long long)part * T::SLAB, tid); return false; }
+    return true;
+  }
+  template <class LD, class F> __device__ __forceinline__ void store(char* smem, LD&& load, F&& f) {
+    tile.template store<false, NJ>(smem, wid, lane, load, f, [](int, int, float*) {}, JOIN ? part : 0);
+  }
+};
+#define GATED_BOUNDS __launch_bounds__(256, BT == 256 || NST > 2 ? 1 : 2)
+
+template <int BT, int NST, bool JOIN, int ACT, bool SAVE> __global__ GATED_BOUNDS void gated_up_kernel(const GatedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Block<BT, NST, JOIN> b;
+  b.begin(a);
   int ti, tj;
-  tile_of(blockIdx.x, gridDim.x, (a.M + BT - 1) / BT, (a.F + BT / 2 - 1) / (BT / 2), ti, tj);
+  tile_of(b.t, (a.M + BT - 1) / BT, (a.F + BT / 2 - 1) / (BT / 2), ti, tj);
   const int m0 = ti * BT, f0 = tj * (BT / 2);
-  gt::Tile<BT, BT> tile;
-  tile.zero();
   gt::Stager<BT, gt::CONTIG, 1> sa;
   PairStager<BT> sb;
-  sa.init(gt::Operand{a.x, a.D, m0, a.M, a.D}, wid, lane);
-  sb.init(a.wg, a.wu, a.D, f0, a.F, a.D, wid, lane);
-  tile.template mul<gt::Bf16, gt::CONTIG, gt::CONTIG, 1>(sa, sb, (a.D + 63) / 64, smem, wid, lane);
-  tile.store_pairs(smem, wid, lane, [&](int r, int f, const float* g, const float* u) {
+  sa.init(gt::Operand{a.x, a.Dp, m0, a.M, a.D}, b.wid, b.lane);
+  sb.init(a.wg, a.wu, a.Dp, f0, a.F, a.D, b.wid, b.lane);
+  if (!b.template product<gt::CONTIG, gt::CONTIG>(a, sa, sb, (a.D + 63) / 64, smem)) return;
+  b.tile.template store_pairs<b.NJ>(smem, b.wid, b.lane, [&](int r, int f, const float* g, const float* u) {
     r += m0; f += f0;
-    if (r >= a.M || f >= a.F) return;
-    const long long o = (long long)r * a.F + f;
+    if (r >= a.M || f >= a.Fp) return;
+    const long long o = (long long)r * a.Fp + f;
     float h[8], p[8], q[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -162,59 +230,55 @@ __global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_up_kernel(const 
     }
     store8(a.h + o, h);
     if (SAVE) {
-      const long long plane = (long long)a.M * a.F;
+      const long long plane = (long long)a.M * a.Fp;
       keep24<8>(a.keep16 + o, a.keep8 + o, p);
       keep24<8>(a.keep16 + plane + o, a.keep8 + plane + o, q);
     }
+  }, JOIN ? b.part : 0);
+}
+
+template <int BT, int NST, bool JOIN> __global__ GATED_BOUNDS void gated_down_kernel(const GatedArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  Block<BT, NST, JOIN> b;
+  b.begin(a);
+  int ti, tj;
+  tile_of(b.t, (a.M + BT - 1) / BT, (a.D + BT - 1) / BT, ti, tj);
+  const int m0 = ti * BT, n0 = tj * BT;
+  gt::Stager<BT, gt::CONTIG, 1> sa, sb;
+  sa.init(gt::Operand{a.h, a.Fp, m0, a.M, a.F}, b.wid, b.lane);
+  sb.init(gt::Operand{a.wd, a.Fp, n0, a.D, a.F}, b.wid, b.lane);
+  if (!b.template product<gt::CONTIG, gt::CONTIG>(a, sa, sb, (a.F + 63) / 64, smem)) return;
+  b.store(smem, gt::NoLoad{}, [&](int r, int c, const float* v, gt::None) {
+    r += m0; c += n0;
+    if (r < a.M && c < a.D) result16(a.y, r, c, a.D, v);
   });
 }
 
-template <int BT>
-__global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_down_kernel(const GatedArgs a) {
+template <int BT, int NST, bool JOIN> __global__ GATED_BOUNDS void gated_dh_kernel(const GatedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Block<BT, NST, JOIN> b;
+  b.begin(a);
   int ti, tj;
-  tile_of(blockIdx.x, gridDim.x, (a.M + BT - 1) / BT, (a.D + BT - 1) / BT, ti, tj);
+  tile_of(b.t, (a.M + BT - 1) / BT, (a.F + BT - 1) / BT, ti, tj);
   const int m0 = ti * BT, n0 = tj * BT;
-  gt::Tile<BT, BT> tile;
-  tile.zero();
-  gt::Stager<BT, gt::CONTIG, 1> sa, sb;
-  sa.init(gt::Operand{a.h, a.F, m0, a.M, a.F}, wid, lane);
-  sb.init(gt::Operand{a.wd, a.F, n0, a.D, a.F}, wid, lane);
-  tile.template mul<gt::Bf16, gt::CONTIG, gt::CONTIG, 1>(sa, sb, (a.F + 63) / 64, smem, wid, lane);
-  tile.template store<false>(smem, wid, lane, gt::NoLoad{}, [&](int r, int c, const float* v, gt::None) {
-    r += m0; c += n0;
-    if (r < a.M && c < a.D) store8(a.y + (long long)r * a.D + c, v);
-  }, [](int, int, float*) {});
-}
-
-template <int BT>
-__global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_dh_kernel(const GatedArgs a) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int ti, tj;
-  tile_of(blockIdx.x, gridDim.x, (a.M + BT - 1) / BT, (a.F + BT - 1) / BT, ti, tj);
-  const int m0 = ti * BT, n0 = tj * BT;
-  gt::Tile<BT, BT> tile;
-  tile.zero();
   gt::Stager<BT, gt::CONTIG, 1> sa;
   gt::Stager<BT, gt::SLOW, 1> sb;
-  sa.init(gt::Operand{a.dy, a.D, m0, a.M, a.D}, wid, lane);
-  sb.init(gt::Operand{a.wd, a.F, n0, a.F, a.D}, wid, lane);
-  tile.template mul<gt::Bf16, gt::CONTIG, gt::SLOW, 1>(sa, sb, (a.D + 63) / 64, smem, wid, lane);
-  const long long plane = (long long)a.M * a.F;
+  sa.init(gt::Operand{a.dy, a.Dp, m0, a.M, a.D}, b.wid, b.lane);
+  sb.init(gt::Operand{a.wd, a.Fp, n0, a.Fp, a.D}, b.wid, b.lane);
+  if (!b.template product<gt::CONTIG, gt::SLOW>(a, sa, sb, (a.D + 63) / 64, smem)) return;
+  const long long plane = (long long)a.M * a.Fp;
   struct Factors { Kept p, q; };
   auto load = [&](int r, int c) {
     r += m0; c += n0;
-    const long long o = (long long)r * a.F + c;
+    const long long o = (long long)r * a.Fp + c;
     Factors k{};
-    if (r < a.M && c < a.F) { k.p = load24(a.keep16 + o, a.keep8 + o); k.q = load24(a.keep16 + plane + o, a.keep8 + plane + o); }
+    if (r < a.M && c < a.Fp) { k.p = load24(a.keep16 + o, a.keep8 + o); k.q = load24(a.keep16 + plane + o, a.keep8 + plane + o); }
     return k;
   };
-  tile.template store<false>(smem, wid, lane, load, [&](int r, int c, const float* v, const Factors& k) {
+  b.store(smem, load, [&](int r, int c, const float* v, const Factors& k) {
     r += m0; c += n0;
-    if (r >= a.M || c >= a.F) return;
-    const long long o = (long long)r * a.F + c;
+    if (r >= a.M || c >= a.Fp) return;
+    const long long o = (long long)r * a.Fp + c;
     float p[8], q[8], dg[8], du[8];
     get24(k.p, p);
     get24(k.q, q);
@@ -222,73 +286,105 @@ __global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_dh_kernel(const 
     for (int e = 0; e < 8; ++e) { dg[e] = v[e] * p[e]; du[e] = v[e] * q[e]; }
     store8(a.dg + o, dg);
     store8(a.du + o, du);
-  }, [](int, int, float*) {});
+  });
 }
 
-template <int BT>
-__global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_dx_kernel(const GatedArgs a) {
+template <int BT, int NST, bool JOIN> __global__ GATED_BOUNDS void gated_dx_kernel(const GatedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Block<BT, NST, JOIN> b;
+  b.begin(a);
   int ti, tj;
-  tile_of(blockIdx.x, gridDim.x, (a.M + BT - 1) / BT, (a.D + BT - 1) / BT, ti, tj);
+  tile_of(b.t, (a.M + BT - 1) / BT, (a.D + BT - 1) / BT, ti, tj);
   const int m0 = ti * BT, n0 = tj * BT, nk = (a.F + 63) / 64;
-  gt::Tile<BT, BT> tile;
-  tile.zero();
   Twice<gt::Stager<BT, gt::CONTIG, 1>> sa;
   Twice<gt::Stager<BT, gt::SLOW, 1>> sb;
-  sa.s.init(gt::Operand{a.dg, a.F, m0, a.M, a.F}, wid, lane);
-  sa.second = a.du + (long long)m0 * a.F;
-  sb.s.init(gt::Operand{a.wg, a.D, n0, a.D, a.F}, wid, lane);
+  sa.s.init(gt::Operand{a.dg, a.Fp, m0, a.M, a.F}, b.wid, b.lane);
+  sa.second = a.du + (long long)m0 * a.Fp;
+  sb.s.init(gt::Operand{a.wg, a.Dp, n0, a.Dp, a.F}, b.wid, b.lane);
   sb.second = a.wu;
   sa.left = sb.left = nk;
-  tile.template mul<gt::Bf16, gt::CONTIG, gt::SLOW, 1>(sa, sb, 2 * nk, smem, wid, lane);
-  tile.template store<false>(smem, wid, lane, gt::NoLoad{}, [&](int r, int c, const float* v, gt::None) {
+  if (!b.template product<gt::CONTIG, gt::SLOW>(a, sa, sb, 2 * nk, smem)) return;
+  b.store(smem, gt::NoLoad{}, [&](int r, int c, const float* v, gt::None) {
     r += m0; c += n0;
-    if (r < a.M && c < a.D) store8(a.dx + (long long)r * a.D + c, v);
-  }, [](int, int, float*) {});
+    if (r >= a.M || c >= a.D) return;
+    if (a.dx32) result32((float*)a.dx, r, c, a.D, v);
+    else result16((unsigned short*)a.dx, r, c, a.D, v);
+  });
 }
 
-template <int BT>
-__global__ __launch_bounds__(256, BT == 256 ? 1 : 2) void gated_dw_kernel(const GatedArgs a) {
+template <int BT, int NST, bool JOIN> __global__ GATED_BOUNDS void gated_dw_kernel(const GatedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int tf = (a.F + BT - 1) / BT, td = (a.D + BT - 1) / BT, per = tf * td, which = (int)blockIdx.x / per;
+  Block<BT, NST, JOIN> b;
+  b.begin(a);
+  const int tf = (a.F + BT - 1) / BT, td = (a.D + BT - 1) / BT, each = tf * td, which = b.t / each;
   int ti, tj;
-  tile_of(blockIdx.x - (unsigned)(which * per), (unsigned)per, which == 2 ? td : tf, which == 2 ? tf : td, ti, tj);
+  tile_of((unsigned)(b.t - which * each), which == 2 ? td : tf, which == 2 ? tf : td, ti, tj);
   const int rows = which == 2 ? a.D : a.F, cols = which == 2 ? a.F : a.D;
+  const int lda = which == 2 ? a.Dp : a.Fp, ldb = which == 2 ? a.Fp : a.Dp;
   const unsigned short* const pa = which == 0 ? a.dg : which == 1 ? a.du : a.dy;
   const unsigned short* const pb = which == 2 ? a.h : a.x;
   void* const out = which == 0 ? a.dwg : which == 1 ? a.dwu : a.dwd;
   if (out == nullptr) return;
   const int m0 = ti * BT, n0 = tj * BT;
-  gt::Tile<BT, BT> tile;
-  tile.zero();
   gt::Stager<BT, gt::SLOW, 1> sa, sb;
-  sa.init(gt::Operand{pa, rows, m0, rows, a.M}, wid, lane);
-  sb.init(gt::Operand{pb, cols, n0, cols, a.M}, wid, lane);
-  tile.template mul<gt::Bf16, gt::SLOW, gt::SLOW, 1>(sa, sb, (a.M + 63) / 64, smem, wid, lane);
+  sa.init(gt::Operand{pa, lda, m0, lda, a.M}, b.wid, b.lane);
+  sb.init(gt::Operand{pb, ldb, n0, ldb, a.M}, b.wid, b.lane);
+  if (!b.template product<gt::SLOW, gt::SLOW>(a, sa, sb, (a.M + 63) / 64, smem)) return;
   struct Sum { f32x4 lo, hi; };
   auto load = [&](int r, int c) {
     r += m0; c += n0;
     Sum q{};
-    if (a.accumulate && r < rows && c < cols) {
+    if (a.dw == 1 && r < rows && c < cols) {
       const float* const p = (const float*)out + (long long)r * cols + c;
-      q = Sum{*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 4)};
+      if ((cols & 7) == 0) {
+        q = Sum{*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 4)};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (c + e < cols) q.lo[e] = p[e];
+          if (c + e + 4 < cols) q.hi[e] = p[e + 4];
+        }
+      }
     }
     return q;
   };
-  tile.template store<false>(smem, wid, lane, load, [&](int r, int c, const float* v, const Sum& q) {
+  b.store(smem, load, [&](int r, int c, float* v, const Sum& q) {
     r += m0; c += n0;
     if (r >= rows || c >= cols) return;
-    const long long o = (long long)r * cols + c;
-    if (a.accumulate) {
-      float* const p = (float*)out + o;
-      *reinterpret_cast<f32x4*>(p) = f32x4{q.lo[0] + v[0], q.lo[1] + v[1], q.lo[2] + v[2], q.lo[3] + v[3]};
-      *reinterpret_cast<f32x4*>(p + 4) = f32x4{q.hi[0] + v[4], q.hi[1] + v[5], q.hi[2] + v[6], q.hi[3] + v[7]};
+    if (a.dw == 0) { result16((unsigned short*)out, r, c, cols, v); return; }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[e] += q.lo[e]; v[e + 4] += q.hi[e]; }
+    result32((float*)out, r, c, cols, v);
+  });
+}
+
+// Operands as the products take them: bf16, rows padded with zeros to 8 elements (16 bytes), contiguous.  What is so already is used as it lies;
+// the rest (fp32, other widths or row strides) is copied here, all in one launch.
+struct PadJob { const void* src; unsigned short* dst; long long stride, first; int rows, cols, is32, wide; };
+struct PadArgs { PadJob job[4]; int n; long long total; };
+__global__ __launch_bounds__(256) void gated_pad_kernel(const PadArgs a) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.total; i += (long long)gridDim.x * 256) {
+    int j = 0;
+    while (j + 1 < a.n && i >= a.job[j + 1].first) ++j;
+    const PadJob& q = a.job[j];
+    const int per = (q.cols + 7) / 8;
+    const long long in = i - q.first, row = in / per;
+    const int c = (int)(in - row * per) * 8;
+    const long long at = row * q.stride + c;
+    float v[8];
+    if (q.wide && q.is32) {
+      *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>((const float*)q.src + at);
+      *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>((const float*)q.src + at + 4);
+    } else if (q.wide) {
+      *reinterpret_cast<u32x4*>(q.dst + in * 8) = *reinterpret_cast<const u32x4*>((const unsigned short*)q.src + at);
+      continue;
     } else {
-      store8((unsigned short*)out + o, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        v[e] = c + e >= q.cols ? 0.f : q.is32 ? ((const float*)q.src)[at + e] : bf16_to_f32(((const bf16_t*)q.src)[at + e]);
     }
-  }, [](int, int, float*) {});
+    store8(q.dst + in * 8, v);
+  }
 }
 
 // ---- few tokens (serving): bound by reading the weights once.  A block owns 16 features (their gate and up rows, or 16 rows of Wd); its waves
@@ -301,13 +397,13 @@ __global__ __launch_bounds__(64 * WAVES) void gated_few_kernel(const GatedArgs a
   __shared__ f32x4 red[WAVES][NM * TB][64];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = lane & 15, kc = (lane >> 4) * 8;
-  const int K = PAIR ? a.D : a.F, N = PAIR ? a.F : a.D;                  // reduction, rows of the weights
+  const int K = PAIR ? a.D : a.F, N = PAIR ? a.F : a.D, ld = PAIR ? a.Dp : a.Fp;   // reduction, rows of the weights, row length of both operands
   const int f0 = blockIdx.x * 16;
   const unsigned short* const in = PAIR ? a.x : a.h;
-  const unsigned long long wbytes = (unsigned long long)(N - f0 < 16 ? N - f0 : 16) * (unsigned long long)K * 2ull;
-  const __amdgpu_buffer_rsrc_t w0 = __builtin_amdgcn_make_buffer_rsrc((void*)((PAIR ? a.wg : a.wd) + (long long)f0 * K), 0, (int)wbytes, 0x00020000);
-  const __amdgpu_buffer_rsrc_t w1 = __builtin_amdgcn_make_buffer_rsrc((void*)((PAIR ? a.wu : a.wd) + (long long)f0 * K), 0, (int)wbytes, 0x00020000);
-  const __amdgpu_buffer_rsrc_t xs = __builtin_amdgcn_make_buffer_rsrc((void*)in, 0, (int)((unsigned long long)a.M * K * 2ull), 0x00020000);
+  const unsigned long long wbytes = (unsigned long long)(N - f0 < 16 ? N - f0 : 16) * (unsigned long long)ld * 2ull;
+  const __amdgpu_buffer_rsrc_t w0 = __builtin_amdgcn_make_buffer_rsrc((void*)((PAIR ? a.wg : a.wd) + (long long)f0 * ld), 0, (int)wbytes, 0x00020000);
+  const __amdgpu_buffer_rsrc_t w1 = __builtin_amdgcn_make_buffer_rsrc((void*)((PAIR ? a.wu : a.wd) + (long long)f0 * ld), 0, (int)wbytes, 0x00020000);
+  const __amdgpu_buffer_rsrc_t xs = __builtin_amdgcn_make_buffer_rsrc((void*)in, 0, (int)((unsigned long long)a.M * ld * 2ull), 0x00020000);
   f32x4 acc[NM][TB];
 #pragma unroll
   for (int m = 0; m < NM; ++m)
@@ -321,13 +417,13 @@ __global__ __launch_bounds__(64 * WAVES) void gated_few_kernel(const GatedArgs a
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int k = (s + u * WAVES) * 64 + h * 32 + kc;
-        const bool in_k = k < K;                                         // K % 8 == 0: whole pieces
-        const unsigned off = in_k ? (unsigned)(row * K + k) * 2u : gt::OOB;
+        const bool in_k = k < K;                                         // a last piece ends in the padding
+        const unsigned off = in_k ? (unsigned)(row * ld + k) * 2u : gt::OOB;
         w[u][h][0] = __builtin_amdgcn_raw_buffer_load_b128(w0, (int)off, 0, 0);
         if (PAIR) w[u][h][NM - 1] = __builtin_amdgcn_raw_buffer_load_b128(w1, (int)off, 0, 0);
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
-          const unsigned xo = in_k && t * 16 + row < a.M ? (unsigned)((t * 16 + row) * K + k) * 2u : gt::OOB;
+          const unsigned xo = in_k && t * 16 + row < a.M ? (unsigned)((t * 16 + row) * ld + k) * 2u : gt::OOB;
           x[u][h][t] = __builtin_amdgcn_raw_buffer_load_b128(xs, (int)xo, 0, 0);
         }
       }
@@ -350,7 +446,7 @@ __global__ __launch_bounds__(64 * WAVES) void gated_few_kernel(const GatedArgs a
   __syncthreads();
   for (int i = tid; i < TB * 64; i += 64 * WAVES) {
     const int t = i >> 6, l = i & 63, tok = t * 16 + (l & 15), f = f0 + (l >> 4) * 4;
-    if (tok >= a.M || f >= N) continue;
+    if (tok >= a.M || f >= (PAIR ? a.Fp : N)) continue;
     f32x4 v[NM];
 #pragma unroll
     for (int m = 0; m < NM; ++m) {
@@ -362,7 +458,7 @@ __global__ __launch_bounds__(64 * WAVES) void gated_few_kernel(const GatedArgs a
         for (int e = 0; e < 4; ++e) v[m][e] += o[e];
       }
     }
-    const long long o = (long long)tok * N + f;
+    const long long o = (long long)tok * (PAIR ? a.Fp : N) + f;
     float y[4], p[4], q[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -375,9 +471,14 @@ __global__ __launch_bounds__(64 * WAVES) void gated_few_kernel(const GatedArgs a
         y[e] = v[0][e];
       }
     }
-    *reinterpret_cast<u32x2*>((PAIR ? a.h : a.y) + o) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+    if (PAIR || (N & 3) == 0) {
+      *reinterpret_cast<u32x2*>((PAIR ? a.h : a.y) + o) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) if (f + e < N) a.y[o + e] = f32_to_bf16(y[e]);
+    }
     if (SAVE) {
-      const long long plane = (long long)a.M * a.F;
+      const long long plane = (long long)a.M * a.Fp;
       keep24<4>(a.keep16 + o, a.keep8 + o, p);
       keep24<4>(a.keep16 + plane + o, a.keep8 + plane + o, q);
     }
@@ -387,23 +488,56 @@ __global__ __launch_bounds__(64 * WAVES) void gated_few_kernel(const GatedArgs a
 inline long long tiles(int n, int t) { return ((long long)n + t - 1) / t; }
 
 // one launch of a kernel that takes GatedArgs; opts in to its LDS once per device
-template <int BT, auto KERNEL> int launch(long long blocks, const GatedArgs& a, void* stream) {
+template <int BT, int NST, auto KERNEL> int launch(long long blocks, const GatedArgs& a, void* stream) {
   static SmemAttrOnce once;
   if (blocks <= 0 || blocks > 0x7fffffffll) return -2;
-  constexpr int smem = gt::Tile<BT, BT>::SMEM;
+  constexpr int smem = gt::Tile<BT, BT, NST>::SMEM;
   const int rc = once.ensure(reinterpret_cast<const void*>(KERNEL), smem);
   if (rc != 0) return rc;
   hipLaunchKernelGGL(KERNEL, dim3((unsigned)blocks), dim3(256), smem, (hipStream_t)stream, a);
   return (int)hipGetLastError();
 }
 
-template <int BT, int ACT> int launch_up(const GatedArgs& a, bool save, void* st) {
-  const long long nb = tiles(a.M, BT) * tiles(a.F, BT / 2);
-  return save ? launch<BT, &gated_up_kernel<BT, ACT, true>>(nb, a, st) : launch<BT, &gated_up_kernel<BT, ACT, false>>(nb, a, st);
+// How `count` products of rows x cols over ks stages are cut.  256 x 256 tiles run four times the work of a 128 x 128 stage in about 1.4 times
+// the time of a CU's pair of them, but one at a time, so that nothing hides a block's ends.
+struct Cut { bool large; int splits, per; long long tiles; };
+Cut cut_of(int count, int rows, int cols, int ks) {
+  Cut c{};
+  const long long big = count * tiles(rows, 256) * tiles(cols, 256);
+  c.tiles = count * tiles(rows, 128) * tiles(cols, 128);
+  double small = 0.0;
+  c.per = gt::chunk_for(c.tiles, ks, &small);
+  c.splits = (ks + c.per - 1) / c.per;
+  c.large = 1.44 * (double)((big + gt::CUS - 1) / gt::CUS) * (ks + 10) < small;
+  if (c.large) { c.tiles = big; c.splits = 1; c.per = ks; }
+  return c;
 }
-template <int BT> int up_act(const GatedArgs& a, int act, bool save, void* st) {
-  return act == SILU ? launch_up<BT, SILU>(a, save, st) : act == GELU ? launch_up<BT, GELU>(a, save, st) : launch_up<BT, RELU>(a, save, st);
+long long slab_floats(const Cut& c) { return c.splits > 1 ? c.tiles * c.splits * gt::Tile<128, 128>::SLAB : 0; }
+
+// P::at<BT, NST, JOIN>: the kernel
+template <class P> int product(const Cut& c, GatedArgs a, void* st) {
+  a.splits = c.splits; a.per = c.per;
+  if (c.splits > 1 && a.slabs == nullptr) return -1;
+  if (c.large) return launch<256, 2, P::template at<256, 2, false>>(c.tiles, a, st);
+  const long long blocks = c.tiles * c.splits;
+  int rc = blocks <= gt::CUS ? launch<128, 4, P::template at<128, 4, false>>(blocks, a, st)
+                             : launch<128, 2, P::template at<128, 2, false>>(blocks, a, st);
+  if (rc == 0 && c.splits > 1) rc = launch<128, 2, P::template at<128, 2, true>>(c.tiles * gt::Tile<128, 128>::FM, a, st);
+  return rc;
 }
+template <int ACT, bool SAVE> struct Up { template <int BT, int NST, bool JOIN> static constexpr auto at = &gated_up_kernel<BT, NST, JOIN, ACT, SAVE>; };
+struct Down { template <int BT, int NST, bool JOIN> static constexpr auto at = &gated_down_kernel<BT, NST, JOIN>; };
+struct Dh { template <int BT, int NST, bool JOIN> static constexpr auto at = &gated_dh_kernel<BT, NST, JOIN>; };
+struct Dx { template <int BT, int NST, bool JOIN> static constexpr auto at = &gated_dx_kernel<BT, NST, JOIN>; };
+struct Dw { template <int BT, int NST, bool JOIN> static constexpr auto at = &gated_dw_kernel<BT, NST, JOIN>; };
+
+int stages(int k) { return (int)tiles(k, 64); }
+Cut cut_up(int M, int D, int F) { return cut_of(1, M, 2 * F, stages(D)); }
+Cut cut_down(int M, int D, int F) { return cut_of(1, M, D, stages(F)); }
+Cut cut_dh(int M, int D, int F) { return cut_of(1, M, F, stages(D)); }
+Cut cut_dx(int M, int D, int F) { return cut_of(1, M, D, 2 * stages(F)); }
+Cut cut_dw(int M, int D, int F) { return cut_of(3, F, D, stages(M)); }
+
 constexpr int FEW = 64;                            // tokens up to which gated_few_kernel is used
 
 template <int TB, bool PAIR, int ACT, bool SAVE> int launch_few_t(const GatedArgs& a, void* st) {
@@ -422,67 +556,86 @@ template <int ACT> int few_up(const GatedArgs& a, bool save, void* st) {
 // 32-bit offsets inside 16 rows of a weight and inside the tokens
 bool few(int M, int K) { return M <= FEW && (long long)FEW * K * 2 < 0x7fffffffll; }
 
-// 256 x 256 tiles where they fill the chip
-bool large(int m, int n) { return tiles(m, 256) * tiles(n, 256) >= 256; }
+bool sizes_ok(int M, int D, int F) { return M > 0 && D > 0 && F > 0 && D < (1 << 30) && F < (1 << 30); }
 
-bool sizes_ok(int M, int D, int F) { return M > 0 && D > 0 && F > 0 && D % 8 == 0 && F % 8 == 0; }
+template <int ACT> int up(const GatedArgs& a, void* st) {
+  const bool save = a.keep16 != nullptr;
+  if (few(a.M, a.Dp)) return few_up<ACT>(a, save, st);
+  const Cut c = cut_up(a.M, a.D, a.F);
+  return save ? product<Up<ACT, true>>(c, a, st) : product<Up<ACT, false>>(c, a, st);
+}
+
+inline int pad8(int n) { return (n + 7) & ~7; }
 
 }  // namespace
 
-// h [M][F];  keep16 [2][M][F] (16 bit) and keep8 [2][M][F] (8 bit), or both null: what the backward pass needs
-extern "C" int ddl_gated_up(const void* x, const void* wg, const void* wu, void* h, void* keep16, void* keep8, int M, int D, int F, int act,
-                            void* stream) {
+// Floats of partial tiles that a forward (0) or backward pass (1: dh and dx, 2: weight gradients, 3: both) needs
+extern "C" long long ddl_gated_workspace(int M, int D, int F, int pass) {
+  if (!sizes_ok(M, D, F) || pass < 0 || pass > 3) return -1;
+  long long n = 0;
+  auto most = [&](const Cut& c) { n = max(n, slab_floats(c)); };
+  if (pass == 0) {
+    if (!few(M, pad8(D))) most(cut_up(M, D, F));
+    if (!few(M, pad8(F))) most(cut_down(M, D, F));
+  }
+  if (pass & 1) { most(cut_dh(M, D, F)); most(cut_dx(M, D, F)); }
+  if (pass & 2) most(cut_dw(M, D, F));
+  return n;
+}
+
+// n <= 4 matrices [rows][cols] with the given row strides (elements) -> bf16 [rows][cols padded to 8]
+extern "C" int ddl_gated_pad(const void* const* src, void* const* dst, const int* rows, const int* cols, const long long* stride, const int* is32,
+                             int n, void* stream) {
+  if (n < 1 || n > 4) return -1;
+  PadArgs a{};
+  a.n = n;
+  for (int i = 0; i < n; ++i) {
+    if (rows[i] < 0 || cols[i] <= 0) return -1;
+    PadJob& j = a.job[i];
+    j = PadJob{src[i], (unsigned short*)dst[i], stride[i], a.total, rows[i], cols[i], is32[i], 0};
+    j.wide = cols[i] % 8 == 0 && stride[i] % (is32[i] ? 4 : 8) == 0 && (unsigned long long)src[i] % 16 == 0;
+    a.total += (long long)rows[i] * (pad8(cols[i]) / 8);
+  }
+  if (a.total == 0) return 0;
+  hipLaunchKernelGGL(gated_pad_kernel, dim3(grid_for(a.total, 256, 16384)), dim3(256), 0, (hipStream_t)stream, a);
+  return (int)hipGetLastError();
+}
+
+// x [M][Dp], wg and wu [F][Dp], wd [D][Fp], h [M][Fp], y [M][D];  keep16 [2][M][Fp] (16 bit) and keep8 [2][M][Fp] (8 bit), or both null: what
+// the backward pass needs.  Dp and Fp: D and F padded to 8 with zeros.
+extern "C" int ddl_gated_fwd(const void* x, const void* wg, const void* wu, const void* wd, void* h, void* keep16, void* keep8, void* y, float* slabs,
+                             int M, int D, int F, int act, void* stream) {
   if (!sizes_ok(M, D, F) || (keep16 == nullptr) != (keep8 == nullptr)) return -1;
   GatedArgs a{};
-  a.x = (const unsigned short*)x; a.wg = (const unsigned short*)wg; a.wu = (const unsigned short*)wu;
+  a.x = (const unsigned short*)x; a.wg = (const unsigned short*)wg; a.wu = (const unsigned short*)wu; a.wd = (const unsigned short*)wd;
+  a.h = (unsigned short*)h; a.keep16 = (unsigned short*)keep16; a.keep8 = (unsigned char*)keep8; a.y = (unsigned short*)y;
+  a.slabs = slabs;
+  a.M = M; a.D = D; a.F = F; a.Dp = pad8(D); a.Fp = pad8(F);
+  int rc = -1;
+  if (act == SILU) rc = up<SILU>(a, stream);
+  else if (act == GELU) rc = up<GELU>(a, stream);
+  else if (act == RELU) rc = up<RELU>(a, stream);
+  if (rc != 0) return rc;
+  return few(M, a.Fp) ? launch_few<false, SILU, false>(a, stream) : product<Down>(cut_down(M, D, F), a, stream);
+}
+
+// pass: 1 dg and du (and dx, unless null), 2 weight gradients (those that are not null; they take dg and du), 3 both.  dy [M][Dp], dg and du
+// [M][Fp], dx [M][D] bf16 or (dx32) fp32, dwg and dwu [F][D], dwd [D][F]: dw 0 bf16, 1 fp32 that are added to, 2 fp32
+extern "C" int ddl_gated_bwd(const void* x, const void* dy, const void* wg, const void* wu, const void* wd, const void* h, const void* keep16,
+                             const void* keep8, void* dg, void* du, void* dx, int dx32, void* dwg, void* dwu, void* dwd, int dw, float* slabs,
+                             int M, int D, int F, int pass, void* stream) {
+  if (!sizes_ok(M, D, F) || pass < 1 || pass > 3 || dw < 0 || dw > 2) return -1;
+  GatedArgs a{};
+  a.x = (const unsigned short*)x; a.dy = (const unsigned short*)dy;
+  a.wg = (const unsigned short*)wg; a.wu = (const unsigned short*)wu; a.wd = (const unsigned short*)wd;
   a.h = (unsigned short*)h; a.keep16 = (unsigned short*)keep16; a.keep8 = (unsigned char*)keep8;
-  a.M = M; a.D = D; a.F = F;
-  if (act < SILU || act > RELU) return -1;
-  const bool save = keep16 != nullptr;
-  if (few(M, D)) return act == SILU ? few_up<SILU>(a, save, stream) : act == GELU ? few_up<GELU>(a, save, stream) : few_up<RELU>(a, save, stream);
-  return large(M, 2 * F) ? up_act<256>(a, act, save, stream) : up_act<128>(a, act, save, stream);
-}
-
-extern "C" int ddl_gated_down(const void* h, const void* wd, void* y, int M, int D, int F, void* stream) {
-  if (!sizes_ok(M, D, F)) return -1;
-  GatedArgs a{};
-  a.h = (unsigned short*)h; a.wd = (const unsigned short*)wd; a.y = (unsigned short*)y;
-  a.M = M; a.D = D; a.F = F;
-  if (few(M, F)) return launch_few<false, SILU, false>(a, stream);
-  return large(M, D) ? launch<256, &gated_down_kernel<256>>(tiles(M, 256) * tiles(D, 256), a, stream)
-                     : launch<128, &gated_down_kernel<128>>(tiles(M, 128) * tiles(D, 128), a, stream);
-}
-
-extern "C" int ddl_gated_dh(const void* dy, const void* wd, const void* keep16, const void* keep8, void* dg, void* du, int M, int D, int F,
-                            void* stream) {
-  if (!sizes_ok(M, D, F)) return -1;
-  GatedArgs a{};
-  a.dy = (const unsigned short*)dy; a.wd = (const unsigned short*)wd;
-  a.keep16 = (unsigned short*)keep16; a.keep8 = (unsigned char*)keep8; a.dg = (unsigned short*)dg; a.du = (unsigned short*)du;
-  a.M = M; a.D = D; a.F = F;
-  return large(M, F) ? launch<256, &gated_dh_kernel<256>>(tiles(M, 256) * tiles(F, 256), a, stream)
-                     : launch<128, &gated_dh_kernel<128>>(tiles(M, 128) * tiles(F, 128), a, stream);
-}
-
-extern "C" int ddl_gated_dx(const void* dg, const void* du, const void* wg, const void* wu, void* dx, int M, int D, int F, void* stream) {
-  if (!sizes_ok(M, D, F)) return -1;
-  GatedArgs a{};
-  a.dg = (unsigned short*)dg; a.du = (unsigned short*)du; a.wg = (const unsigned short*)wg; a.wu = (const unsigned short*)wu;
-  a.dx = (unsigned short*)dx;
-  a.M = M; a.D = D; a.F = F;
-  return large(M, D) ? launch<256, &gated_dx_kernel<256>>(tiles(M, 256) * tiles(D, 256), a, stream)
-                     : launch<128, &gated_dx_kernel<128>>(tiles(M, 128) * tiles(D, 128), a, stream);
-}
-
-// weight gradients: bf16, written (accumulate 0), or fp32, added to (accumulate 1); a null one is left out
-extern "C" int ddl_gated_dw(const void* x, const void* dy, const void* h, const void* dg, const void* du, void* dwg, void* dwu, void* dwd, int M,
-                            int D, int F, int accumulate, void* stream) {
-  if (!sizes_ok(M, D, F)) return -1;
-  GatedArgs a{};
-  a.x = (const unsigned short*)x; a.dy = (const unsigned short*)dy; a.h = (unsigned short*)h;
-  a.dg = (unsigned short*)dg; a.du = (unsigned short*)du;
-  a.dwg = dwg; a.dwu = dwu; a.dwd = dwd;
-  a.M = M; a.D = D; a.F = F; a.accumulate = accumulate;
-  return large(3 * F, D) ? launch<256, &gated_dw_kernel<256>>(3 * tiles(F, 256) * tiles(D, 256), a, stream)
-                         : launch<128, &gated_dw_kernel<128>>(3 * tiles(F, 128) * tiles(D, 128), a, stream);
+  a.dg = (unsigned short*)dg; a.du = (unsigned short*)du; a.dx = dx; a.dx32 = dx32;
+  a.dwg = dwg; a.dwu = dwu; a.dwd = dwd; a.dw = dw;
+  a.slabs = slabs;
+  a.M = M; a.D = D; a.F = F; a.Dp = pad8(D); a.Fp = pad8(F);
+  int rc = 0;
+  if (pass & 1) rc = product<Dh>(cut_dh(M, D, F), a, stream);
+  if (rc == 0 && (pass & 1) && dx != nullptr) rc = product<Dx>(cut_dx(M, D, F), a, stream);
+  if (rc == 0 && (pass & 2)) rc = product<Dw>(cut_dw(M, D, F), a, stream);
+  return rc;
 }

@@ -122,6 +122,14 @@ struct Stager {
   }
   static constexpr int KSTEP = PROD == 3 ? 32 : 64;
 
+  // only stages [first, first + n) of the reduction
+  __device__ __forceinline__ void part(int first, int n) {
+    const int end = (first + n) * KSTEP;
+    kdone = first * KSTEP;
+    base += MODE == SLOW ? kdone * ld : (long long)first * 64;
+    k = end < k ? end : k;
+  }
+
   // Staging of one stage: begin, every piece, end.  Stages behind the end of the reduction come out as zeros.
   u32x4 rsrc;
   unsigned kill;
@@ -362,12 +370,12 @@ template <int BM, int BN, int NST = 2> struct Tile {
 
   // Gate / up pairs: columns [0, WN/2) of a wave are gate features, the rest the up features of the same index:
   // f(m, feature, gate[8], up[8]) with tile-relative m and feature.
-  template <class F>
-  __device__ __forceinline__ void store_pairs(char* smem, int wid, int lane, F&& f) {
+  template <int NJ = FM, class F>
+  __device__ __forceinline__ void store_pairs(char* smem, int wid, int lane, F&& f, int j0 = 0) {
     float* const win = reinterpret_cast<float*>(smem + wid * WBYTES);
-    const int wm0 = (wid & 1) * WM, wf0 = (wid >> 1) * (WN / 2);
+    const int wm0 = (wid & 1) * WM + j0 * 16, wf0 = (wid >> 1) * (WN / 2);
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
+    for (int j = 0; j < NJ; ++j) {
 #pragma unroll
       for (int i = 0; i < FN; ++i)
         *reinterpret_cast<f32x4*>(win + (lane & 15) * WPITCH + i * 16 + (lane >> 4) * 4) = acc[i][j];
@@ -387,5 +395,24 @@ template <int BM, int BN, int NST = 2> struct Tile {
     }
   }
 };
+
+constexpr int CUS = 256, SLOTS = 2 * CUS;         // two 128 x 128 blocks run on a CU
+
+// Stages of its reduction that a block does when `tiles` equal 128 x 128 tiles have `ks` stages each: the split with the least rounds of blocks
+// times stages.  A partial tile costs 64 KiB written and read, about 6 stages' time beside the block's own start and end; a block alone on its
+// CU runs its stages in 0.6 of the time it needs beside another.  `time`, if wanted: of the choice, in stages of a full CU.
+inline int chunk_for(long long tiles, int ks, double* time = nullptr) {
+  int best = ks;
+  double least = 1e30;
+  for (int s = 1; s == 1 || s <= ks / 8; ++s) {
+    const long long blocks = tiles * s;
+    if (s > 1 && blocks > 4 * SLOTS) break;
+    const int per = (ks + s - 1) / s;
+    const double t = (double)((blocks + SLOTS - 1) / SLOTS) * (per + 6) * (blocks <= CUS ? 0.6 : 1.0) + (s > 1 ? 6.0 + 0.5 * s : 0.0);
+    if (t < least) { least = t; best = per; }
+  }
+  if (time != nullptr) *time = least;
+  return best;
+}
 
 }  // namespace gt

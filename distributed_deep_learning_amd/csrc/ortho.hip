@@ -660,27 +660,15 @@ __global__ __launch_bounds__(512, 2) void ns_solo_kernel(const NsArgs a, const i
       }
 }
 
-constexpr int CUS = 256, SLOTS = 2 * CUS;         // two 128 x 128 blocks run on a CU
+using gt::CUS;
+using gt::SLOTS;
+using gt::chunk_for;
 constexpr int SLAB = gt::Tile<128, 128>::SLAB;
 
 inline int tri(int thin) { const int t = (thin + 127) / 128; return t * (t + 1) / 2; }
 inline int full(int rows, int cols, int bt) { return ((rows + bt - 1) / bt) * ((cols + bt - 1) / bt); }
 inline int stages(int k, int prod) { return prod == 3 ? (k + 31) / 32 : (k + 63) / 64; }
 
-// Stages of its reduction that a block does when `tiles` equal tiles have `ks` stages each: the split with the least rounds of blocks times
-// stages.  A partial tile costs 64 KiB written and read, about 6 stages' time beside the block's own start and end; a block alone on its
-// CU runs its stages in 0.6 of the time it needs beside another.
-inline int chunk_for(long long tiles, int ks) {
-  int best = ks;
-  double least = 1e30;
-  for (int s = 1; s == 1 || s <= ks / 8; ++s) {
-    const long long blocks = tiles * s;
-    const int per = (ks + s - 1) / s;
-    const double t = (double)((blocks + SLOTS - 1) / SLOTS) * (per + 6) * (blocks <= CUS ? 0.6 : 1.0) + (s > 1 ? 6.0 + 0.5 * s : 0.0);
-    if (t < least) { least = t; best = per; }
-  }
-  return best;
-}
 // X' = a X + B X in 256 x 256 tiles (half the staged bytes per operation) where they alone fill the chip and the reduction is long enough for
 // one block on a CU to hide its ends: 8192 x 2048 fp32 164 us against 183;  8 x 512 x 4608 bf16 (8 stages) 70 us against 44.
 inline bool large_apply(int rows, int cols, long long batch) { return min(rows, cols) >= 1024 && full(rows, cols, 256) * batch >= CUS; }

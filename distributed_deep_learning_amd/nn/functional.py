@@ -950,75 +950,56 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
 
 
 def _weight16(w: torch.Tensor) -> torch.Tensor:
-    """bf16 values of a weight: itself, the arena's shadow when that is current, or a fresh copy."""
-    if w.dtype == BF16:
-        return w.detach()
-    if getattr(w, "_ddl_shadow", None) is not None and getattr(w, "_ddl_shadow_version", -1) == w._version:
+    """The arena's bf16 shadow of an fp32 weight when that is current, else the weight itself."""
+    if w.dtype is not BF16 and getattr(w, "_ddl_shadow", None) is not None and getattr(w, "_ddl_shadow_version", -1) == w._version:
         return w._ddl_shadow
-    return w.detach().to(BF16)
+    return w.detach()
 
 
 class GatedMLP(torch.autograd.Function):
-    """The gated feed-forward block on ``csrc/gated.hip``: two launches forward, three backward.  Use :func:`gated_mlp`.  Gradients of fp32
+    """The gated feed-forward block on ``csrc/gated.hip``: two products forward, three backward.  Use :func:`gated_mlp`.  Gradients of fp32
     weights that live in an arena are added straight into it (on the side stream, like every other weight gradient)."""
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation):
-        D, F_ = x.shape[1], w_gate.shape[0]
-        pd, pf = -D % 8, -F_ % 8                                       # widths that are no multiples of 8: zero columns
-        pad = torch.nn.functional.pad
-        x16 = _bf16(x.detach())
-        wg, wu, wd = (_weight16(w) for w in (w_gate, w_up, w_down))
-        if pd or pf:
-            x16 = pad(x16, (0, pd))
-            wg, wu, wd = pad(wg, (0, pd, 0, pf)), pad(wu, (0, pd, 0, pf)), pad(wd, (0, pf, 0, pd))
-        x16, wg, wu, wd = (K._aligned(t) for t in (x16, wg, wu, wd))
-        train = any(ctx.needs_input_grad[:4])
-        h, keep = K.gated_up(x16, wg, wu, activation, save=train)
-        y = K.gated_down(h, wd)
+        shape, (F_, D) = x.shape, w_gate.shape
+        M = x.numel() // D
+        x2, *w = K.gated_operands((x.reshape(M, D), M, D), (_weight16(w_gate), F_, D), (_weight16(w_up), F_, D), (_weight16(w_down), D, F_))
+        train = any(ctx.needs_input_grad)
+        y, kept = K.gated_fwd(x2, *w, M, D, F_, activation, save=train)
         if train:
-            ctx.save_for_backward(x16, wg, wu, wd, h, *keep)
-            ctx.meta = (D, F_, x.dtype, (w_gate, w_up, w_down))
-        return y[:, :D] if pd else y
+            ctx.save_for_backward(x2, *w, kept)
+            ctx.meta = (M, D, F_, x.dtype, shape, (w_gate, w_up, w_down))
+        return y.view(shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, wg, wu, wd, h, *keep = ctx.saved_tensors
-        D, F_, x_dtype, weights = ctx.meta
+        x, wg, wu, wd, kept = ctx.saved_tensors
+        M, D, F_, x_dtype, shape, weights = ctx.meta
         need = ctx.needs_input_grad
-        padded = x.shape[1] != D or h.shape[1] != F_
         with device_of(x):
-            dy = _bf16(dy)
-            if x.shape[1] != D:
-                dy = torch.nn.functional.pad(dy, (0, x.shape[1] - D))
-            dy = K._aligned(dy)
-            dg = du = dx = None
-            if need[0] or need[1] or need[2]:
-                dg, du = K.gated_dh(dy, wd, keep)
-            if need[0]:
-                dx = K.gated_dx(dg, du, wg, wu)
-                dx = (dx[:, :D] if x.shape[1] != D else dx).to(x_dtype)
-            grads = [None, None, None]
+            dy, = K.gated_operands((dy.reshape(M, D), M, D))
+            dx = torch.empty(shape, dtype=x_dtype, device=x.device) if need[0] else None
+            dgu = K.gated_dh(dy, wg, wu, wd, kept, M, D, F_, dx) if need[0] or need[1] or need[2] else None
             want = [w if n else None for w, n in zip(weights, need[1:4])]
             live = [w for w in want if w is not None]
-            if live:
-                arena = getattr(live[0], "_ddl_arena", None)
-                direct = not padded and arena is not None and all(
-                    getattr(w, "_ddl_arena", None) is arena and arena.grad_is_arena_view(w) and w.grad.is_contiguous() for w in live)
-                if direct:
-                    with streams.fork(x, dy, h, dg, du):
-                        K.gated_dw(x, dy, h, dg, du, [None if w is None else w.grad for w in want], accumulate=True)
-                    for w in reversed(live):
-                        arena.notify_grad_ready(w)
-                else:
-                    fp32 = any(w.dtype == torch.float32 for w in live)
-                    make = torch.zeros_like if fp32 else torch.empty_like
-                    out = [None if w is None else make(w16, dtype=torch.float32 if fp32 else BF16)
-                           for w, w16 in zip(want, (wg, wu, wd))]
-                    K.gated_dw(x, dy, h, dg, du, out, accumulate=fp32)
-                    grads = [None if t is None else t[:w.shape[0], :w.shape[1]].to(w.dtype) for t, w in zip(out, weights)]
-        return dx, *grads, None
+            if not live:
+                return dx, None, None, None, None
+            arena = getattr(live[0], "_ddl_arena", None)
+            if arena is not None and all(getattr(w, "_ddl_arena", None) is arena and arena.grad_is_arena_view(w) and w.grad.is_contiguous()
+                                         for w in live):
+                with streams.fork(x, dy, kept, *([] if dgu is None else [dgu])):
+                    K.gated_dw(x, dy, kept, dgu, [None if w is None else w.grad for w in want], M, D, F_, accumulate=True)
+                for w in reversed(live):
+                    arena.notify_grad_ready(w)
+                return dx, None, None, None, None
+            dtype = BF16 if all(w.dtype is BF16 for w in live) else torch.float32
+            out = [None if w is None else torch.empty(w.shape, dtype=dtype, device=x.device) for w in want]
+            K.gated_dw(x, dy, kept, dgu, out, M, D, F_)
+            if dtype is not BF16:
+                out = [None if w is None else t.to(w.dtype) for w, t in zip(want, out)]
+        return dx, *out, None
 
 
 def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str = "silu") -> torch.Tensor:
@@ -1037,11 +1018,12 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         act = {"silu": torch.nn.functional.silu, "gelu": torch.nn.functional.gelu, "relu": torch.relu}[activation]
         lin = torch.nn.functional.linear
         return lin(act(lin(x, w_gate)) * lin(x, w_up), w_down)
-    if any(t.dtype not in (BF16, torch.float32) for t in (x, w_gate, w_up, w_down)):
-        raise TypeError("gated_mlp: inputs and weights must be bf16 or fp32")
-    if any(t.device != x.device for t in (w_gate, w_up, w_down)):
-        raise ValueError("gated_mlp: inputs and weights must be on one device")
+    for t in (x, w_gate, w_up, w_down):
+        if t.dtype is not BF16 and t.dtype is not torch.float32:
+            raise TypeError("gated_mlp: inputs and weights must be bf16 or fp32")
+        if t.device != x.device:
+            raise ValueError("gated_mlp: inputs and weights must be on one device")
     if D == 0 or w_gate.shape[0] == 0:
         raise ValueError("gated_mlp: empty widths")
     with device_of(x):
-        return GatedMLP.apply(x.reshape(-1, D), w_gate, w_up, w_down, activation).reshape(x.shape)
+        return GatedMLP.apply(x, w_gate, w_up, w_down, activation)

@@ -111,11 +111,10 @@ _SIGS = {
     "ddl_ns_shape": [_i, _i, _i, _i, _ll, _ll, _vp],
     "ddl_orthogonalize": [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _f, _vp],
     "ddl_muon_step": [_vp] * 12 + [_i, _i, _vp, _f, _i, _i, _i, _vp],
-    "ddl_gated_up": [_vp] * 6 + [_i, _i, _i, _i, _vp],
-    "ddl_gated_down": [_vp, _vp, _vp, _i, _i, _i, _vp],
-    "ddl_gated_dh": [_vp] * 6 + [_i, _i, _i, _vp],
-    "ddl_gated_dx": [_vp] * 5 + [_i, _i, _i, _vp],
-    "ddl_gated_dw": [_vp] * 8 + [_i, _i, _i, _i, _vp],
+    "ddl_gated_workspace": [_i, _i, _i, _i],
+    "ddl_gated_pad": [_vp] * 6 + [_i, _vp],
+    "ddl_gated_fwd": [_vp] * 9 + [_i, _i, _i, _i, _vp],
+    "ddl_gated_bwd": [_vp] * 11 + [_i] + [_vp] * 3 + [_i, _vp, _i, _i, _i, _i, _vp],
     "ddl_logprob_top_max": [],
     "ddl_logprob_workspace": [_ll, _i, _i, _i],
     "ddl_logprob_fwd": [_vp, _i, _vp, _ll, _i, _i] + [_vp] * 7,
@@ -124,7 +123,8 @@ _SIGS = {
 
 
 _LONG_RESULT = {"ddl_conv_wgrad_plan", "ddl_conv_c64_launches", "ddl_wgrad_halo_launches", "ddl_ns_workspace",
-                "ddl_ns_shape", "ddl_ns_work", "ddl_logprob_workspace"}
+                "ddl_ns_shape", "ddl_ns_work", "ddl_logprob_workspace",
+                "ddl_gated_workspace"}
 
 
 def _load():

@@ -1236,94 +1236,85 @@ def token_logprobs_bwd(logits, tokens, norm, entropy, g_logp=None, g_entropy=Non
 GATED_ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}        # mirrors csrc/gated.hip
 
 
-def _chk_gated(name: str, **mats):
-    """Every argument: ``(tensor, shape)`` - contiguous 16-byte aligned bf16 on the current GPU."""
-    for k, (t, shape) in mats.items():
-        if t is None:
+def gated_operands(*mats):
+    """``(matrix, rows, cols)`` each, bf16 or fp32 -> the tensors that the gated block's products take: bf16, contiguous, 16-byte aligned,
+    rows padded with zeros to a multiple of 8.  A matrix that is so already comes back itself; the others are copied, in one launch."""
+    out, todo = [], None
+    for i, (t, rows, cols) in enumerate(mats):
+        if t.dtype is BF16 and not cols % 8 and t.is_contiguous() and not t.data_ptr() % 16:
+            out.append(t)
             continue
-        _chk_act(t, f"{name}: {k}")
-        if tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.data_ptr() % 16:
-            raise ValueError(f"{name}: {k} must be a contiguous, 16-byte aligned {tuple(shape)} tensor, got {tuple(t.shape)}")
+        if t.stride(1) != 1:
+            t = t.contiguous()
+        out.append(torch.empty((rows, (cols + 7) // 8 * 8), dtype=BF16, device=t.device))
+        todo = todo or []
+        todo.append((t, out[-1], rows, cols))
+    if todo:
+        import ctypes as C
+        n = len(todo)
+        ints, ptrs = C.c_int * n, C.c_void_p * n
+        check(_lib.require().ddl_gated_pad(
+            ptrs(*(t.data_ptr() for t, _, _, _ in todo)), ptrs(*(o.data_ptr() for _, o, _, _ in todo)), ints(*(r for _, _, r, _ in todo)),
+            ints(*(c for _, _, _, c in todo)), (C.c_longlong * n)(*(t.stride(0) for t, _, _, _ in todo)),
+            ints(*(t.dtype is not BF16 for t, _, _, _ in todo)), n, stream_ptr()), "gated_pad")
+    return out
 
 
-def gated_up(x, w_gate, w_up, activation: str = "silu", save: bool = False):
-    """``h = act(x @ w_gate^T) * (x @ w_up^T)``: ``x`` ``[M, D]``, weights ``[F, D]``, all bf16, ``D`` and ``F`` multiples of 8.
-    Returns ``(h, keep)``: with ``save`` (training) ``keep`` is the pair of tensors :func:`gated_dh` takes - the factors ``u act'(g)``
-    and ``act(g)`` in 24 bits, 16 of them in an int16 and 8 in a uint8 tensor ``[2, M, F]`` - else ``None``."""
+def _gated_slabs(lib, M, D, F_, which, device):
+    n = lib.ddl_gated_workspace(M, D, F_, which)
+    return torch.empty(n, dtype=torch.float32, device=device) if n else None
+
+
+def gated_fwd(x, w_gate, w_up, w_down, M: int, D: int, F_: int, activation: str = "silu", save: bool = False):
+    """``y = (act(x w_gate^T) * (x w_up^T)) w_down^T`` of :func:`gated_operands` (``csrc/gated.hip``).  Returns ``(y, kept)``: ``y`` bf16
+    ``[M, D]``; with ``save`` (training) ``kept`` is the byte tensor that :func:`gated_bwd` takes, for every token and (padded) feature
+    ``h`` in bf16 and the factors ``u act'(g)`` and ``act(g)`` in 24 bits, else ``None``."""
     lib = _lib.require()
-    M, D = x.shape
-    F_ = w_gate.shape[0]
-    if D % 8 or F_ % 8:
-        raise ValueError("gated_up: widths must be multiples of 8")
-    _chk_gated("gated_up", x=(x, (M, D)), w_gate=(w_gate, (F_, D)), w_up=(w_up, (F_, D)))
-    h = torch.empty((M, F_), dtype=BF16, device=x.device)
-    keep = (torch.empty((2, M, F_), dtype=torch.int16, device=x.device),
-            torch.empty((2, M, F_), dtype=torch.uint8, device=x.device)) if save else None
+    _lib.check_device(x, "gated_fwd")
+    n = M * ((F_ + 7) // 8 * 8)
+    y = torch.empty((M, D), dtype=BF16, device=x.device)
+    buf = torch.empty(n * (8 if save else 2), dtype=torch.uint8, device=x.device)
     if M > 0:
-        check(lib.ddl_gated_up(ptr(x), ptr(w_gate), ptr(w_up), ptr(h), ptr(keep[0]) if save else None, ptr(keep[1]) if save else None,
-                               M, D, F_, GATED_ACTIVATIONS[activation], stream_ptr()), "gated_up")
-    return h, keep
+        slabs, h = _gated_slabs(lib, M, D, F_, 0, x.device), buf.data_ptr()
+        check(lib.ddl_gated_fwd(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), h, h + 2 * n if save else None,
+                                h + 6 * n if save else None, y.data_ptr(), ptr(slabs), M, D, F_, GATED_ACTIVATIONS[activation],
+                                stream_ptr()), "gated_fwd")
+    return y, buf if save else None
 
 
-def gated_down(h, w_down):
-    """``y = h @ w_down^T``: ``h`` ``[M, F]``, ``w_down`` ``[D, F]``, bf16."""
+def gated_dh(dy, w_gate, w_up, w_down, kept, M: int, D: int, F_: int, dx=None):
+    """``(dg, du)`` (one bf16 tensor ``[2, M, F padded]``) from ``dy`` (:func:`gated_operands`), and ``dg w_gate + du w_up`` into ``dx``
+    (bf16 or fp32 ``[M, D]``) if that is given."""
     lib = _lib.require()
-    M, F_ = h.shape
-    D = w_down.shape[0]
-    if D % 8 or F_ % 8:
-        raise ValueError("gated_down: widths must be multiples of 8")
-    _chk_gated("gated_down", h=(h, (M, F_)), w_down=(w_down, (D, F_)))
-    y = torch.empty((M, D), dtype=BF16, device=h.device)
+    _lib.check_device(dy, "gated_dh")
+    n = M * ((F_ + 7) // 8 * 8)
+    dgu = torch.empty((2, n), dtype=BF16, device=dy.device)
     if M > 0:
-        check(lib.ddl_gated_down(ptr(h), ptr(w_down), ptr(y), M, D, F_, stream_ptr()), "gated_down")
-    return y
+        slabs, h, dg = _gated_slabs(lib, M, D, F_, 1, dy.device), kept.data_ptr(), dgu.data_ptr()
+        check(lib.ddl_gated_bwd(None, dy.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), h, h + 2 * n, h + 6 * n,
+                                dg, dg + 2 * n, ptr(dx), int(dx is not None and dx.dtype is not BF16), None, None, None, 0, ptr(slabs),
+                                M, D, F_, 1, stream_ptr()), "gated_dh")
+    return dgu
 
 
-def gated_dh(dy, w_down, keep):
-    """``dh = dy @ w_down`` folded straight into ``(dg, du) = (dh u act'(g), dh act(g))``, bf16 ``[M, F]``; ``keep`` from :func:`gated_up`."""
+def gated_dw(x, dy, kept, dgu, out, M: int, D: int, F_: int, accumulate: bool = False):
+    """Weight gradients ``dg^T x``, ``du^T x`` (``[F, D]``) and ``dy^T h`` (``[D, F]``) in one launch into the three contiguous tensors of
+    ``out`` (``None``: not wanted): all bf16 or all fp32, overwritten or, ``accumulate`` (fp32), added to."""
     lib = _lib.require()
-    M, D = dy.shape
-    F_ = w_down.shape[1]
-    _chk_gated("gated_dh", dy=(dy, (M, D)), w_down=(w_down, (D, F_)))
-    for t, dt in zip(keep, (torch.int16, torch.uint8)):
-        if tuple(t.shape) != (2, M, F_) or t.dtype != dt or not t.is_contiguous() or t.device != dy.device:
-            raise ValueError("gated_dh: keep must be what gated_up(save=True) returned for these sizes")
-    dg, du = (torch.empty((M, F_), dtype=BF16, device=dy.device) for _ in range(2))
-    if M > 0:
-        check(lib.ddl_gated_dh(ptr(dy), ptr(w_down), ptr(keep[0]), ptr(keep[1]), ptr(dg), ptr(du), M, D, F_, stream_ptr()), "gated_dh")
-    return dg, du
-
-
-def gated_dx(dg, du, w_gate, w_up):
-    """``dx = dg @ w_gate + du @ w_up`` (one reduction over both), bf16 ``[M, D]``."""
-    lib = _lib.require()
-    M, F_ = dg.shape
-    D = w_gate.shape[1]
-    _chk_gated("gated_dx", dg=(dg, (M, F_)), du=(du, (M, F_)), w_gate=(w_gate, (F_, D)), w_up=(w_up, (F_, D)))
-    dx = torch.empty((M, D), dtype=BF16, device=dg.device)
-    if M > 0:
-        check(lib.ddl_gated_dx(ptr(dg), ptr(du), ptr(w_gate), ptr(w_up), ptr(dx), M, D, F_, stream_ptr()), "gated_dx")
-    return dx
-
-
-def gated_dw(x, dy, h, dg, du, out, accumulate: bool = False):
-    """Weight gradients ``dg^T x``, ``du^T x`` (``[F, D]``) and ``dy^T h`` (``[D, F]``) in one launch into the three tensors of ``out``
-    (``None``: not wanted): bf16, overwritten, or with ``accumulate`` fp32, added to (arena gradients)."""
-    lib = _lib.require()
-    M, D = x.shape
-    F_ = h.shape[1]
-    _chk_gated("gated_dw", x=(x, (M, D)), dy=(dy, (M, D)), h=(h, (M, F_)), dg=(dg, (M, F_)), du=(du, (M, F_)))
-    want = torch.float32 if accumulate else BF16
+    _lib.check_device(x, "gated_dw")
+    live = [t for t in out if t is not None]
+    kind = 0 if live[0].dtype is BF16 else 1 if accumulate else 2
     for t, shape in zip(out, ((F_, D), (F_, D), (D, F_))):
-        if t is not None and (t.dtype != want or tuple(t.shape) != shape or not t.is_contiguous() or t.data_ptr() % 16):
-            raise ValueError(f"gated_dw: outputs must be contiguous, 16-byte aligned {want} tensors {shape}")
+        if t is not None and (t.dtype is not (torch.float32 if kind else BF16) or tuple(t.shape) != shape or not t.is_contiguous() or t.data_ptr() % 16):
+            raise ValueError(f"gated_dw: outputs must be contiguous, 16-byte aligned tensors {shape} of one dtype, added to only in fp32")
     if M > 0:
-        check(lib.ddl_gated_dw(ptr(x), ptr(dy), ptr(h), ptr(dg), ptr(du), ptr(out[0]), ptr(out[1]), ptr(out[2]), M, D, F_,
-                               int(accumulate), stream_ptr()), "gated_dw")
+        n = M * ((F_ + 7) // 8 * 8)
+        slabs, dg = _gated_slabs(lib, M, D, F_, 2, x.device), ptr(dgu)
+        check(lib.ddl_gated_bwd(x.data_ptr(), dy.data_ptr(), None, None, None, kept.data_ptr(), None, None, dg, dg + 2 * n if dg else None, None, 0,
+                                *(ptr(t) for t in out), kind, ptr(slabs), M, D, F_, 2, stream_ptr()), "gated_dw")
     elif not accumulate:
-        for t in out:
-            if t is not None:
-                t.zero_()
+        for t in live:
+            t.zero_()
 
 
 # ----------------------------------------------------------------------------------------------- orthogonalisation
