@@ -177,9 +177,11 @@ template <int BT, int NST, bool JOIN> struct Block {
   static constexpr bool SPLIT = BT == 128 && !JOIN;
   T tile;
   int tid, lane, wid, t, part;                    // t: the tile;  part: of its reduction (JOIN: its row group)
-  __device__ __forceinline__ void begin(const GatedArgs& a) {
+  // `products` of equal grids one after the other: all XCDs work on one at a time and share its operands behind their L2s
+  __device__ __forceinline__ void begin(const GatedArgs& a, unsigned products = 1) {
     tid = threadIdx.x; lane = tid & 63; wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-    t = (int)xcd_remap(blockIdx.x, gridDim.x); part = 0;
+    const unsigned each = gridDim.x / products, before = blockIdx.x / each * each;
+    t = (int)(before + xcd_remap(blockIdx.x - before, each)); part = 0;
     if (JOIN) { part = t % T::FM; t /= T::FM; }
     else if (SPLIT && a.splits > 1) { part = t % a.splits; t /= a.splits; }
   }
@@ -315,7 +317,7 @@ template <int BT, int NST, bool JOIN> __global__ GATED_BOUNDS void gated_dx_kern
 template <int BT, int NST, bool JOIN> __global__ GATED_BOUNDS void gated_dw_kernel(const GatedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   Block<BT, NST, JOIN> b;
-  b.begin(a);
+  b.begin(a, 3);
   const int tf = (a.F + BT - 1) / BT, td = (a.D + BT - 1) / BT, each = tf * td, which = b.t / each;
   int ti, tj;
   tile_of((unsigned)(b.t - which * each), which == 2 ? td : tf, which == 2 ? tf : td, ti, tj);
