@@ -896,7 +896,7 @@ class TokenLogProbs(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, tokens, top):
-        logp, ent, norm, tv, ti = K.token_logprobs_fwd(logits, tokens, top)
+        logp, ent, norm, tv, ti = K.token_logprobs_fwd(logits, tokens, top, train=True)
         ctx.save_for_backward(logits, tokens, norm, ent, ti)
         ctx.mark_non_differentiable(ti)
         ctx.set_materialize_grads(False)
@@ -942,7 +942,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
     z, t = logits.reshape(-1, V), tokens.reshape(-1)
     if logits.is_cuda:
         with device_of(logits):
-            out = TokenLogProbs.apply(z, t, int(top))
+            if z.requires_grad and torch.is_grad_enabled():
+                out = TokenLogProbs.apply(z, t, int(top))
+            else:
+                logp, ent, _, tv, ti = K.token_logprobs_fwd(z, t, int(top))
+                out = logp, ent, tv, ti
     else:
         out = _token_logprobs_cpu(z, t, int(top))
     logp, ent, tv, ti = out
@@ -956,21 +960,24 @@ def _weight16(w: torch.Tensor) -> torch.Tensor:
     return w.detach()
 
 
+def _gated_forward(x, w_gate, w_up, w_down, activation, train):
+    shape, (F_, D) = x.shape, w_gate.shape
+    M = x.numel() // D
+    ops = K.gated_operands((x.detach().reshape(M, D), M, D), (_weight16(w_gate), F_, D), (_weight16(w_up), F_, D), (_weight16(w_down), D, F_))
+    y, kept = K.gated_fwd(*ops, M, D, F_, activation, save=train)
+    return y.view(shape), (*ops, kept), (M, D, F_)
+
+
 class GatedMLP(torch.autograd.Function):
     """The gated feed-forward block on ``csrc/gated.hip``: two products forward, three backward.  Use :func:`gated_mlp`.  Gradients of fp32
     weights that live in an arena are added straight into it (on the side stream, like every other weight gradient)."""
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation):
-        shape, (F_, D) = x.shape, w_gate.shape
-        M = x.numel() // D
-        x2, *w = K.gated_operands((x.reshape(M, D), M, D), (_weight16(w_gate), F_, D), (_weight16(w_up), F_, D), (_weight16(w_down), D, F_))
-        train = any(ctx.needs_input_grad)
-        y, kept = K.gated_fwd(x2, *w, M, D, F_, activation, save=train)
-        if train:
-            ctx.save_for_backward(x2, *w, kept)
-            ctx.meta = (M, D, F_, x.dtype, shape, (w_gate, w_up, w_down))
-        return y.view(shape)
+        y, saved, sizes = _gated_forward(x, w_gate, w_up, w_down, activation, True)
+        ctx.save_for_backward(*saved)
+        ctx.meta = (*sizes, x.dtype, x.shape, (w_gate, w_up, w_down))
+        return y
 
     @staticmethod
     @once_differentiable
@@ -1026,4 +1033,6 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     if D == 0 or w_gate.shape[0] == 0:
         raise ValueError("gated_mlp: empty widths")
     with device_of(x):
-        return GatedMLP.apply(x, w_gate, w_up, w_down, activation)
+        if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
+            return GatedMLP.apply(x, w_gate, w_up, w_down, activation)
+        return _gated_forward(x, w_gate, w_up, w_down, activation, False)[0]

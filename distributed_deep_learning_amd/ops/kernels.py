@@ -1178,10 +1178,12 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def token_logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
+def token_logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, train: bool = False):
     """``logits`` bf16 / fp32 ``[N, V]``, ``tokens`` int64 ``[N]`` -> fp32 ``(logp [N], entropy [N], norm [N, 2],
     top_logp [N, top])`` and int64 ``top_index [N, top]`` (descending, equal values by the lowest index), one pass over the logits
-    (``csrc/logprob.hip``); ``norm`` is what the backward pass needs: the row's maximum and the log of its sum.  A token outside ``[0, V)`` (padding) gives log probability 0."""
+    (``csrc/logprob.hip``); ``norm`` is what the backward pass needs: the row's
+    maximum and the log of its sum.  A token outside ``[0, V)`` (padding) gives log probability 0.  ``train``: a backward pass follows, what of
+    the logits fits the memory-side cache is left there for it."""
     lib = _lib.require()
     if logits.dtype not in (BF16, torch.float32):
         raise TypeError(f"token_logprobs: logits must be bf16 or fp32, got {logits.dtype}")
@@ -1206,7 +1208,7 @@ def token_logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0)
     if N > 0:
         is16 = int(logits.dtype == BF16)
         ws = torch.empty(lib.ddl_logprob_workspace(N, V, is16, top), dtype=torch.uint8, device=dev)
-        check(lib.ddl_logprob_fwd(ptr(logits), is16, ptr(tokens), N, V, top, ptr(ws), ptr(logp), ptr(ent), ptr(norm), ptr(tv), ptr(ti),
+        check(lib.ddl_logprob_fwd(ptr(logits), is16, ptr(tokens), N, V, top, int(train), ptr(ws), ptr(logp), ptr(ent), ptr(norm), ptr(tv), ptr(ti),
                                   stream_ptr()), "token_logprobs")
     return logp, ent, norm, tv, ti
 
