@@ -185,7 +185,7 @@ __device__ __forceinline__ u64 block_max(u64 v, u64* red) {              // red[
   return r;
 }
 
-// norm: (m, log s) of every row; their sum is lse, but far from zero it would swallow log s
+// norm (null: not wanted): (m, log s) of every row; their sum is lse, but far from zero it would swallow log s
 struct Outs { float* logp; float* ent; float* norm; float* top; long long* idx; };
 
 // thread 0 writes the row's scalars, threads < k its list
@@ -198,8 +198,10 @@ __device__ __forceinline__ void finish_row(const Stat& st, const T* row, long lo
     const float zt = in ? Io<T>::one(row + token) : 0.f;
     o.logp[r] = in ? (empty ? -INFINITY : (zt - st.m) - ls) : 0.f;
     o.ent[r] = empty ? 0.f : ls - st.q / st.s;
-    o.norm[2 * r] = st.m;
-    o.norm[2 * r + 1] = empty ? -INFINITY : ls;
+    if (o.norm != nullptr) {
+      o.norm[2 * r] = st.m;
+      o.norm[2 * r + 1] = empty ? -INFINITY : ls;
+    }
   }
   if ((int)threadIdx.x < k) {
     const float z = value_of((unsigned)(mine >> 32));
@@ -541,10 +543,11 @@ extern "C" long long ddl_logprob_workspace(long long rows, int V, int is_bf16, i
   if (rows <= 0 || V <= 0 || k < 0 || k > TOP_MAX) return -1;
   int per;
   const long long parts = parts_for(rows, V, is_bf16, k, &per);
-  if (parts <= 1) return 16;
+  if (parts <= 1) return 0;
   return (rows * parts * (long long)sizeof(Stat) + 15) / 16 * 16 + rows * parts * k * 8;
 }
 
+// ws: null where ddl_logprob_workspace is 0;  train: norm is wanted, a backward call follows
 extern "C" int ddl_logprob_fwd(const void* z, int is_bf16, const long long* tokens, long long rows, int V, int k, int train, void* ws, float* logp,
                                float* ent, float* norm, float* top, long long* idx, void* stream) {
   if (rows <= 0 || V <= 0 || V > 0x7fffff00 || k < 0 || k > TOP_MAX || k > V) return -1;

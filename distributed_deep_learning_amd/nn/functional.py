@@ -939,7 +939,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
     lead, V = logits.shape[:-1], logits.shape[-1]
     if not 0 <= top <= min(V, K.LOGPROB_MAX_TOP):
         raise ValueError(f"token_logprobs: top must be between 0 and min(V, {K.LOGPROB_MAX_TOP}), got {top} with V = {V}")
-    z, t = logits.reshape(-1, V), tokens.reshape(-1)
+    flat = len(lead) == 1
+    z, t = (logits, tokens) if flat else (logits.reshape(-1, V), tokens.reshape(-1))
     if logits.is_cuda:
         with device_of(logits):
             if z.requires_grad and torch.is_grad_enabled():
@@ -949,6 +950,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
                 out = logp, ent, tv, ti
     else:
         out = _token_logprobs_cpu(z, t, int(top))
+    if flat:
+        return out
     logp, ent, tv, ti = out
     return logp.reshape(lead), ent.reshape(lead), tv.reshape(*lead, top), ti.reshape(*lead, top)
 

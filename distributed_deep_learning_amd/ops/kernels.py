@@ -1179,9 +1179,9 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 
 def token_logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, train: bool = False):
-    """``logits`` bf16 / fp32 ``[N, V]``, ``tokens`` int64 ``[N]`` -> fp32 ``(logp [N], entropy [N], norm [N, 2],
+    """``logits`` bf16 / fp32 ``[N, V]``, ``tokens`` int64 ``[N]`` -> fp32 ``(logp [N], entropy [N], norm [N, 2] or None,
     top_logp [N, top])`` and int64 ``top_index [N, top]`` (descending, equal values by the lowest index), one pass over the logits
-    (``csrc/logprob.hip``); ``norm`` is what the backward pass needs: the row's
+    (``csrc/logprob.hip``); ``norm`` (with ``train``) is what the backward pass needs: the row's
     maximum and the log of its sum.  A token outside ``[0, V)`` (padding) gives log probability 0.  ``train``: a backward pass follows, what of
     the logits fits the memory-side cache is left there for it."""
     lib = _lib.require()
@@ -1201,13 +1201,14 @@ def token_logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
         raise ValueError("token_logprobs: the vocabulary is empty")
     logits, tokens = logits.contiguous(), tokens.contiguous()
     dev = logits.device
-    logp, ent = (torch.empty(N, dtype=torch.float32, device=dev) for _ in range(2))
-    norm = torch.empty((N, 2), dtype=torch.float32, device=dev)
+    logp, ent = torch.empty(N, dtype=torch.float32, device=dev), torch.empty(N, dtype=torch.float32, device=dev)
+    norm = torch.empty((N, 2), dtype=torch.float32, device=dev) if train else None
     tv = torch.empty((N, top), dtype=torch.float32, device=dev)
     ti = torch.empty((N, top), dtype=torch.int64, device=dev)
     if N > 0:
         is16 = int(logits.dtype == BF16)
-        ws = torch.empty(lib.ddl_logprob_workspace(N, V, is16, top), dtype=torch.uint8, device=dev)
+        ws = lib.ddl_logprob_workspace(N, V, is16, top)
+        ws = torch.empty(ws, dtype=torch.uint8, device=dev) if ws else None
         check(lib.ddl_logprob_fwd(ptr(logits), is16, ptr(tokens), N, V, top, int(train), ptr(ws), ptr(logp), ptr(ent), ptr(norm), ptr(tv), ptr(ti),
                                   stream_ptr()), "token_logprobs")
     return logp, ent, norm, tv, ti
