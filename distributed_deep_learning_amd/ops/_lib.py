@@ -113,7 +113,7 @@ _SIGS = {
     "ddl_muon_step": [_vp] * 12 + [_i, _i, _vp, _f, _i, _i, _i, _vp],
     "ddl_gated_workspace": [_i, _i, _i, _i],
     "ddl_gated_pad": [_vp] * 6 + [_i, _vp],
-    "ddl_gated_fwd": [_vp] * 9 + [_i, _i, _i, _i, _vp],
+    "ddl_gated_fwd": [_vp] * 10 + [_i, _i, _i, _i, _vp],
     "ddl_gated_bwd": [_vp] * 11 + [_i] + [_vp] * 3 + [_i, _vp, _i, _i, _i, _i, _vp],
     "ddl_logprob_top_max": [],
     "ddl_logprob_workspace": [_ll, _i, _i, _i],

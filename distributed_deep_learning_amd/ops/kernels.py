@@ -1276,11 +1276,12 @@ def gated_fwd(x, w_gate, w_up, w_down, M: int, D: int, F_: int, activation: str 
     _lib.check_device(x, "gated_fwd")
     n = M * ((F_ + 7) // 8 * 8)
     y = torch.empty((M, D), dtype=BF16, device=x.device)
-    buf = torch.empty(n * (8 if save else 2), dtype=torch.uint8, device=x.device)
+    size = n * (8 if save else 2)
+    buf = torch.empty(size + (2 * n if M <= 8 else 0), dtype=torch.uint8, device=x.device)
     if M > 0:
         slabs, h = _gated_slabs(lib, M, D, F_, 0, x.device), buf.data_ptr()
-        check(lib.ddl_gated_fwd(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), h, h + 2 * n if save else None,
-                                h + 6 * n if save else None, y.data_ptr(), ptr(slabs), M, D, F_, GATED_ACTIVATIONS[activation],
+        check(lib.ddl_gated_fwd(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), h, h + size if M <= 8 else None,
+                                h + 2 * n if save else None, h + 6 * n if save else None, y.data_ptr(), ptr(slabs), M, D, F_, GATED_ACTIVATIONS[activation],
                                 stream_ptr()), "gated_fwd")
     return y, buf if save else None
 
