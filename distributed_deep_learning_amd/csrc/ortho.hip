@@ -720,9 +720,10 @@ inline float chain_scale(const float* abc) {
   while (q >= 256.f && f * f * f * q > 60000.f) q *= 0.5f;
   return f * 4096.f < 60000.f && q >= 256.f ? q : 0.f;
 }
-// A set of matrices: operations in chains (6 m^2 n + 14 m^3 each) against single steps (15 m^2 n + 5 m^3).  Chains are 18 launches instead of 15
-// and their m x m products fill the chip less.
-inline bool use_chains(double chained, double single) { return chained <= 0.8 * single; }
+// A set of matrices: operations in chains (6 m^2 n + 14 m^3 each) against single steps (15 m^2 n + 5 m^3).  Chains are 18 launches instead of 15,
+// and up to 4 more that join: some 35 us where all of them are short, what 1e10 operations take with split operands; and their m x m products
+// fill the chip less.  (LeNet-5's Muon step 179 us in chains, 162 in single steps;  8192 x 2048 1205 us against 1760.)
+inline bool use_chains(double chained, double single) { return chained <= 0.8 * single && single - chained > 1e10; }
 inline double chained_work(double thin, double wide) { return 6 * thin * thin * wide + 14 * thin * thin * thin; }
 inline double single_work(double thin, double wide) { return 15 * thin * thin * wide + 5 * thin * thin * thin; }
 
