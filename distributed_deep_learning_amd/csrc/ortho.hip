@@ -572,7 +572,9 @@ __global__ __launch_bounds__(512, 2) void ns_solo_kernel(const NsArgs a, const i
     }
   };
   const int off_c = L::contig(row0, col0), off_s = L::slow(row0, col0);
-  auto put_contig = [&](char* buf, const f32x4 (*v)[2]) {
+  // cols: of the operand.  What no product reads is not written (whole 64 x 32 parts; a product reads up to a multiple of KSTEP columns).
+  auto put_contig = [&](char* buf, const f32x4 (*v)[2], int cols) {
+    if (wm * 64 >= thin || wn * 32 >= (cols + L::KSTEP - 1) / L::KSTEP * L::KSTEP) return;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -581,7 +583,8 @@ __global__ __launch_bounds__(512, 2) void ns_solo_kernel(const NsArgs a, const i
         solo_put<PROD>(buf + j * L::ROWS16, off, off ^ 64, v[j][i]);
       }
   };
-  auto put_slow = [&](char* buf, const f32x4 (*v)[2]) {
+  auto put_slow = [&](char* buf, const f32x4 (*v)[2], int cols) {
+    if (wm * 64 >= thin || wn * 32 >= cols) return;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -597,7 +600,7 @@ __global__ __launch_bounds__(512, 2) void ns_solo_kernel(const NsArgs a, const i
     clear();
 #pragma unroll
     for (int t = 0; t < NT; ++t) {                                      // S = X X^T
-      put_contig(t & 1 ? buf1 : buf0, x[t]);
+      put_contig(t & 1 ? buf1 : buf0, x[t], wide - t * 128);
       __syncthreads();                                                  // the other buffer's readers passed the previous barrier
       mul(t & 1 ? buf1 : buf0, t & 1 ? buf1 : buf0, No{}, wide - t * 128, thin);
     }
@@ -608,7 +611,7 @@ __global__ __launch_bounds__(512, 2) void ns_solo_kernel(const NsArgs a, const i
       for (int i = 0; i < 2; ++i) sv[j][i] = acc[j][i] * UNSCALE;
     char* const bs = NT & 1 ? buf1 : buf0;                              // not read since the last barrier
     char* const bb = NT & 1 ? buf0 : buf1;
-    put_contig(bs, sv);
+    put_contig(bs, sv, thin);
     __syncthreads();
     clear();
     mul(bs, bs, No{}, thin, thin);                                                  // B = b S + c S S
@@ -616,11 +619,11 @@ __global__ __launch_bounds__(512, 2) void ns_solo_kernel(const NsArgs a, const i
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int i = 0; i < 2; ++i) sv[j][i] = sv[j][i] * cb + acc[j][i] * (cc * UNSCALE);
-    put_contig(bb, sv);
+    put_contig(bb, sv, thin);
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < NT; ++t) {                                      // X = a X + B X
-      put_slow(bs, x[t]);
+      put_slow(bs, x[t], wide - t * 128);
       __syncthreads();
       clear();
       mul(bb, bs, Yes{}, thin, wide - t * 128);
