@@ -695,3 +695,119 @@ def test_gated_mlp_large_tiles(T, D, H):
     for o, q in zip(got, ref):
         rows = (o.float() - q).norm(dim=1) / q.norm(dim=1)
         assert torch.isfinite(o).all() and float(rows.max()) <= 4 * B8, float(rows.max())
+
+
+@gpu
+@pytest.mark.parametrize("case", [(70, 2056, 136, "silu"), (200, 136, 2056, "gelu"), (1500, 130, 100, "silu"), (515, 100, 1501, "relu"),
+                                  (66, 1500, 1100, "silu"), (1030, 24, 40, "gelu")])
+def test_gated_mlp_shared_reductions_and_widths_that_need_padding(case):
+    """Few tiles and long reductions (blocks share them and a second launch adds the parts), in bf16 and with fp32 leaves."""
+    T, D, H, act = case
+    (x, wg, wu, wd, dy), ref, tol = _gated_case(T, D, H, act, seed=71)
+    for dtype in (BF, torch.float32):
+        leaves = [t.cuda().to(dtype).requires_grad_() for t in (x, wg, wu, wd)]
+        y = F.gated_mlp(*leaves, activation=act)
+        assert y.dtype == BF and y.is_contiguous()
+        _check(y, ref["y"], tol["y"], "y")
+        for k, t in zip(("dx", "dwg", "dwu", "dwd"), torch.autograd.grad(y, leaves, dy.cuda())):
+            assert t.dtype == dtype and t.is_contiguous()
+            _check(t, ref[k], tol[k], k)
+
+
+@gpu
+@pytest.mark.parametrize("D,H", [(33, 50), (64, 90)])
+def test_gated_mlp_arena_gradients_at_odd_widths_leave_their_neighbours(D, H):
+    (x, wg, wu, wd, dy), ref, tol = _gated_case(77, D, H, "silu", seed=81)
+    m = dnn.GatedMLP(D, H).cuda()
+    arena = ParamArena(m.named_parameters())
+    with torch.no_grad():
+        for p, w in zip((m.gate.weight, m.up.weight, m.down.weight), (wg, wu, wd)):
+            p.copy_(w)
+    arena.sync_shadow()
+    for n in (1, 2):
+        m(x.cuda()).backward(dy.cuda())
+        for p, k in zip((m.gate.weight, m.up.weight, m.down.weight), ("dwg", "dwu", "dwd")):
+            _check(p.grad, n * ref[k], n * tol[k], k)
+    torch.cuda.synchronize()
+    for s in arena.segments:                                                       # the padding behind a matrix
+        assert float(arena.grad[s.offset + s.numel:s.offset + s.padded].abs().sum()) == 0.0
+
+
+@gpu
+def test_gated_mlp_captured_graphs_and_streams_do_not_share_workspaces():
+    cases = [_gated_case(T, D, H, "silu", seed=90 + T) for T, D, H in ((200, 136, 2056), (3, 136, 2056))]
+    dev = [[t.cuda() for t in c[0][:4]] for c in cases]
+    eager = [F.gated_mlp(*t) for t in dev]
+    graphs, outs = [], []
+    for t in dev:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(F.gated_mlp(*t))
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        for g in graphs:
+            g.replay()
+        mid = F.gated_mlp(*dev[0])
+        torch.cuda.synchronize()
+        assert torch.equal(mid, eager[0]) and all(torch.equal(o, e) for o, e in zip(outs, eager))
+    streams = [torch.cuda.Stream() for _ in dev]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(F.gated_mlp(*dev[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, e) for g, e in zip(got, eager) for o in g)
+
+
+@gpu
+def test_gated_mlp_offsets_past_32_bits():
+    T, D, H = 180_000, 64, 12_288                                                  # T * H: 2.2e9 hidden values
+    (x, wg, wu, wd, dy), ref, tol = _gated_case(40, D, H, "silu", seed=95)
+    xl = torch.zeros(T, D, dtype=BF, device="cuda")
+    dyl = torch.zeros(T, D, dtype=BF, device="cuda")
+    xl[-40:], dyl[-40:] = x.cuda(), dy.cuda()
+    leaves = [xl.requires_grad_(), *(t.cuda().requires_grad_() for t in (wg, wu, wd))]
+    y = F.gated_mlp(*leaves)
+    grads = torch.autograd.grad(y, leaves, dyl)
+    _check(y[-40:], ref["y"], tol["y"], "y")
+    _check(grads[0][-40:], ref["dx"], tol["dx"], "dx")
+    assert float(y[:-40].abs().max()) == 0.0 and float(grads[0][:-40].abs().max()) == 0.0
+    for k, t in zip(("dwg", "dwu", "dwd"), grads[1:]):                             # the other tokens are zero: the sums' own error stays
+        _check(t, ref[k], tol[k], k)
+
+
+@gpu
+@pytest.mark.parametrize("name,N,V", [("bf16", 520, 262147), ("fp32", 530, 131075), ("bf16", 66_000, 32_768)])
+def test_token_logprobs_of_logits_beyond_the_caches(name, N, V):
+    """More than 256 MiB of logits (streamed), rows at odd addresses, and more than 2^31 of them; rows at both ends and inside are checked."""
+    gen = torch.Generator(device="cuda").manual_seed(V)
+    z = torch.randn(N, V, generator=gen, device="cuda", dtype=DT[name]).requires_grad_()
+    tok = torch.randint(0, V, (N,), generator=gen, device="cuda")
+    rows = torch.tensor([0, 1, N // 2, N - 2, N - 1])
+    zr, tr = z.detach()[rows.cuda()].cpu(), tok[rows.cuda()].cpu()
+    ref = _logp64(zr, tr, 3)
+    with torch.no_grad():
+        _check_logp([o[rows.cuda()] for o in F.token_logprobs(z, tok, 3)], ref)
+        _check_logp([o[rows.cuda()] for o in F.token_logprobs(z, tok)], _logp64(zr, tr, 0))
+    out = F.token_logprobs(z, tok, 3)
+    _check_logp([o[rows.cuda()] for o in out], ref)
+    gl, gt = torch.randn(N, generator=gen, device="cuda"), torch.randn(N, 3, generator=gen, device="cuda")
+    (dz,) = torch.autograd.grad([out[0], out[2]], z, [gl, gt])
+    want = _logp_grad64(zr, tr, ref[3], gl[rows.cuda()].cpu(), None, gt[rows.cuda()].cpu())
+    size = (gl.abs() + gt.abs().sum(1))[rows.cuda()].cpu().double()[:, None]
+    # as in test_token_logprobs_match_64_bits: a thread adds at most 128 terms, then the sums of its 8 turns, so SUM holds at these lengths
+    tol = (B8 if name == "bf16" else 8 * H24) * want.abs() + 4 * SUM * size * _logp64(zr, tr, 0)[4] + 4 * H24 * size
+    assert float(((dz[rows.cuda()].cpu().double() - want).abs() - tol).max()) <= 0.0
+
+
+@gpu
+def test_orthogonalize_offsets_past_32_bits():
+    g = torch.randn(540, 2000, 2008, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda", dtype=BF)
+    out = K.orthogonalize(g)
+    for i in (0, 535, 539):                                                        # 2^31 elements end in matrix 534
+        ref = _orth64(g[i].double())
+        assert float((out[i].double() - ref).norm()) <= ORTH_TOL["bf16"] * float(ref.norm()), i
