@@ -104,11 +104,11 @@ _SIGS = {
     "ddl_ns_workspace": [_i, _i, _i],
     "ddl_ns_max_parts": [],
     "ddl_ns_mat_bytes": [],
-    "ddl_ns_work": [_i, _i, _i, _i],
+    "ddl_ns_chunks": [_vp, _vp, _i, _i, _vp],
     "ddl_ns_solo": [_i, _i],
     "ddl_ns_prod": [_i, _i, _i],
     "ddl_ns_chains": [_vp, _vp, _i],
-    "ddl_ns_shape": [_i, _i, _i, _i, _ll, _ll, _vp],
+    "ddl_ns_shape": [_i, _i, _i, _i, _i, _i, _vp],
     "ddl_orthogonalize": [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _f, _vp],
     "ddl_muon_step": [_vp] * 12 + [_i, _i, _vp, _f, _i, _i, _i, _vp],
     "ddl_gated_workspace": [_i, _i, _i, _i],
@@ -123,7 +123,7 @@ _SIGS = {
 
 
 _LONG_RESULT = {"ddl_conv_wgrad_plan", "ddl_conv_c64_launches", "ddl_wgrad_halo_launches", "ddl_ns_workspace",
-                "ddl_ns_shape", "ddl_ns_work", "ddl_logprob_workspace",
+                "ddl_ns_shape", "ddl_logprob_workspace",
                 "ddl_gated_workspace"}
 
 

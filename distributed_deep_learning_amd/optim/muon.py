@@ -91,11 +91,13 @@ class Muon(_ArenaOptimizer):
         table, launches = np.zeros(len(self.matrices), dtype=rec), [[] for _ in range(8)]
         ws, slabs, out = 0, 0, (C.c_int * 10)()
         solo = all(lib.ddl_ns_solo(rows, cols) for _, rows, cols, _ in self.matrices)        # every matrix fits a CU: one launch for all
-        work = [sum(lib.ddl_ns_work(rows, cols, prod, square) for _, rows, cols, _ in self.matrices) for square in (0, 1)]
+        sides = [(C.c_int * len(self.matrices))(*(f(rows, cols) for _, rows, cols, _ in self.matrices)) for f in (min, max)]
+        chunks = (C.c_int * 2)()
+        _lib.check(lib.ddl_ns_chunks(*sides, len(self.matrices), prod, chunks), "ns_chunks")
         # long reductions first: the blocks that run longest start first
         for i in sorted(range(len(self.matrices)), key=lambda i: -max(self.matrices[i][1], self.matrices[i][2])):
             s, rows, cols, scale = self.matrices[i]
-            need = lib.ddl_ns_shape(rows, cols, prod, 1, *work, out)
+            need = lib.ddl_ns_shape(rows, cols, prod, 1, *chunks, out)
             if need < 0:
                 raise RuntimeError(f"Muon: no plan for a {rows} x {cols} matrix")
             table[i] = (s.offset, ws, slabs, rows, cols, s.index, scale, out[0], out[1])
@@ -104,7 +106,6 @@ class Muon(_ArenaOptimizer):
                 slabs += need
             for m, n in zip(launches, [1] + [0] * 7 if solo else out[2:10]):
                 m.append(np.stack([np.full(n, i, dtype=np.int32), np.arange(n, dtype=np.int32)], 1))
-        sides = [(C.c_int * len(self.matrices))(*(f(rows, cols) for _, rows, cols, _ in self.matrices)) for f in (min, max)]
         dev = self.arena.device
         maps = np.concatenate([np.concatenate(m) for m in launches])
         return {"table": torch.from_numpy(table.view(np.uint8).copy()).to(dev), "maps": torch.from_numpy(np.ascontiguousarray(maps)).to(dev),
