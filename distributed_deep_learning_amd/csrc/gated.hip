@@ -13,6 +13,8 @@
 // only scale dh, so they need not be rounded twice as coarsely as that: they are kept in 24 bits (the upper 16 bits of the fp32 value in
 // one plane, the next 8 in another; half-step 2^-17), 2 bytes more per feature and token than bf16 copies of g and u, which would add
 // two more roundings of 2^-9 to every gradient (measured: relative error of dx, dWg, dWu 0.0031 with g and u in bf16, 0.0024 so).
+// Few tokens leave few roundings to average over, and little work: up to 64 tokens h, dg and du are pairs of bf16 values (16 bits; what the
+// rounding left is a second plane) and their products run over both planes, so that results have no rounding but their own (0.0017).
 #include "common.h"
 #include "host_util.h"
 #include "gemm_tile.h"
@@ -113,24 +115,29 @@ template <int BN> struct PairStager {
   }
 };
 
-// Two operands of the same shape one after the other along the reduction.
-template <class S> struct Twice {
+// N operands of the same shape one after the other along the reduction: p0, p1, p0 + step, p1 + step.
+template <class S, int N> struct Series {
   static constexpr int NP = S::NP;
   S s;
-  const unsigned short* second;
-  int left;                                       // stages of the first
+  const unsigned short *p0, *p1;
+  long long step;
+  int stages, left, seg;                          // stages of each;  of this one to come;  this one
+  __device__ __forceinline__ void start(const unsigned short* a, const unsigned short* b, long long st, int nk) {
+    p0 = a; p1 = b; step = st; stages = left = nk; seg = 0;
+  }
+  __device__ __forceinline__ const unsigned short* base() const { return ((seg & 1) ? p1 : p0) + (N > 2 && seg >= 2 ? step : 0); }
   __device__ __forceinline__ void part(int first, int) {
-    if (first < left) {
-      s.part(first, left - first);
-      left -= first;
-    } else {
-      s.base = second;
-      s.part(first - left, left);
-      left = -1;
-    }
+    seg = first / stages;
+    first -= seg * stages;
+    s.base = base();
+    s.part(first, stages - first);
+    left = stages - first;
   }
   __device__ __forceinline__ void begin() {
-    if (left == 0) { s.base = second; s.kdone = 0; }
+    if (left == 0) {
+      if (seg + 1 < N) { ++seg; left = stages; s.base = base(); s.kdone = 0; }       // behind the last: zeros (kdone >= k)
+      else left = 1 << 30;
+    }
     --left;
     s.begin();
   }
@@ -141,7 +148,7 @@ template <class S> struct Twice {
 struct GatedArgs {
   const unsigned short *x, *wg, *wu, *wd, *dy;
   unsigned short *h, *dg, *du, *y;
-  unsigned short* hlo;                             // null, or what the rounding of h left, rounded: few tokens only
+  unsigned short *hlo, *dglo, *dulo;               // null, or what the rounding of h, dg and du left: few tokens only
   void* dx;
   unsigned short* keep16; unsigned char* keep8;    // P then Q, [2][M][Fp]
   void *dwg, *dwu, *dwd;
@@ -152,6 +159,12 @@ struct GatedArgs {
 };
 
 __device__ __forceinline__ void store8(unsigned short* p, const float* v) { *reinterpret_cast<u32x4*>(p) = pack8(v); }
+__device__ __forceinline__ void lower8(unsigned short* p, const float* v) {     // what store8 leaves
+  float l[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) l[e] = v[e] - bf16_to_f32(f32_to_bf16(v[e]));
+  store8(p, l);
+}
 // results have rows of their own length n: columns c .. c + 7 of row r
 __device__ __forceinline__ void result16(unsigned short* p, long long r, int c, int n, const float* v) {
   p += r * n + c;
@@ -257,7 +270,7 @@ template <int BT, int NST, bool JOIN> __global__ GATED_BOUNDS void gated_down_ke
   });
 }
 
-template <int BT, int NST, bool JOIN> __global__ GATED_BOUNDS void gated_dh_kernel(const GatedArgs a) {
+template <int BT, int NST, bool JOIN, bool LO> __global__ GATED_BOUNDS void gated_dh_kernel(const GatedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   Block<BT, NST, JOIN> b;
   b.begin(a);
@@ -289,24 +302,26 @@ template <int BT, int NST, bool JOIN> __global__ GATED_BOUNDS void gated_dh_kern
     for (int e = 0; e < 8; ++e) { dg[e] = v[e] * p[e]; du[e] = v[e] * q[e]; }
     store8(a.dg + o, dg);
     store8(a.du + o, du);
+    if (LO) { lower8(a.dglo + o, dg); lower8(a.dulo + o, du); }
   });
 }
 
-template <int BT, int NST, bool JOIN> __global__ GATED_BOUNDS void gated_dx_kernel(const GatedArgs a) {
+template <int BT, int NST, bool JOIN, bool LO> __global__ GATED_BOUNDS void gated_dx_kernel(const GatedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   Block<BT, NST, JOIN> b;
   b.begin(a);
   int ti, tj;
   tile_of(b.t, (a.M + BT - 1) / BT, (a.D + BT - 1) / BT, ti, tj);
   const int m0 = ti * BT, n0 = tj * BT, nk = (a.F + 63) / 64;
-  Twice<gt::Stager<BT, gt::CONTIG, 1>> sa;
-  Twice<gt::Stager<BT, gt::SLOW, 1>> sb;
+  constexpr int N = LO ? 4 : 2;
+  Series<gt::Stager<BT, gt::CONTIG, 1>, N> sa;
+  Series<gt::Stager<BT, gt::SLOW, 1>, N> sb;
+  const long long row = (long long)m0 * a.Fp;
   sa.s.init(gt::Operand{a.dg, a.Fp, m0, a.M, a.F}, b.wid, b.lane);
-  sa.second = a.du + (long long)m0 * a.Fp;
+  sa.start(a.dg + row, a.du + row, LO ? a.dglo - a.dg : 0, nk);
   sb.s.init(gt::Operand{a.wg, a.Dp, n0, a.Dp, a.F}, b.wid, b.lane);
-  sb.second = a.wu;
-  sa.left = sb.left = nk;
-  if (!b.template product<gt::CONTIG, gt::SLOW>(a, sa, sb, 2 * nk, smem)) return;
+  sb.start(a.wg, a.wu, 0, nk);
+  if (!b.template product<gt::CONTIG, gt::SLOW>(a, sa, sb, N * nk, smem)) return;
   b.store(smem, gt::NoLoad{}, [&](int r, int c, const float* v, gt::None) {
     r += m0; c += n0;
     if (r >= a.M || c >= a.D) return;
@@ -315,7 +330,7 @@ template <int BT, int NST, bool JOIN> __global__ GATED_BOUNDS void gated_dx_kern
   });
 }
 
-template <int BT, int NST, bool JOIN> __global__ GATED_BOUNDS void gated_dw_kernel(const GatedArgs a) {
+template <int BT, int NST, bool JOIN, bool LO> __global__ GATED_BOUNDS void gated_dw_kernel(const GatedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   Block<BT, NST, JOIN> b;
   b.begin(a, 3);
@@ -329,10 +344,20 @@ template <int BT, int NST, bool JOIN> __global__ GATED_BOUNDS void gated_dw_kern
   void* const out = which == 0 ? a.dwg : which == 1 ? a.dwu : a.dwd;
   if (out == nullptr) return;
   const int m0 = ti * BT, n0 = tj * BT;
-  gt::Stager<BT, gt::SLOW, 1> sa, sb;
-  sa.init(gt::Operand{pa, lda, m0, lda, a.M}, b.wid, b.lane);
-  sb.init(gt::Operand{pb, ldb, n0, ldb, a.M}, b.wid, b.lane);
-  if (!b.template product<gt::SLOW, gt::SLOW>(a, sa, sb, (a.M + 63) / 64, smem)) return;
+  if constexpr (LO) {
+    Series<gt::Stager<BT, gt::SLOW, 1>, 2> sa, sb;
+    const int nk = (a.M + 63) / 64;
+    sa.s.init(gt::Operand{pa, lda, m0, lda, a.M}, b.wid, b.lane);
+    sb.s.init(gt::Operand{pb, ldb, n0, ldb, a.M}, b.wid, b.lane);
+    sa.start(pa, which == 0 ? a.dglo : which == 1 ? a.dulo : a.dy, 0, nk);
+    sb.start(pb, which == 2 ? a.hlo : a.x, 0, nk);
+    if (!b.template product<gt::SLOW, gt::SLOW>(a, sa, sb, 2 * nk, smem)) return;
+  } else {
+    gt::Stager<BT, gt::SLOW, 1> sa, sb;
+    sa.init(gt::Operand{pa, lda, m0, lda, a.M}, b.wid, b.lane);
+    sb.init(gt::Operand{pb, ldb, n0, ldb, a.M}, b.wid, b.lane);
+    if (!b.template product<gt::SLOW, gt::SLOW>(a, sa, sb, (a.M + 63) / 64, smem)) return;
+  }
   struct Sum { f32x4 lo, hi; };
   auto load = [&](int r, int c) {
     r += m0; c += n0;
@@ -393,11 +418,13 @@ __global__ __launch_bounds__(256) void gated_pad_kernel(const PadArgs a) {
 // ---- few tokens (serving): bound by reading the weights once.  A block owns 16 features (their gate and up rows, or 16 rows of Wd); its waves
 // share the reduction in steps of 64 (one 128-byte line of each row; wave w takes steps w, w + WAVES, ...), load the weights straight into
 // matrix-instruction operands - nothing is staged, every byte is used once - several steps ahead, and add their fp32 tiles in LDS in a fixed order.
-// TB: blocks of 16 tokens.  LO (up to 8 tokens): h goes from one product to the other as a pair of bf16 values, 16 bits, the lower ones in the place
-// of tokens 8 to 15, which the matrix instructions multiply anyway: y has no rounding but its own (relative error 0.0024 -> 0.0016) at no cost.
+// TB: blocks of 16 columns.  LO: h goes from one product to the other as a pair of bf16 values; the lower ones take the second half of the columns
+// (up to 8 tokens one block serves for both, at no cost).
 template <int TB, int WAVES, bool PAIR, int ACT, bool SAVE, bool LO>
 __global__ __launch_bounds__(64 * WAVES) void gated_few_kernel(const GatedArgs a) {
   constexpr int NM = PAIR ? 2 : 1, U = TB == 4 ? 2 : 4;                  // weight matrices; steps in flight
+  constexpr bool TWO = LO && !PAIR;                                      // upper and lower values of h
+  constexpr int COLS = TWO ? TB * 8 : TB * 16;                           // columns for tokens
   __shared__ f32x4 red[WAVES][NM * TB][64];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = lane & 15, kc = (lane >> 4) * 8;
@@ -407,7 +434,7 @@ __global__ __launch_bounds__(64 * WAVES) void gated_few_kernel(const GatedArgs a
   const unsigned long long wbytes = (unsigned long long)(N - f0 < 16 ? N - f0 : 16) * (unsigned long long)ld * 2ull;
   const __amdgpu_buffer_rsrc_t w0 = __builtin_amdgcn_make_buffer_rsrc((void*)((PAIR ? a.wg : a.wd) + (long long)f0 * ld), 0, (int)wbytes, 0x00020000);
   const __amdgpu_buffer_rsrc_t w1 = __builtin_amdgcn_make_buffer_rsrc((void*)((PAIR ? a.wu : a.wd) + (long long)f0 * ld), 0, (int)wbytes, 0x00020000);
-  const unsigned lo = LO && !PAIR ? (unsigned)(a.hlo - a.h) : 0u;         // elements from the upper to the lower values
+  const unsigned lo = TWO ? (unsigned)(a.hlo - a.h) : 0u;         // elements from the upper to the lower values
   const __amdgpu_buffer_rsrc_t xs = __builtin_amdgcn_make_buffer_rsrc((void*)in, 0, (int)(((unsigned long long)a.M * ld + lo) * 2ull), 0x00020000);
   f32x4 acc[NM][TB];
 #pragma unroll
@@ -428,8 +455,8 @@ __global__ __launch_bounds__(64 * WAVES) void gated_few_kernel(const GatedArgs a
         if (PAIR) w[u][h][NM - 1] = __builtin_amdgcn_raw_buffer_load_b128(w1, (int)off, 0, 0);
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
-          const int tok = LO && !PAIR ? row & 7 : t * 16 + row;
-          const unsigned xo = in_k && tok < a.M ? (unsigned)(tok * ld + k + (LO && !PAIR && row >= 8 ? (int)lo : 0)) * 2u : gt::OOB;
+          const int col = t * 16 + row, tok = col % COLS;
+          const unsigned xo = in_k && tok < a.M ? ((unsigned)(tok * ld + k) + (col >= COLS ? lo : 0u)) * 2u : gt::OOB;
           x[u][h][t] = __builtin_amdgcn_raw_buffer_load_b128(xs, (int)xo, 0, 0);
         }
       }
@@ -452,7 +479,7 @@ __global__ __launch_bounds__(64 * WAVES) void gated_few_kernel(const GatedArgs a
   __syncthreads();
   for (int i = tid; i < TB * 64; i += 64 * WAVES) {
     const int t = i >> 6, l = i & 63, tok = t * 16 + (l & 15), f = f0 + (l >> 4) * 4;
-    if (tok >= a.M || f >= (PAIR ? a.Fp : N)) continue;
+    if (tok >= a.M || tok >= COLS || f >= (PAIR ? a.Fp : N)) continue;
     f32x4 v[NM];
 #pragma unroll
     for (int m = 0; m < NM; ++m) {
@@ -463,10 +490,10 @@ __global__ __launch_bounds__(64 * WAVES) void gated_few_kernel(const GatedArgs a
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[m][e] += o[e];
       }
-      if (LO && !PAIR) {                                                 // lane l + 8: the same token's lower values
+      if (TWO) {                                                         // the same token's lower values: COLS columns further
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
-          const f32x4 o = red[w][m * TB + t][l + 8];
+          const f32x4 o = TB == 1 ? red[w][0][(l + 8) & 63] : red[w][t + TB / 2][l];
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[m][e] += o[e];
         }
@@ -521,14 +548,14 @@ template <int BT, int NST, auto KERNEL> int launch(long long blocks, const Gated
 // How `count` products of rows x cols over ks stages are cut.  256 x 256 tiles run four times the work of a 128 x 128 stage in about 1.4 times
 // the time of a CU's pair of them, but one at a time, so that nothing hides a block's ends.
 struct Cut { bool large; int splits, per; long long tiles; };
-Cut cut_of(int count, int rows, int cols, int ks) {
+Cut cut_of(int count, int rows, int cols, int ks, bool few = false) {
   Cut c{};
   const long long big = count * tiles(rows, 256) * tiles(cols, 256);
   c.tiles = count * tiles(rows, 128) * tiles(cols, 128);
   double small = 0.0;
   c.per = gt::chunk_for(c.tiles, ks, &small);
   c.splits = (ks + c.per - 1) / c.per;
-  c.large = 1.44 * (double)((big + gt::CUS - 1) / gt::CUS) * (ks + 10) < small;
+  c.large = !few && 1.44 * (double)((big + gt::CUS - 1) / gt::CUS) * (ks + 10) < small;
   if (c.large) { c.tiles = big; c.splits = 1; c.per = ks; }
   return c;
 }
@@ -538,25 +565,39 @@ long long slab_floats(const Cut& c) { return c.splits > 1 ? c.tiles * c.splits *
 template <class P> int product(const Cut& c, GatedArgs a, void* st) {
   a.splits = c.splits; a.per = c.per;
   if (c.splits > 1 && a.slabs == nullptr) return -1;
-  if (c.large) return launch<256, 2, P::template at<256, 2, false>>(c.tiles, a, st);
+  if constexpr (P::LARGE) {
+    if (c.large) return launch<256, 2, P::template at<256, 2, false>>(c.tiles, a, st);
+  }
   const long long blocks = c.tiles * c.splits;
   int rc = blocks <= gt::CUS ? launch<128, 4, P::template at<128, 4, false>>(blocks, a, st)
                              : launch<128, 2, P::template at<128, 2, false>>(blocks, a, st);
   if (rc == 0 && c.splits > 1) rc = launch<128, 2, P::template at<128, 2, true>>(c.tiles * gt::Tile<128, 128>::FM, a, st);
   return rc;
 }
-template <int ACT, bool SAVE> struct Up { template <int BT, int NST, bool JOIN> static constexpr auto at = &gated_up_kernel<BT, NST, JOIN, ACT, SAVE>; };
-struct Down { template <int BT, int NST, bool JOIN> static constexpr auto at = &gated_down_kernel<BT, NST, JOIN>; };
-struct Dh { template <int BT, int NST, bool JOIN> static constexpr auto at = &gated_dh_kernel<BT, NST, JOIN>; };
-struct Dx { template <int BT, int NST, bool JOIN> static constexpr auto at = &gated_dx_kernel<BT, NST, JOIN>; };
-struct Dw { template <int BT, int NST, bool JOIN> static constexpr auto at = &gated_dw_kernel<BT, NST, JOIN>; };
+template <int ACT, bool SAVE> struct Up {
+  static constexpr bool LARGE = true;
+  template <int BT, int NST, bool JOIN> static constexpr auto at = &gated_up_kernel<BT, NST, JOIN, ACT, SAVE>;
+};
+struct Down { static constexpr bool LARGE = true; template <int BT, int NST, bool JOIN> static constexpr auto at = &gated_down_kernel<BT, NST, JOIN>; };
+template <bool LO> struct Dh {
+  static constexpr bool LARGE = !LO;
+  template <int BT, int NST, bool JOIN> static constexpr auto at = &gated_dh_kernel<BT, NST, JOIN, LO>;
+};
+template <bool LO> struct Dx {
+  static constexpr bool LARGE = !LO;
+  template <int BT, int NST, bool JOIN> static constexpr auto at = &gated_dx_kernel<BT, NST, JOIN, LO>;
+};
+template <bool LO> struct Dw {
+  static constexpr bool LARGE = !LO;
+  template <int BT, int NST, bool JOIN> static constexpr auto at = &gated_dw_kernel<BT, NST, JOIN, LO>;
+};
 
 int stages(int k) { return (int)tiles(k, 64); }
 Cut cut_up(int M, int D, int F) { return cut_of(1, M, 2 * F, stages(D)); }
 Cut cut_down(int M, int D, int F) { return cut_of(1, M, D, stages(F)); }
-Cut cut_dh(int M, int D, int F) { return cut_of(1, M, F, stages(D)); }
-Cut cut_dx(int M, int D, int F) { return cut_of(1, M, D, 2 * stages(F)); }
-Cut cut_dw(int M, int D, int F) { return cut_of(3, F, D, stages(M)); }
+Cut cut_dh(int M, int D, int F, bool lo) { return cut_of(1, M, F, stages(D), lo); }
+Cut cut_dx(int M, int D, int F, bool lo) { return cut_of(1, M, D, (lo ? 4 : 2) * stages(F), lo); }
+Cut cut_dw(int M, int D, int F, bool lo) { return cut_of(3, F, D, (lo ? 2 : 1) * stages(M), lo); }
 
 constexpr int FEW = 64;                            // tokens up to which gated_few_kernel is used
 
@@ -567,7 +608,12 @@ template <int TB, bool PAIR, int ACT, bool SAVE, bool LO> int launch_few_t(const
   return (int)hipGetLastError();
 }
 template <bool PAIR, int ACT, bool SAVE> int launch_few(const GatedArgs& a, void* st) {
-  if (a.hlo != nullptr) return launch_few_t<1, PAIR, ACT, SAVE, true>(a, st);
+  if (a.hlo != nullptr && PAIR)
+    return a.M <= 16 ? launch_few_t<1, PAIR, ACT, SAVE, true>(a, st) : a.M <= 32 ? launch_few_t<2, PAIR, ACT, SAVE, true>(a, st)
+                                                                                 : launch_few_t<4, PAIR, ACT, SAVE, true>(a, st);
+  if (a.hlo != nullptr && a.M <= 32)               // twice the columns
+    return a.M <= 8 ? launch_few_t<1, PAIR, ACT, SAVE, true>(a, st) : a.M <= 16 ? launch_few_t<2, PAIR, ACT, SAVE, true>(a, st)
+                                                                                : launch_few_t<4, PAIR, ACT, SAVE, true>(a, st);
   return a.M <= 16 ? launch_few_t<1, PAIR, ACT, SAVE, false>(a, st) : a.M <= 32 ? launch_few_t<2, PAIR, ACT, SAVE, false>(a, st)
                                                                                 : launch_few_t<4, PAIR, ACT, SAVE, false>(a, st);
 }
@@ -576,6 +622,9 @@ template <int ACT> int few_up(const GatedArgs& a, bool save, void* st) {
 }
 // 32-bit offsets inside 16 rows of a weight and inside the tokens
 bool few(int M, int K) { return M <= FEW && (long long)FEW * K * 2 < 0x7fffffffll; }
+
+// h, dg and du as pairs: offsets between the planes in 32 bits too
+bool pairs(int M, int Dp, int Fp) { return few(M, Dp) && (long long)FEW * Fp * 10 < 0x7fffffffll; }
 
 bool sizes_ok(int M, int D, int F) { return M > 0 && D > 0 && F > 0 && D < (1 << 30) && F < (1 << 30); }
 
@@ -599,8 +648,9 @@ extern "C" long long ddl_gated_workspace(int M, int D, int F, int pass) {
     if (!few(M, pad8(D))) most(cut_up(M, D, F));
     if (!few(M, pad8(F))) most(cut_down(M, D, F));
   }
-  if (pass & 1) { most(cut_dh(M, D, F)); most(cut_dx(M, D, F)); }
-  if (pass & 2) most(cut_dw(M, D, F));
+  const bool lo = pairs(M, pad8(D), pad8(F));
+  if (pass & 1) { most(cut_dh(M, D, F, lo)); most(cut_dx(M, D, F, lo)); }
+  if (pass & 2) most(cut_dw(M, D, F, lo));
   return n;
 }
 
@@ -623,16 +673,16 @@ extern "C" int ddl_gated_pad(const void* const* src, void* const* dst, const int
 }
 
 // x [M][Dp], wg and wu [F][Dp], wd [D][Fp], h [M][Fp], y [M][D];  keep16 [2][M][Fp] (16 bit) and keep8 [2][M][Fp] (8 bit), or both null: what
-// the backward pass needs;  hlo [M][Fp], or null (more than 8 tokens: always), behind h in the same allocation.  Dp and Fp: D and F padded to 8 with zeros.
+// the backward pass needs;  hlo [M][Fp] behind h in the same allocation, up to 64 tokens (else unused).  Dp and Fp: D and F padded to 8 with zeros.
 extern "C" int ddl_gated_fwd(const void* x, const void* wg, const void* wu, const void* wd, void* h, void* hlo, void* keep16, void* keep8, void* y,
                              float* slabs, int M, int D, int F, int act, void* stream) {
-  if (!sizes_ok(M, D, F) || (keep16 == nullptr) != (keep8 == nullptr) || (hlo != nullptr && M > 8)) return -1;
+  if (!sizes_ok(M, D, F) || (keep16 == nullptr) != (keep8 == nullptr)) return -1;
   GatedArgs a{};
   a.x = (const unsigned short*)x; a.wg = (const unsigned short*)wg; a.wu = (const unsigned short*)wu; a.wd = (const unsigned short*)wd;
   a.h = (unsigned short*)h; a.keep16 = (unsigned short*)keep16; a.keep8 = (unsigned char*)keep8; a.y = (unsigned short*)y;
   a.slabs = slabs;
   a.M = M; a.D = D; a.F = F; a.Dp = pad8(D); a.Fp = pad8(F);
-  if (few(M, a.Dp) && few(M, a.Fp)) a.hlo = (unsigned short*)hlo;
+  if (pairs(M, a.Dp, a.Fp) && (M <= 32 || keep16 != nullptr)) a.hlo = (unsigned short*)hlo;
   int rc = -1;
   if (act == SILU) rc = up<SILU>(a, stream);
   else if (act == GELU) rc = up<GELU>(a, stream);
@@ -641,23 +691,32 @@ extern "C" int ddl_gated_fwd(const void* x, const void* wg, const void* wu, cons
   return few(M, a.Fp) ? launch_few<false, SILU, false>(a, stream) : product<Down>(cut_down(M, D, F), a, stream);
 }
 
-// pass: 1 dg and du (and dx, unless null), 2 weight gradients (those that are not null; they take dg and du), 3 both.  dy [M][Dp], dg and du
-// [M][Fp], dx [M][D] bf16 or (dx32) fp32, dwg and dwu [F][D], dwd [D][F]: dw 0 bf16, 1 fp32 that are added to, 2 fp32
-extern "C" int ddl_gated_bwd(const void* x, const void* dy, const void* wg, const void* wu, const void* wd, const void* h, const void* keep16,
-                             const void* keep8, void* dg, void* du, void* dx, int dx32, void* dwg, void* dwu, void* dwd, int dw, float* slabs,
+// pass: 1 dg and du (and dx, unless null), 2 weight gradients (those that are not null; they take dg and du), 3 both.  dy [M][Dp], dgu: dg, du and,
+// up to 64 tokens, what their rounding left, [M][Fp] each, dx [M][D] bf16 or (dx32) fp32, dwg and dwu [F][D], dwd [D][F]: dw 0 bf16, 1 fp32 that are added to, 2 fp32
+extern "C" int ddl_gated_bwd(const void* x, const void* dy, const void* wg, const void* wu, const void* wd, const void* h, const void* hlo,
+                             const void* keep16, const void* keep8, void* dgu, void* dx, int dx32, void* dwg, void* dwu, void* dwd, int dw, float* slabs,
                              int M, int D, int F, int pass, void* stream) {
   if (!sizes_ok(M, D, F) || pass < 1 || pass > 3 || dw < 0 || dw > 2) return -1;
   GatedArgs a{};
   a.x = (const unsigned short*)x; a.dy = (const unsigned short*)dy;
   a.wg = (const unsigned short*)wg; a.wu = (const unsigned short*)wu; a.wd = (const unsigned short*)wd;
   a.h = (unsigned short*)h; a.keep16 = (unsigned short*)keep16; a.keep8 = (unsigned char*)keep8;
-  a.dg = (unsigned short*)dg; a.du = (unsigned short*)du; a.dx = dx; a.dx32 = dx32;
+  a.dx = dx; a.dx32 = dx32;
   a.dwg = dwg; a.dwu = dwu; a.dwd = dwd; a.dw = dw;
   a.slabs = slabs;
   a.M = M; a.D = D; a.F = F; a.Dp = pad8(D); a.Fp = pad8(F);
+  const long long plane = (long long)M * a.Fp;
+  a.dg = (unsigned short*)dgu;
+  if (dgu != nullptr) { a.du = a.dg + plane; a.dglo = a.du + plane; a.dulo = a.dglo + plane; }
+  a.hlo = (unsigned short*)hlo;
+  const bool lo = pairs(M, a.Dp, a.Fp);
   int rc = 0;
-  if (pass & 1) rc = product<Dh>(cut_dh(M, D, F), a, stream);
-  if (rc == 0 && (pass & 1) && dx != nullptr) rc = product<Dx>(cut_dx(M, D, F), a, stream);
-  if (rc == 0 && (pass & 2)) rc = product<Dw>(cut_dw(M, D, F), a, stream);
+  if (pass & 1) {
+    rc = lo ? product<Dh<true>>(cut_dh(M, D, F, lo), a, stream) : product<Dh<false>>(cut_dh(M, D, F, lo), a, stream);
+    if (rc == 0 && dx != nullptr)
+      rc = lo ? product<Dx<true>>(cut_dx(M, D, F, lo), a, stream) : product<Dx<false>>(cut_dx(M, D, F, lo), a, stream);
+  }
+  if (rc == 0 && (pass & 2))
+    rc = lo ? product<Dw<true>>(cut_dw(M, D, F, lo), a, stream) : product<Dw<false>>(cut_dw(M, D, F, lo), a, stream);
   return rc;
 }

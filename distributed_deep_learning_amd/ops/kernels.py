@@ -1271,32 +1271,32 @@ def _gated_slabs(lib, M, D, F_, which, device):
 def gated_fwd(x, w_gate, w_up, w_down, M: int, D: int, F_: int, activation: str = "silu", save: bool = False):
     """``y = (act(x w_gate^T) * (x w_up^T)) w_down^T`` of :func:`gated_operands` (``csrc/gated.hip``).  Returns ``(y, kept)``: ``y`` bf16
     ``[M, D]``; with ``save`` (training) ``kept`` is the byte tensor that :func:`gated_bwd` takes, for every token and (padded) feature
-    ``h`` in bf16 and the factors ``u act'(g)`` and ``act(g)`` in 24 bits, else ``None``."""
+    ``h`` in bf16, the factors ``u act'(g)`` and ``act(g)`` in 24 bits and, up to 64 tokens, what the rounding of ``h`` left, else ``None``."""
     lib = _lib.require()
     _lib.check_device(x, "gated_fwd")
     n = M * ((F_ + 7) // 8 * 8)
     y = torch.empty((M, D), dtype=BF16, device=x.device)
     size = n * (8 if save else 2)
-    buf = torch.empty(size + (2 * n if M <= 8 else 0), dtype=torch.uint8, device=x.device)
+    buf = torch.empty(size + (2 * n if M <= 64 else 0), dtype=torch.uint8, device=x.device)
     if M > 0:
         slabs, h = _gated_slabs(lib, M, D, F_, 0, x.device), buf.data_ptr()
-        check(lib.ddl_gated_fwd(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), h, h + size if M <= 8 else None,
+        check(lib.ddl_gated_fwd(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), h, h + size if M <= 64 else None,
                                 h + 2 * n if save else None, h + 6 * n if save else None, y.data_ptr(), ptr(slabs), M, D, F_, GATED_ACTIVATIONS[activation],
                                 stream_ptr()), "gated_fwd")
     return y, buf if save else None
 
 
 def gated_dh(dy, w_gate, w_up, w_down, kept, M: int, D: int, F_: int, dx=None):
-    """``(dg, du)`` (one bf16 tensor ``[2, M, F padded]``) from ``dy`` (:func:`gated_operands`), and ``dg w_gate + du w_up`` into ``dx``
+    """``(dg, du)`` (one bf16 tensor ``[2, M * F padded]``; up to 64 tokens ``[4, ..]``, with what their rounding left) from ``dy`` (:func:`gated_operands`), and ``dg w_gate + du w_up`` into ``dx``
     (bf16 or fp32 ``[M, D]``) if that is given."""
     lib = _lib.require()
     _lib.check_device(dy, "gated_dh")
     n = M * ((F_ + 7) // 8 * 8)
-    dgu = torch.empty((2, n), dtype=BF16, device=dy.device)
+    dgu = torch.empty((4 if M <= 64 else 2, n), dtype=BF16, device=dy.device)
     if M > 0:
-        slabs, h, dg = _gated_slabs(lib, M, D, F_, 1, dy.device), kept.data_ptr(), dgu.data_ptr()
-        check(lib.ddl_gated_bwd(None, dy.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), h, h + 2 * n, h + 6 * n,
-                                dg, dg + 2 * n, ptr(dx), int(dx is not None and dx.dtype is not BF16), None, None, None, 0, ptr(slabs),
+        slabs, h = _gated_slabs(lib, M, D, F_, 1, dy.device), kept.data_ptr()
+        check(lib.ddl_gated_bwd(None, dy.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), h, None, h + 2 * n, h + 6 * n,
+                                dgu.data_ptr(), ptr(dx), int(dx is not None and dx.dtype is not BF16), None, None, None, 0, ptr(slabs),
                                 M, D, F_, 1, stream_ptr()), "gated_dh")
     return dgu
 
@@ -1313,8 +1313,8 @@ def gated_dw(x, dy, kept, dgu, out, M: int, D: int, F_: int, accumulate: bool = 
             raise ValueError(f"gated_dw: outputs must be contiguous, 16-byte aligned tensors {shape} of one dtype, added to only in fp32")
     if M > 0:
         n = M * ((F_ + 7) // 8 * 8)
-        slabs, dg = _gated_slabs(lib, M, D, F_, 2, x.device), ptr(dgu)
-        check(lib.ddl_gated_bwd(x.data_ptr(), dy.data_ptr(), None, None, None, kept.data_ptr(), None, None, dg, dg + 2 * n if dg else None, None, 0,
+        slabs, h = _gated_slabs(lib, M, D, F_, 2, x.device), kept.data_ptr()
+        check(lib.ddl_gated_bwd(x.data_ptr(), dy.data_ptr(), None, None, None, h, h + 8 * n if M <= 64 else None, None, None, ptr(dgu), None, 0,
                                 *(ptr(t) for t in out), kind, ptr(slabs), M, D, F_, 2, stream_ptr()), "gated_dw")
     elif not accumulate:
         for t in live:

@@ -292,7 +292,7 @@ def _act64(g, act):
     return torch.relu(g), (g > 0).double()
 
 
-def _gated_case(T, D, H, act, seed=0):
+def _gated_case(T, D, H, act, seed=0, inner=B8):
     x, dy = _randn(seed, T, D).to(BF), _randn(seed + 1, T, D, scale=0.1).to(BF)
     wg, wu = _randn(seed + 2, H, D, scale=D ** -0.5).to(BF), _randn(seed + 3, H, D, scale=D ** -0.5).to(BF)
     wd = _randn(seed + 4, D, H, scale=H ** -0.5).to(BF)
@@ -306,9 +306,9 @@ def _gated_case(T, D, H, act, seed=0):
     # roundings on the way: h once; the factors u act'(g) and act(g) are kept with a half-step of 2^-17, act' carries 1e-5 of |g| + 1 from the
     # projections' sums and the exponential; dg and du once; sums of n products n 2^-24 of the magnitudes; the result once
     ab = torch.abs
-    eh = B8 * ab(h) + 1e-5 * ab(u) * (ab(g) + 1)
-    edg = (B8 + 2.0 ** -17) * ab(dg) + 1e-5 * ab(dh * u) * (ab(g) + 1) + 1e-6
-    edu = (B8 + 2.0 ** -17) * ab(du) + 1e-5 * ab(dh) * (ab(g) + 1) + 1e-6
+    eh = inner * ab(h) + 1e-5 * ab(u) * (ab(g) + 1)
+    edg = (inner + 2.0 ** -17) * ab(dg) + 1e-5 * ab(dh * u) * (ab(g) + 1) + 1e-6
+    edu = (inner + 2.0 ** -17) * ab(du) + 1e-5 * ab(dh) * (ab(g) + 1) + 1e-6
     n = max(T, D, H) * H24
     sums = {"y": ab(h) @ ab(W).T, "dx": ab(dg) @ ab(G_) + ab(du) @ ab(U_), "dwg": ab(dg).T @ ab(X), "dwu": ab(du).T @ ab(X), "dwd": ab(DY).T @ ab(h)}
     err = {"y": eh @ ab(W).T, "dx": edg @ ab(G_) + edu @ ab(U_), "dwg": edg.T @ ab(X), "dwu": edu.T @ ab(X), "dwd": ab(DY).T @ eh}
@@ -811,3 +811,20 @@ def test_orthogonalize_offsets_past_32_bits():
     for i in (0, 535, 539):                                                        # 2^31 elements end in matrix 534
         ref = _orth64(g[i].double())
         assert float((out[i].double() - ref).norm()) <= ORTH_TOL["bf16"] * float(ref.norm()), i
+
+
+@gpu
+@pytest.mark.parametrize("case", [(1, 64, 128, "silu"), (7, 40, 300, "gelu"), (9, 136, 264, "silu"), (16, 1032, 96, "relu"), (32, 66, 2050, "silu"),
+                                  (33, 200, 1500, "gelu"), (64, 2056, 328, "silu")])
+def test_gated_mlp_of_few_tokens_rounds_results_only(case):
+    """Up to 64 tokens h, dg and du are pairs of bf16 values: what the pair leaves is half a step of the lower one, 2^-8 of 2^-8 (y: up to 32)."""
+    T, D, H, act = case
+    (x, wg, wu, wd, dy), ref, tol = _gated_case(T, D, H, act, seed=101, inner=B8 * B8)
+    leaves = [t.cuda().requires_grad_() for t in (x, wg, wu, wd)]
+    y = F.gated_mlp(*leaves, activation=act)
+    grads = torch.autograd.grad(y, leaves, dy.cuda())
+    if T <= 32:
+        _check(y, ref["y"], tol["y"], "y")
+        _check(F.gated_mlp(*(t.cuda() for t in (x, wg, wu, wd)), activation=act), ref["y"], tol["y"], "y")
+    for k, t in zip(("dx", "dwg", "dwu", "dwd"), grads):
+        _check(t, ref[k], tol[k], k)
