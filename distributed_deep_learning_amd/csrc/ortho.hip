@@ -21,6 +21,10 @@
 //     1e-6 of the norm, the same as fp32 products, at a third of the fp16 rate instead of a sixteenth.
 // The Frobenius norm is summed in fp64, in a fixed order.
 //
+// Measured, 8192 x 2048 fp32 (two chains): norm 13 us, X0 23, gram 2 x (115 + join 17; 0.95 PFLOP/s of fp16 products), m x m products 14 x (33 + 12;
+// 0.85, few tiles), X 2 x 170 (1.22): bound by the matrix rate.  8 x 512 x 4608 bf16, five steps: gram 20 + 5.5, square 11, X 42 us (190 MB, 4.5 TB/s:
+// bandwidth).  ResNet-50's Muon step: norm and momentum 51 us, X0 57 (both 5.5 TB/s), gram 2 x 70, m x m 14 x 32, X 121 + 140.
+//
 // Many matrices share every launch: blocks find their matrix through maps of (matrix, block) pairs, so an optimizer step over a whole
 // network is 2 launches and 3 to 6 for every step of the iteration (joins of split reductions, two tile sizes), whatever it has of them.
 #include "common.h"
@@ -730,7 +734,7 @@ inline bool use_chains(double chained, double single) { return chained <= 0.8 * 
 inline double chained_work(double thin, double wide) { return 6 * thin * thin * wide + 14 * thin * thin * thin; }
 inline double single_work(double thin, double wide) { return 15 * thin * thin * wide + 5 * thin * thin * thin; }
 
-// Measured: 128 x 256 94 us against about 170 in 17 launches.  Four tiles (120 x 400 fp32) spill and run 257 us against 150: two at most.
+// Measured: 16 x 16 20 us, 64 x 147 49 us, 128 x 256 94 us (fp32 or bf16) against 100 to 170 us in 17 launches.  Four tiles (120 x 400 fp32) spill and run 257 us against 150: two at most.
 constexpr int SOLO_TILES = 2;
 inline bool solo(int rows, int cols) { return min(rows, cols) <= 128 && max(rows, cols) <= SOLO_TILES * 128; }
 
