@@ -997,13 +997,15 @@ class GatedMLP(torch.autograd.Function):
             if not live:
                 return dx, None, None, None, None
             arena = getattr(live[0], "_ddl_arena", None)
-            if arena is not None and all(getattr(w, "_ddl_arena", None) is arena and arena.grad_is_arena_view(w) and w.grad.is_contiguous()
-                                         for w in live):
+            if (arena is not None and len({id(w) for w in live}) == len(live)      # a weight in two places: autograd adds its gradients
+                    and all(getattr(w, "_ddl_arena", None) is arena and arena.grad_is_arena_view(w) and w.grad.is_contiguous() for w in live)):
                 with streams.fork(x, dy, kept, *([] if dgu is None else [dgu])):
                     K.gated_dw(x, dy, kept, dgu, [None if w is None else w.grad for w in want], M, D, F_, accumulate=True)
                 for w in reversed(live):
                     arena.notify_grad_ready(w)
                 return dx, None, None, None, None
+            if arena is not None:
+                streams.join()                                             # autograd will add to gradients the side stream may be adding to
             dtype = BF16 if all(w.dtype is BF16 for w in live) else torch.float32
             out = [None if w is None else torch.empty(w.shape, dtype=dtype, device=x.device) for w in want]
             K.gated_dw(x, dy, kept, dgu, out, M, D, F_)

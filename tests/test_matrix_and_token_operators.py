@@ -828,3 +828,26 @@ def test_gated_mlp_of_few_tokens_rounds_results_only(case):
         _check(F.gated_mlp(*(t.cuda() for t in (x, wg, wu, wd)), activation=act), ref["y"], tol["y"], "y")
     for k, t in zip(("dx", "dwg", "dwu", "dwd"), grads):
         _check(t, ref[k], tol[k], k)
+
+
+@gpu
+def test_gated_mlp_one_arena_weight_in_two_places():
+    (x, w, _, wd, dy), _, _ = _gated_case(200, 64, 264, "silu", seed=111)
+    net = tnn.ParameterList([tnn.Parameter(w.float().cuda()), tnn.Parameter(wd.float().cuda())])
+    arena = ParamArena(net.named_parameters())
+    F.gated_mlp(x.cuda(), net[0], net[0], net[1]).backward(dy.cuda())
+    torch.cuda.synchronize()
+    leaves = [t.cuda().requires_grad_() for t in (w, w, wd)]
+    a, b, c = torch.autograd.grad(F.gated_mlp(x.cuda(), *leaves), leaves, dy.cuda())
+    for p, ref in ((net[0], a.float() + b.float()), (net[1], c.float())):
+        assert arena.grad_is_arena_view(p)
+        assert float((p.grad - ref).norm()) <= 2 * B8 * float(ref.norm())              # the bf16 results' own rounding
+    arena.grad.zero_()
+    other = tnn.Parameter(leaves[1].detach().float() * 0.5)                            # and with a second call that adds to net[0] directly
+    both = F.gated_mlp(x.cuda(), net[0], net[0], net[1]) + F.gated_mlp(x.cuda(), net[0], other.to(BF), net[1])
+    both.backward(dy.cuda())
+    torch.cuda.synchronize()
+    half = (leaves[1].detach() * 0.5).requires_grad_()
+    a2, c2 = torch.autograd.grad(F.gated_mlp(x.cuda(), leaves[0], half, leaves[2]), (leaves[0], leaves[2]), dy.cuda())
+    for p, ref in ((net[0], a.float() + b.float() + a2.float()), (net[1], c.float() + c2.float())):
+        assert float((p.grad - ref).norm()) <= 3 * B8 * float(ref.norm())
