@@ -156,6 +156,7 @@ struct GatedArgs {
   int M, D, F, Dp, Fp;                            // Dp, Fp: D and F padded to 8, the row lengths of all operands (the padding is zero)
   int dx32, dw;                                   // dx fp32 instead of bf16;  weight gradients: 0 bf16, 1 fp32 added to, 2 fp32
   int splits, per;                                // blocks that share the reduction of a tile, stages of each
+  int first;                                      // 256 x 256 tiles that another launch does (Block::place)
 };
 
 __device__ __forceinline__ void store8(unsigned short* p, const float* v) { *reinterpret_cast<u32x4*>(p) = pack8(v); }
@@ -191,14 +192,27 @@ template <int BT, int NST, bool JOIN> struct Block {
   static constexpr bool SPLIT = BT == 128 && !JOIN;
   T tile;
   int tid, lane, wid, t, part;                    // t: the tile;  part: of its reduction (JOIN: its row group)
-  // `products` of equal grids one after the other: all XCDs work on one at a time and share its operands behind their L2s
-  __device__ __forceinline__ void begin(const GatedArgs& a, unsigned products = 1) {
+  // Tiles are dealt to the XCDs in runs, within `window` blocks at a time (0: all)
+  __device__ __forceinline__ void begin(const GatedArgs& a, unsigned window = 0) {
     tid = threadIdx.x; lane = tid & 63; wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const unsigned each = gridDim.x / products, before = blockIdx.x / each * each;
-    t = (int)(before + xcd_remap(blockIdx.x - before, each)); part = 0;
+    const unsigned before = window == 0 ? 0u : blockIdx.x / window * window, left = gridDim.x - before;
+    t = (int)(before + xcd_remap(blockIdx.x - before, window == 0 ? left : min(window, left))); part = 0;
     if (JOIN) { part = t % T::FM; t /= T::FM; }
     else if (SPLIT && a.splits > 1) { part = t % a.splits; t /= a.splits; }
   }
+  // Where tile `index` of a rows x cols result lies, COLS columns a tile; false: it is empty.  After a.first tiles of twice the size that another
+  // launch does, index counts the quarters of tiles of that size.
+  template <int COLS = BT> __device__ __forceinline__ bool place(const GatedArgs& a, int index, int rows, int cols, int& ti, int& tj) const {
+    if (BT == 128 && a.first > 0) {
+      tile_of((unsigned)index >> 2, (rows + 2 * BT - 1) / (2 * BT), (cols + 2 * COLS - 1) / (2 * COLS), ti, tj);
+      ti = 2 * ti + ((index >> 1) & 1);
+      tj = 2 * tj + (index & 1);
+      return ti * BT < rows && tj * COLS < cols;
+    }
+    tile_of((unsigned)index, (rows + BT - 1) / BT, (cols + COLS - 1) / COLS, ti, tj);
+    return true;
+  }
+  __device__ __forceinline__ int index(const GatedArgs& a) const { return BT == 128 ? t + 4 * a.first : t; }
   // true: the tile's epilogue is this block's
   template <int AM, int BMD, class SA, class SB> __device__ __forceinline__ bool product(const GatedArgs& a, SA& sa, SB& sb, int nk, char* smem) {
     float* const slab = a.slabs + (long long)t * a.splits * T::SLAB;
@@ -231,7 +245,7 @@ template <int BT, int NST, bool JOIN, int ACT, bool SAVE> __global__ GATED_BOUND
   Block<BT, NST, JOIN> b;
   b.begin(a);
   int ti, tj;
-  tile_of(b.t, (a.M + BT - 1) / BT, (a.F + BT / 2 - 1) / (BT / 2), ti, tj);
+  if (!b.template place<BT / 2>(a, b.index(a), a.M, a.F, ti, tj)) return;
   const int m0 = ti * BT, f0 = tj * (BT / 2);
   gt::Stager<BT, gt::CONTIG, 1> sa;
   PairStager<BT> sb;
@@ -265,7 +279,7 @@ template <int BT, int NST, bool JOIN> __global__ GATED_BOUNDS void gated_down_ke
   Block<BT, NST, JOIN> b;
   b.begin(a);
   int ti, tj;
-  tile_of(b.t, (a.M + BT - 1) / BT, (a.D + BT - 1) / BT, ti, tj);
+  if (!b.place(a, b.index(a), a.M, a.D, ti, tj)) return;
   const int m0 = ti * BT, n0 = tj * BT;
   gt::Stager<BT, gt::CONTIG, 1> sa, sb;
   sa.init(gt::Operand{a.h, a.Fp, m0, a.M, a.F}, b.wid, b.lane);
@@ -283,7 +297,7 @@ template <int BT, int NST, bool JOIN, bool LO> __global__ GATED_BOUNDS void gate
   Block<BT, NST, JOIN> b;
   b.begin(a);
   int ti, tj;
-  tile_of(b.t, (a.M + BT - 1) / BT, (a.F + BT - 1) / BT, ti, tj);
+  if (!b.place(a, b.index(a), a.M, a.F, ti, tj)) return;
   const int m0 = ti * BT, n0 = tj * BT;
   gt::Stager<BT, gt::CONTIG, 1> sa;
   gt::Stager<BT, gt::SLOW, 1> sb;
@@ -320,7 +334,7 @@ template <int BT, int NST, bool JOIN, bool LO> __global__ GATED_BOUNDS void gate
   Block<BT, NST, JOIN> b;
   b.begin(a);
   int ti, tj;
-  tile_of(b.t, (a.M + BT - 1) / BT, (a.D + BT - 1) / BT, ti, tj);
+  if (!b.place(a, b.index(a), a.M, a.D, ti, tj)) return;
   const int m0 = ti * BT, n0 = tj * BT, nk = (a.F + 63) / 64;
   constexpr int N = LO ? 4 : 2;
   Series<gt::Stager<BT, gt::CONTIG, 1>, N> sa;
@@ -344,11 +358,12 @@ template <int BT, int NST, bool JOIN, bool LO> __global__ GATED_BOUNDS void gate
 template <int BT, int NST, bool JOIN, bool LO> __global__ GATED_BOUNDS void gated_dw_kernel(const GatedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   Block<BT, NST, JOIN> b;
-  b.begin(a, 3);
-  const int tf = (a.F + BT - 1) / BT, td = (a.D + BT - 1) / BT, each = tf * td, which = b.t / each;
+  const bool rest = BT == 128 && a.first > 0;
+  const int size = rest ? 256 : BT, each = ((a.F + size - 1) / size) * ((a.D + size - 1) / size) * (rest ? 4 : 1);
+  b.begin(a, rest ? 0u : (unsigned)(each * (JOIN ? gt::Tile<BT, BT>::FM : BT == 128 ? a.splits : 1)));
+  const int which = b.index(a) / each, rows = which == 2 ? a.D : a.F, cols = which == 2 ? a.F : a.D;
   int ti, tj;
-  tile_of((unsigned)(b.t - which * each), which == 2 ? td : tf, which == 2 ? tf : td, ti, tj);
-  const int rows = which == 2 ? a.D : a.F, cols = which == 2 ? a.F : a.D;
+  if (!b.place(a, b.index(a) - which * each, rows, cols, ti, tj)) return;
   const int lda = which == 2 ? a.Dp : a.Fp, ldb = which == 2 ? a.Fp : a.Dp;
   const unsigned short* const pa = which == 0 ? a.dg : which == 1 ? a.du : a.dy;
   const unsigned short* const pb = which == 2 ? a.h : a.x;
@@ -558,18 +573,29 @@ template <int BT, int NST, auto KERNEL> int launch(long long blocks, const Gated
   return (int)hipGetLastError();
 }
 
-// How `count` products of rows x cols over ks stages are cut.  256 x 256 tiles run four times the work of a 128 x 128 stage in about 1.4 times
-// the time of a CU's pair of them, but one at a time, so that nothing hides a block's ends.
-struct Cut { bool large; int splits, per; long long tiles; };
+// How `count` products of rows x cols over ks stages are cut, by estimated times in stages of a CU's pair of 128 x 128 tiles (about 1 us).  Measured
+// rounds: 512 small tiles ks + 6;  256 large ones, four times the work of half as many blocks, 1.75 (ks + 7.5) (9 stages 30 us, 16 42, 32 73, 64 120).
+// Large tiles may take whole rounds of the chip and leave the rest to small ones, whose reductions can be shared: 6000 x 4096 x 11008 forward and
+// backward 4.79 -> 4.30 ms;  3000 x 2048 x 5632 0.85 -> 0.74.
+struct Cut { int first, splits, per; long long tiles; };                    // large tiles;  then small ones
 Cut cut_of(int count, int rows, int cols, int ks, bool few = false) {
-  Cut c{};
-  const long long big = count * tiles(rows, 256) * tiles(cols, 256);
-  c.tiles = count * tiles(rows, 128) * tiles(cols, 128);
-  double small = 0.0;
+  const long long big = count * tiles(rows, 256) * tiles(cols, 256), rounds = big / gt::CUS, rest = big - rounds * gt::CUS;
+  const double round = 1.75 * (ks + 7.5);
+  Cut c{0, 1, ks, count * tiles(rows, 128) * tiles(cols, 128)};
+  double small = 0.0, ends = 0.0;
   c.per = gt::chunk_for(c.tiles, ks, &small);
+  if (c.per == ks && c.tiles > gt::SLOTS) {               // several rounds overlap: a last one of single blocks is shorter, many drift apart
+    const long long full = c.tiles / gt::SLOTS, left = c.tiles - full * gt::SLOTS;
+    const double steps = (double)full + (left == 0 ? 0.0 : left <= gt::CUS ? 0.6 : 1.0), drift = (double)c.tiles / gt::SLOTS + 0.25;
+    small = (steps < drift ? steps : drift) * (ks + 6);
+  }
+  if (!few && big < (1 << 28)) {
+    const int per = rest > 0 ? gt::chunk_for(4 * rest, ks, &ends) : ks;
+    const double whole = round * (double)(rounds + (rest > 0)), mixed = round * (double)rounds + ends + 8;      // 8: a launch more
+    if (whole < small && whole <= mixed) c = Cut{(int)big, 1, ks, 0};
+    else if (rounds > 0 && mixed < small) c = Cut{(int)(rounds * gt::CUS), 1, per, 4 * rest};
+  }
   c.splits = (ks + c.per - 1) / c.per;
-  c.large = !few && 1.44 * (double)((big + gt::CUS - 1) / gt::CUS) * (ks + 10) < small;
-  if (c.large) { c.tiles = big; c.splits = 1; c.per = ks; }
   return c;
 }
 long long slab_floats(const Cut& c) { return c.splits > 1 ? c.tiles * c.splits * gt::Tile<128, 128>::SLAB : 0; }
@@ -578,12 +604,15 @@ long long slab_floats(const Cut& c) { return c.splits > 1 ? c.tiles * c.splits *
 template <class P> int product(const Cut& c, GatedArgs a, void* st) {
   a.splits = c.splits; a.per = c.per;
   if (c.splits > 1 && a.slabs == nullptr) return -1;
+  int rc = 0;
   if constexpr (P::LARGE) {
-    if (c.large) return launch<256, 2, P::template at<256, 2, false>>(c.tiles, a, st);
+    if (c.first > 0) rc = launch<256, 2, P::template at<256, 2, false>>(c.first, a, st);
   }
+  if (rc != 0 || c.tiles == 0) return rc;
+  a.first = c.first;
   const long long blocks = c.tiles * c.splits;
-  int rc = blocks <= gt::CUS ? launch<128, 4, P::template at<128, 4, false>>(blocks, a, st)
-                             : launch<128, 2, P::template at<128, 2, false>>(blocks, a, st);
+  rc = blocks <= gt::CUS ? launch<128, 4, P::template at<128, 4, false>>(blocks, a, st)
+                         : launch<128, 2, P::template at<128, 2, false>>(blocks, a, st);
   if (rc == 0 && c.splits > 1) rc = launch<128, 2, P::template at<128, 2, true>>(c.tiles * gt::Tile<128, 128>::FM, a, st);
   return rc;
 }

@@ -846,17 +846,17 @@ template <class KS> int set_chunk(const int* thin, int n, KS&& ks) {
   for (int i = 0; i < n; ++i) most = max(most, ks(i));
   double least = 1e30;
   for (int c = min(8, most); ; c = min(c + 8, most)) {
-    double blocks = 0, sum = 0, parts = 1, longest = 0;
+    double blocks = 0, sum = 0, parts = 0, longest = 0;
     for (int i = 0; i < n; ++i) {
       const int s = (ks(i) + c - 1) / c, per = (ks(i) + s - 1) / s;
       blocks += (double)tri(thin[i]) * s;
       sum += (double)tri(thin[i]) * s * (per + 6);
-      parts = s > parts ? s : parts;
+      if (s > 1) parts += (double)tri(thin[i]) * s;
       longest = per + 6 > longest ? per + 6 : longest;
     }
     double t = blocks <= CUS ? 0.6 * longest : longest;
     if (blocks > SLOTS && sum / SLOTS + 0.5 * longest > t) t = sum / SLOTS + 0.5 * longest;
-    if (parts > 1) t += 6 + 0.5 * parts;
+    if (parts > 0) t += 2.5 + parts / 60;
     if (t < least) { least = t; best = c; }
     if (c == most) break;
   }

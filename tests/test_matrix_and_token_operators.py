@@ -851,3 +851,9 @@ def test_gated_mlp_one_arena_weight_in_two_places():
     a2, c2 = torch.autograd.grad(F.gated_mlp(x.cuda(), leaves[0], half, leaves[2]), (leaves[0], leaves[2]), dy.cuda())
     for p, ref in ((net[0], a.float() + b.float() + a2.float()), (net[1], c.float() + c2.float())):
         assert float((p.grad - ref).norm()) <= 3 * B8 * float(ref.norm())
+
+
+@gpu
+@pytest.mark.parametrize("T,D,H", [(2048, 2048, 5632), (2100, 1290, 5001), (5000, 1900, 1801)])
+def test_gated_mlp_large_tiles_and_small_ones_for_the_rest(T, D, H):
+    test_gated_mlp_large_tiles(T, D, H)
