@@ -968,7 +968,7 @@ def _gated_forward(x, w_gate, w_up, w_down, activation, train):
     M = x.numel() // D
     ops = K.gated_operands((x.detach().reshape(M, D), M, D), (_weight16(w_gate), F_, D), (_weight16(w_up), F_, D), (_weight16(w_down), D, F_))
     y, kept = K.gated_fwd(*ops, M, D, F_, activation, save=train)
-    return y.view(shape), (*ops, kept), (M, D, F_)
+    return y if len(shape) == 2 else y.view(shape), (*ops, kept), (M, D, F_)
 
 
 class GatedMLP(torch.autograd.Function):
@@ -990,7 +990,7 @@ class GatedMLP(torch.autograd.Function):
         need = ctx.needs_input_grad
         with device_of(x):
             dy, = K.gated_operands((dy.reshape(M, D), M, D))
-            dx = torch.empty(shape, dtype=x_dtype, device=x.device) if need[0] else None
+            dx = None if not need[0] else x.new_empty(shape) if x_dtype is BF16 else x.new_empty(shape, dtype=x_dtype)
             dgu = K.gated_dh(dy, wg, wu, wd, kept, M, D, F_, dx) if need[0] or need[1] or need[2] else None
             want = [w if n else None for w, n in zip(weights, need[1:4])]
             live = [w for w in want if w is not None]
@@ -1007,7 +1007,8 @@ class GatedMLP(torch.autograd.Function):
             if arena is not None:
                 streams.join()                                             # autograd will add to gradients the side stream may be adding to
             dtype = BF16 if all(w.dtype is BF16 for w in live) else torch.float32
-            out = [None if w is None else torch.empty(w.shape, dtype=dtype, device=x.device) for w in want]
+            like = wg if dtype is BF16 else wg.new_empty(0, dtype=dtype)
+            out = [None if w is None else like.new_empty(w.shape) for w in want]
             K.gated_dw(x, dy, kept, dgu, out, M, D, F_)
             if dtype is not BF16:
                 out = [None if w is None else t.to(w.dtype) for w, t in zip(want, out)]

@@ -1178,6 +1178,12 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _scratch(t: torch.Tensor, nbytes: int):
+    """Workspace beside ``t`` (``None``: none needed).  In ``t``'s dtype: an allocation that names neither dtype nor device costs a third of one
+    that does, and calls on small tensors are bound by the host."""
+    return t.new_empty(-(-nbytes // t.element_size())) if nbytes else None
+
+
 def token_logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, train: bool = False):
     """``logits`` bf16 / fp32 ``[N, V]``, ``tokens`` int64 ``[N]`` -> fp32 ``(logp [N], entropy [N], norm [N, 2] or None,
     top_logp [N, top])`` and int64 ``top_index [N, top]`` (descending, equal values by the lowest index), one pass over the logits
@@ -1201,14 +1207,12 @@ def token_logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
         raise ValueError("token_logprobs: the vocabulary is empty")
     logits, tokens = logits.contiguous(), tokens.contiguous()
     dev = logits.device
-    logp, ent = torch.empty(N, dtype=torch.float32, device=dev), torch.empty(N, dtype=torch.float32, device=dev)
-    norm = torch.empty((N, 2), dtype=torch.float32, device=dev) if train else None
-    tv = torch.empty((N, top), dtype=torch.float32, device=dev)
-    ti = torch.empty((N, top), dtype=torch.int64, device=dev)
+    logp = torch.empty(N, dtype=torch.float32, device=dev)
+    ent, tv, ti = torch.empty_like(logp), logp.new_empty((N, top)), tokens.new_empty((N, top))
+    norm = logp.new_empty((N, 2)) if train else None
     if N > 0:
         is16 = int(logits.dtype == BF16)
-        ws = lib.ddl_logprob_workspace(N, V, is16, top)
-        ws = torch.empty(ws, dtype=torch.uint8, device=dev) if ws else None
+        ws = _scratch(tokens, lib.ddl_logprob_workspace(N, V, is16, top))
         check(lib.ddl_logprob_fwd(ptr(logits), is16, ptr(tokens), N, V, top, int(train), ptr(ws), ptr(logp), ptr(ent), ptr(norm), ptr(tv), ptr(ti),
                                   stream_ptr()), "token_logprobs")
     return logp, ent, norm, tv, ti
@@ -1263,23 +1267,18 @@ def gated_operands(*mats):
     return out
 
 
-def _gated_slabs(lib, M, D, F_, which, device):
-    n = lib.ddl_gated_workspace(M, D, F_, which)
-    return torch.empty(n, dtype=torch.float32, device=device) if n else None
-
-
 def gated_fwd(x, w_gate, w_up, w_down, M: int, D: int, F_: int, activation: str = "silu", save: bool = False):
     """``y = (act(x w_gate^T) * (x w_up^T)) w_down^T`` of :func:`gated_operands` (``csrc/gated.hip``).  Returns ``(y, kept)``: ``y`` bf16
-    ``[M, D]``; with ``save`` (training) ``kept`` is the byte tensor that :func:`gated_bwd` takes, for every token and (padded) feature
+    ``[M, D]``; with ``save`` (training) ``kept`` is the buffer that :func:`gated_bwd` takes, for every token and (padded) feature
     ``h`` in bf16, the factors ``u act'(g)`` and ``act(g)`` in 24 bits and, up to 64 tokens, what the rounding of ``h`` left, else ``None``."""
     lib = _lib.require()
     _lib.check_device(x, "gated_fwd")
     n = M * ((F_ + 7) // 8 * 8)
-    y = torch.empty((M, D), dtype=BF16, device=x.device)
+    y = x.new_empty((M, D))
     size = n * (8 if save else 2)
-    buf = torch.empty(size + (2 * n if M <= 64 else 0), dtype=torch.uint8, device=x.device)
+    buf = x.new_empty((size + (2 * n if M <= 64 else 0)) // 2)
     if M > 0:
-        slabs, h = _gated_slabs(lib, M, D, F_, 0, x.device), buf.data_ptr()
+        slabs, h = _scratch(x, 4 * lib.ddl_gated_workspace(M, D, F_, 0)), buf.data_ptr()
         check(lib.ddl_gated_fwd(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), h, h + size if M <= 64 else None,
                                 h + 2 * n if save else None, h + 6 * n if save else None, y.data_ptr(), ptr(slabs), M, D, F_, GATED_ACTIVATIONS[activation],
                                 stream_ptr()), "gated_fwd")
@@ -1292,9 +1291,9 @@ def gated_dh(dy, w_gate, w_up, w_down, kept, M: int, D: int, F_: int, dx=None):
     lib = _lib.require()
     _lib.check_device(dy, "gated_dh")
     n = M * ((F_ + 7) // 8 * 8)
-    dgu = torch.empty((4 if M <= 64 else 2, n), dtype=BF16, device=dy.device)
+    dgu = dy.new_empty((4 if M <= 64 else 2, n))
     if M > 0:
-        slabs, h = _gated_slabs(lib, M, D, F_, 1, dy.device), kept.data_ptr()
+        slabs, h = _scratch(dy, 4 * lib.ddl_gated_workspace(M, D, F_, 1)), kept.data_ptr()
         check(lib.ddl_gated_bwd(None, dy.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), h, None, h + 2 * n, h + 6 * n,
                                 dgu.data_ptr(), ptr(dx), int(dx is not None and dx.dtype is not BF16), None, None, None, 0, ptr(slabs),
                                 M, D, F_, 1, stream_ptr()), "gated_dh")
@@ -1313,7 +1312,7 @@ def gated_dw(x, dy, kept, dgu, out, M: int, D: int, F_: int, accumulate: bool = 
             raise ValueError(f"gated_dw: outputs must be contiguous, 16-byte aligned tensors {shape} of one dtype, added to only in fp32")
     if M > 0:
         n = M * ((F_ + 7) // 8 * 8)
-        slabs, h = _gated_slabs(lib, M, D, F_, 2, x.device), kept.data_ptr()
+        slabs, h = _scratch(x, 4 * lib.ddl_gated_workspace(M, D, F_, 2)), kept.data_ptr()
         check(lib.ddl_gated_bwd(x.data_ptr(), dy.data_ptr(), None, None, None, h, h + 8 * n if M <= 64 else None, None, None, ptr(dgu), None, 0,
                                 *(ptr(t) for t in out), kind, ptr(slabs), M, D, F_, 2, stream_ptr()), "gated_dw")
     elif not accumulate:
@@ -1370,10 +1369,9 @@ def orthogonalize(g: torch.Tensor, steps: int = NS_STEPS, coefficients=NS_COEFFI
     out = torch.empty_like(g)
     ws = parts = slabs = None
     if not lib.ddl_ns_solo(rows, cols):
-        slabs = lib.ddl_ns_shape(rows, cols, prod, batch, 0, 0, (C.c_int * 10)())
-        slabs = torch.empty(batch * slabs, dtype=torch.float32, device=g.device) if slabs else None
-        ws = torch.empty(batch * lib.ddl_ns_workspace(rows, cols, prod), dtype=torch.float16, device=g.device)
-        parts = torch.empty(batch * lib.ddl_ns_max_parts(), dtype=torch.float64, device=g.device)
+        slabs = _scratch(g, 4 * batch * lib.ddl_ns_shape(rows, cols, prod, batch, 0, 0, (C.c_int * 10)()))
+        ws = _scratch(g, 2 * batch * lib.ddl_ns_workspace(rows, cols, prod))
+        parts = _scratch(g, 8 * batch * lib.ddl_ns_max_parts())
     check(lib.ddl_orthogonalize(ptr(g), int(is16), ptr(out), ptr(ws), ptr(parts), ptr(slabs), batch, rows, cols, prod, int(steps),
                                 (C.c_float * 3)(a, b, c), float(eps), stream_ptr()), "orthogonalize")
     return out
