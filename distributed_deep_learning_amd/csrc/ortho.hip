@@ -21,7 +21,7 @@
 //     1e-6 of the norm, the same as fp32 products, at a third of the fp16 rate instead of a sixteenth.
 // The Frobenius norm is summed in fp64, in a fixed order.
 //
-// Measured, 8192 x 2048 fp32 (two chains): norm 13 us, X0 23, gram 2 x (115 + join 17; 0.95 PFLOP/s of fp16 products), m x m products 14 x (33 + 12;
+// Measured, 8192 x 2048 fp32 (two chains): norm 13 us, X0 23, gram 2 x (115 + join 12; 0.95 PFLOP/s of fp16 products), m x m products 14 x (33 + 12;
 // 0.85, few tiles), X 2 x 170 (1.22): bound by the matrix rate.  8 x 512 x 4608 bf16, five steps: gram 20 + 5.5, square 11, X 42 us (190 MB, 4.5 TB/s:
 // bandwidth).  ResNet-50's Muon step: norm and momentum 51 us, X0 57 (both 5.5 TB/s), gram 2 x 70, m x m 14 x 32, X 121 + 140.
 //
