@@ -933,7 +933,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
     ``logp`` is the log probability of the given token under ``softmax(logits)`` (0, and no gradient, for a token outside ``[0, V)``:
     padding), ``entropy`` that of the whole distribution in nats, ``top_logp`` / ``top_index`` the ``top`` (at most 64) most likely tokens,
     descending, equal logits by the lowest index.  All but the indices are differentiable.  Logits of ``-inf`` are masked tokens; a row of
-    nothing else gives ``logp = top_logp = -inf``, entropy 0 and no gradient."""
+    nothing else gives ``logp = top_logp = -inf``, entropy 0 and no gradient.  Logits that are not contiguous are copied: to leave positions
+    out, give them a token outside ``[0, V)`` rather than slicing the logits."""
     if tokens.shape != logits.shape[:-1]:
         raise ValueError(f"token_logprobs: tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")
     lead, V = logits.shape[:-1], logits.shape[-1]
@@ -1019,8 +1020,9 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     """``(act(x w_gate^T) * (x w_up^T)) w_down^T``: ``x`` ``[..., D]``, ``w_gate`` and ``w_up`` ``[F, D]``, ``w_down`` ``[D, F]``; ``activation``
     ``"silu"``, ``"gelu"`` (exact) or ``"relu"``.
 
-    On the GPU the products run on bf16 operands (fp32 inputs and weights are rounded; fp32 weights of an arena use its shadow) with
-    fp32 sums, the result is bf16; gradients come in the dtype of what they belong to.  On the CPU: plain torch ops in the inputs' dtype."""
+    On the GPU the products run on bf16 operands (fp32 inputs and weights are rounded, in every call; fp32 weights of an arena use its shadow)
+    with fp32 sums, the result is bf16; gradients come in the dtype of what they belong to.  Widths that are no multiples of 8 are copied to
+    padded operands in every call.  On the CPU: plain torch ops in the inputs' dtype."""
     if activation not in K.GATED_ACTIVATIONS:
         raise ValueError(f"gated_mlp: activation must be one of {sorted(K.GATED_ACTIVATIONS)}, got {activation!r}")
     D = x.shape[-1] if x.dim() else -1
