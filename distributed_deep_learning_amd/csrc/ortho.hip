@@ -23,7 +23,7 @@
 //
 // Measured, 8192 x 2048 fp32 (two chains): norm 13 us, X0 23, gram 2 x (115 + join 12; 0.95 PFLOP/s of fp16 products), m x m products 14 x (33 + 12;
 // 0.85, few tiles), X 2 x 170 (1.22): bound by the matrix rate.  8 x 512 x 4608 bf16, five steps: gram 20 + 5.5, square 11, X 42 us (190 MB, 4.5 TB/s:
-// bandwidth).  ResNet-50's Muon step: norm and momentum 51 us, X0 57 (both 5.5 TB/s), gram 2 x 70, m x m 14 x 32, X 121 + 140.
+// bandwidth).  ResNet-50's Muon step: norm and momentum 51 us, X0 57 (both 5.5 TB/s), gram 2 x 70, m x m 14 x 32, X 95 + 123.
 //
 // Many matrices share every launch: blocks find their matrix through maps of (matrix, block) pairs, so an optimizer step over a whole
 // network is 2 launches and 3 to 6 for every step of the iteration (joins of split reductions, two tile sizes), whatever it has of them.

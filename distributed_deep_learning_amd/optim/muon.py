@@ -42,6 +42,28 @@ def _geometry(name: str, p: torch.Tensor):
     raise ValueError(f"Muon: parameter {name} with strides {tuple(p.stride())} is no matrix over its first dimension in memory")
 
 
+def _deal(blocks, length, spread: bool) -> np.ndarray:
+    """Which block of a shared launch works on which part of which matrix: ``(matrix, part)`` rows.  The matrices' parts are handed out in
+    order of their reductions' ``length``, longest first.  ``spread``: the kernels give each XCD a run of this table; where reductions are not
+    cut to like lengths (the products with X) the table is laid out so that every XCD gets an equal share of each matrix, its parts one after
+    the other, longest matrices first in dispatch order (block ``d`` runs on XCD ``d % 8``): ResNet-50's 121 and 142 us -> 95 and 122.  Else a
+    matrix stays on one XCD, whose L2 its tiles share (spread, the square products take 34 us instead of 32)."""
+    n = sum(blocks)
+    out, at = np.zeros((n, 2), dtype=np.int32), 0
+    for i in sorted(range(len(blocks)), key=lambda i: -length[i]):
+        pos = np.arange(at, at + blocks[i])
+        at += blocks[i]
+        out[pos, 0] = i
+        out[pos[np.lexsort((pos, pos % 8))] if spread else pos, 1] = np.arange(blocks[i])
+    if spread:
+        q, r, d = n // 8, n % 8, np.arange(n)
+        x = d % 8
+        dealt = np.empty_like(out)
+        dealt[np.where(x < r, x * (q + 1), r * (q + 1) + (x - r) * q) + d // 8] = out
+        out = dealt
+    return out
+
+
 class Muon(_ArenaOptimizer):
     """``momentum`` holds Muon's momentum for matrices and Adam's first moment for the rest; ``exp_avg_sq`` is used by the rest only.
 
@@ -94,9 +116,7 @@ class Muon(_ArenaOptimizer):
         sides = [(C.c_int * len(self.matrices))(*(f(rows, cols) for _, rows, cols, _ in self.matrices)) for f in (min, max)]
         chunks = (C.c_int * 2)()
         _lib.check(lib.ddl_ns_chunks(*sides, len(self.matrices), prod, chunks), "ns_chunks")
-        # long reductions first: the blocks that run longest start first
-        for i in sorted(range(len(self.matrices)), key=lambda i: -max(self.matrices[i][1], self.matrices[i][2])):
-            s, rows, cols, scale = self.matrices[i]
+        for i, (s, rows, cols, scale) in enumerate(self.matrices):
             need = lib.ddl_ns_shape(rows, cols, prod, 1, *chunks, out)
             if need < 0:
                 raise RuntimeError(f"Muon: no plan for a {rows} x {cols} matrix")
@@ -105,11 +125,11 @@ class Muon(_ArenaOptimizer):
                 ws += lib.ddl_ns_workspace(rows, cols, prod)
                 slabs += need
             for m, n in zip(launches, [1] + [0] * 7 if solo else out[2:10]):
-                m.append(np.stack([np.full(n, i, dtype=np.int32), np.arange(n, dtype=np.int32)], 1))
+                m.append(n)
         dev = self.arena.device
-        maps = np.concatenate([np.concatenate(m) for m in launches])
+        maps = np.concatenate([_deal(n, sides[0] if k >= 6 else sides[1], k >= 6) for k, n in enumerate(launches)])
         return {"table": torch.from_numpy(table.view(np.uint8).copy()).to(dev), "maps": torch.from_numpy(np.ascontiguousarray(maps)).to(dev),
-                "blocks": (C.c_int * 8)(*(sum(len(x) for x in m) for m in launches)), "prod": prod,
+                "blocks": (C.c_int * 8)(*(sum(m) for m in launches)), "prod": prod,
                 "chains": lib.ddl_ns_chains(*sides, len(self.matrices)),
                 "solo": max(max(rows, cols) for _, rows, cols, _ in self.matrices) if solo else 0,
                 "coef": (C.c_float * 3)(*self.ns_coefficients), "ws": torch.empty(max(ws, 8), dtype=torch.float16, device=dev),

@@ -857,3 +857,20 @@ def test_gated_mlp_one_arena_weight_in_two_places():
 @pytest.mark.parametrize("T,D,H", [(2048, 2048, 5632), (2100, 1290, 5001), (5000, 1900, 1801)])
 def test_gated_mlp_large_tiles_and_small_ones_for_the_rest(T, D, H):
     test_gated_mlp_large_tiles(T, D, H)
+
+
+@pytest.mark.parametrize("spread", [False, True])
+@pytest.mark.parametrize("blocks", [[1], [0, 0], [5, 0, 17, 3], [100, 7, 64], [8, 16, 1000]])
+def test_muon_blocks_are_dealt_once_and_evenly(blocks, spread):
+    from distributed_deep_learning_amd.optim.muon import _deal
+    length = [7 * (i + 1) % 5 for i in range(len(blocks))]
+    out = _deal(blocks, length, spread)
+    assert sorted(map(tuple, out.tolist())) == [(i, k) for i, n in enumerate(blocks) for k in range(n)]
+    if spread and sum(blocks) >= 8:
+        n = len(out)
+        runs = [n // 8 + (x < n % 8) for x in range(8)]
+        at = 0
+        for x in range(8):                                               # every XCD's run holds an eighth of each matrix, up to one block
+            run = out[at:at + runs[x], 0]
+            at += runs[x]
+            assert all(abs(int((run == i).sum()) - b / 8) <= 1 for i, b in enumerate(blocks))
