@@ -1,12 +1,13 @@
 // Gated feed-forward block (gfx950):   h = act(x Wg^T) * (x Wu^T),   y = h Wd^T        x [M][D], Wg and Wu [F][D], Wd [D][F], bf16
 //
-// Forward, two launches:   up    both projections in one product: a block's columns are gate and up rows of the same features side by
+// Forward, two products:   up    both projections in one product: a block's columns are gate and up rows of the same features side by
 //                                side, so that one lane holds g and u of a feature and the activation and the product are the epilogue;
 //                                training also keeps P = u act'(g) and Q = act(g);
 //                          down  y = h Wd^T.
 // Backward, three:         dh    dy Wd, epilogue  dg = dh P,  du = dh Q  (dh itself is never written);
 //                          dx    dg Wg + du Wu, one reduction over both pairs;
 //                          dw    dg^T x, du^T x and dy^T h, one launch.
+// A product is one launch, two where large tiles leave a rest to small ones, and one more where blocks share a tile's reduction (cut_of).
 // All on the tiles of gemm_tile.h, which take the tensors as they lie: no transposed copy of a weight or an activation exists.
 //
 // Numbers.  Products accumulate in fp32.  h, dg and du are rounded to bf16 once, being operands of the next product at the bf16 rate.  P and Q

@@ -539,8 +539,6 @@ bool beyond_cache(long long rows, int V, int is_bf16) { return rows * V * (is_bf
 
 }  // namespace
 
-extern "C" int ddl_logprob_top_max() { return TOP_MAX; }
-
 // bytes of workspace of a forward call
 extern "C" long long ddl_logprob_workspace(long long rows, int V, int is_bf16, int k) {
   if (rows <= 0 || V <= 0 || k < 0 || k > TOP_MAX) return -1;

@@ -115,7 +115,6 @@ _SIGS = {
     "ddl_gated_pad": [_vp] * 6 + [_i, _vp],
     "ddl_gated_fwd": [_vp] * 10 + [_i, _i, _i, _i, _vp],
     "ddl_gated_bwd": [_vp] * 11 + [_i] + [_vp] * 3 + [_i, _vp, _i, _i, _i, _i, _vp],
-    "ddl_logprob_top_max": [],
     "ddl_logprob_workspace": [_ll, _i, _i, _i],
     "ddl_logprob_fwd": [_vp, _i, _vp, _ll, _i, _i, _i] + [_vp] * 7,
     "ddl_logprob_bwd": [_vp, _i] + [_vp] * 7 + [_ll, _i, _i, _vp, _vp],
