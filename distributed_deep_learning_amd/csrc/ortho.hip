@@ -475,7 +475,8 @@ template <int PROD> __device__ __forceinline__ void solo_put(char* buf, int off,
   if (PROD == 3) *reinterpret_cast<f16x4*>(buf + lo) = l;
 }
 
-template <int PROD, int NT, bool MUON>
+// FULL (fp32 matrices): sums of 22-bit products as exact as fp32 products' (64 x 147: error 1.1e-6 -> 0.8e-6 at 45 -> 52 us).
+template <int PROD, int NT, bool MUON, bool FULL>
 __global__ __launch_bounds__(512, 2) void ns_solo_kernel(const NsArgs a, const int steps, const float ca, const float cb, const float cc) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ double red[8];
@@ -551,6 +552,11 @@ __global__ __launch_bounds__(512, 2) void ns_solo_kernel(const NsArgs a, const i
   // k: length of the reduction;  cols: of the result.  A wave whose part of the result is all padding keeps its zeros.
   auto mul = [&](const char* pa, const char* pb, auto slow, int k, int cols) {
     if (wm * 64 >= thin || wn * 32 >= cols) return;
+    f32x4 cross[4][2];                                                  // FULL: hi lo, lo hi and lo lo apart, a third of the roundings of the large sums
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) cross[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
     for (int st = 0; st * L::KSTEP < k && st < L::KSTAGES; ++st, pa += 16384, pb += 16384) {
       s16x8 fa[4], fb[2][2];
@@ -562,17 +568,24 @@ __global__ __launch_bounds__(512, 2) void ns_solo_kernel(const NsArgs a, const i
 #pragma unroll
         for (int i = 0; i < 2; ++i) fb[h][i] = decltype(slow)::value ? rs.get(pb, i, h) : rb.get(pb, i, h);
       };
-      auto go = [&](int h) {
+      auto go = [&](int h, f32x4 (*sum)[2]) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[j][i] = gt::Fp16::mfma(fb[h][i], fa[j], acc[j][i]);
+          for (int j = 0; j < 4; ++j) sum[j][i] = gt::Fp16::mfma(fb[h][i], fa[j], sum[j][i]);
       };
       load_a(0); load_b(0); load_b(1);
-      go(0);
-      if (PROD == 3) go(1);
+      go(0, acc);
+      if (PROD == 3) go(1, FULL ? cross : acc);
       load_a(1);
-      go(PROD == 3 ? 0 : 1);
+      if (PROD == 3) go(0, FULL ? cross : acc); else go(1, acc);
+      if (FULL) go(1, cross);
+    }
+    if (FULL) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[j][i] += cross[j][i];
     }
   };
   const int off_c = L::contig(row0, col0), off_s = L::slow(row0, col0);
@@ -734,21 +747,21 @@ inline bool use_chains(double chained, double single) { return chained <= 0.8 * 
 inline double chained_work(double thin, double wide) { return 6 * thin * thin * wide + 14 * thin * thin * thin; }
 inline double single_work(double thin, double wide) { return 15 * thin * thin * wide + 5 * thin * thin * thin; }
 
-// Measured: 16 x 16 20 us, 64 x 147 49 us, 128 x 256 94 us (fp32 or bf16) against 100 to 170 us in 17 launches.  Four tiles (120 x 400 fp32) spill and run 257 us against 150: two at most.
+// Measured: 16 x 16 20 us, 64 x 147 49 us, 128 x 256 94 us (bf16; fp32 22, 52, 108) against 100 to 170 us in 17 launches.  Four tiles (120 x 400 fp32) spill and run 257 us against 150: two at most.
 constexpr int SOLO_TILES = 2;
 inline bool solo(int rows, int cols) { return min(rows, cols) <= 128 && max(rows, cols) <= SOLO_TILES * 128; }
 
-template <int PROD, int NT, bool MUON> int launch_solo_t(const NsArgs& a, int mats, int steps, const float* abc, hipStream_t st) {
+template <int PROD, int NT, bool MUON, bool FULL> int launch_solo_t(const NsArgs& a, int mats, int steps, const float* abc, hipStream_t st) {
   static SmemAttrOnce once;
-  auto* fn = &ns_solo_kernel<PROD, NT, MUON>;
+  auto* fn = &ns_solo_kernel<PROD, NT, MUON, FULL>;
   const int smem = Solo<PROD>::SMEM, rc = once.ensure(reinterpret_cast<const void*>(fn), smem);
   if (rc != 0) return rc;
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_solo_kernel<PROD, NT, MUON>), dim3(mats), dim3(512), smem, st, a, steps, abc[0], abc[1], abc[2]);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_solo_kernel<PROD, NT, MUON, FULL>), dim3(mats), dim3(512), smem, st, a, steps, abc[0], abc[1], abc[2]);
   return (int)hipGetLastError();
 }
 // wide: the widest matrix
-template <int PROD, bool MUON> int launch_solo(const NsArgs& a, int mats, int wide, int steps, const float* abc, hipStream_t st) {
-  return wide <= 128 ? launch_solo_t<PROD, 1, MUON>(a, mats, steps, abc, st) : launch_solo_t<PROD, 2, MUON>(a, mats, steps, abc, st);
+template <int PROD, bool MUON, bool FULL> int launch_solo(const NsArgs& a, int mats, int wide, int steps, const float* abc, hipStream_t st) {
+  return wide <= 128 ? launch_solo_t<PROD, 1, MUON, FULL>(a, mats, steps, abc, st) : launch_solo_t<PROD, 2, MUON, FULL>(a, mats, steps, abc, st);
 }
 
 // blocks of every launch;  maps likewise (null for a plain call: `per` blocks a matrix);  chains: only with PROD = 3
@@ -931,8 +944,9 @@ extern "C" int ddl_orthogonalize(const void* g, int is_bf16, void* out, void* ws
   if (solo(rows, cols)) {
     a.per = 1;
     const int wide = max(rows, cols);
-    return prod == 3 ? launch_solo<3, false>(a, batch, wide, steps, abc, (hipStream_t)stream)
-                     : launch_solo<1, false>(a, batch, wide, steps, abc, (hipStream_t)stream);
+    if (prod != 3) return -1;                             // ddl_ns_prod
+    return is_bf16 ? launch_solo<3, false, false>(a, batch, wide, steps, abc, (hipStream_t)stream)
+                   : launch_solo<3, false, true>(a, batch, wide, steps, abc, (hipStream_t)stream);
   }
   int blocks[LAUNCHES];
   for (int i = 0; i < LAUNCHES; ++i) {
@@ -961,8 +975,8 @@ extern "C" int ddl_muon_step(const void* table, const void* maps, const int* blo
   a.zero_grad = zero_grad;
   if (solo_wide > 0) {
     a.map = (const int2*)maps;
-    return prod == 3 ? launch_solo<3, true>(a, blocks[0], solo_wide, steps, abc, (hipStream_t)stream)
-                     : launch_solo<1, true>(a, blocks[0], solo_wide, steps, abc, (hipStream_t)stream);
+    return prod == 3 ? launch_solo<3, true, true>(a, blocks[0], solo_wide, steps, abc, (hipStream_t)stream)
+                     : launch_solo<1, true, false>(a, blocks[0], solo_wide, steps, abc, (hipStream_t)stream);
   }
   const int2* list[LAUNCHES];
   const int2* at = (const int2*)maps;
