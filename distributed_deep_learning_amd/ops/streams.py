@@ -75,9 +75,9 @@ def _stream(index: int) -> torch.cuda.Stream:
         # first one that really runs beside the current stream is kept.
         # Always NORMAL priority.  A high-priority stream gets a hardware queue of its own by construction, but a
         # fork/join between a high-priority and a normal-priority stream deadlocks on the GPU as soon as the process
-        # holds more streams than hardware queues (bench/probes/prio_stream_probe.py: {normal, high} x {0, 8 extra
-        # streams} - only high+8 hangs, within the first 500 iterations; MIOpen's RNN and gloo's GPU collectives put a
-        # process into that regime, which is how round 1 met it).  There is no switch to turn that back on.
+        # holds more streams than hardware queues (seen with {normal, high} x {0, 8 extra streams}: only high with 8 hung,
+        # within the first 500 iterations; MIOpen's RNN and gloo's GPU collectives put a process into that regime).
+        # There is no switch to turn that back on.
         main = torch.cuda.current_stream(index)
         cands = []
         for _ in range(5):
