@@ -16,6 +16,9 @@ Ordering rules, all enforced here:
 * join: the first fork inside a backward pass queues an autograd-engine callback that makes the main stream wait
   for the side stream when the pass ends, so ``loss.backward()`` keeps its usual meaning (gradients are ordered
   before anything later on the current stream); :func:`join` does the same on demand (optimizer step);
+* autograd's own additions: a weight whose gradient the side stream adds to may have other uses in the same pass (a
+  penalty, a layer that hands its gradient to autograd), which autograd sums and adds to the same memory;
+  :func:`order`, called by the arena's hook in front of that addition, puts it behind the side stream;
 * collectives: :func:`comm_context` lets the data-parallel reducer enqueue a bucket's all-reduce behind BOTH
   streams without stalling the main one.
 
@@ -167,6 +170,14 @@ def join() -> None:
         # memory may be reused by it
         _held.pop(index, None)
     _dirty.clear()
+
+
+def order(device: torch.device) -> None:
+    """Make ``device``'s current stream wait for what its side stream has been given so far.  Unlike :func:`join` the fork
+    stays open (operands held, the join at the end of the pass still to come): the caller's stream, here the one autograd
+    adds to a gradient on, need not be the one the pass was forked from."""
+    if device.index in _dirty:
+        torch.cuda.current_stream(device).wait_stream(_side[device.index])
 
 
 @contextlib.contextmanager

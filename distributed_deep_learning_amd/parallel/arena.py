@@ -126,6 +126,9 @@ class ParamArena:
                 p.grad = torch.as_strided(self.grad, p.shape, p.stride(), s.offset)
                 p._ddl_arena = self                                   # noqa: SLF001
                 p._ddl_segment = s.index                              # noqa: SLF001
+                if p.dim() >= 2 and not getattr(p, "_ddl_ordered", False):      # what side-stream kernels add gradients of
+                    p.register_hook(_order_autograd)
+                    p._ddl_ordered = True                             # noqa: SLF001
                 if self.shadow is not None:
                     p._ddl_shadow = torch.as_strided(self.shadow, p.shape, p.stride(), s.offset)  # noqa: SLF001
         self._shadow_versions = [-1] * len(self.params)
@@ -250,6 +253,14 @@ class ParamArena:
         mb = self.total * 4 / 2**20
         return (f"ParamArena({len(self.params)} tensors, {self.total} elems = {mb:.1f} MiB fp32, "
                 f"{len(self.buckets)} buckets: " + ", ".join(f"{(b.hi - b.lo) * 4 / 2**20:.1f}" for b in self.buckets) + " MiB)")
+
+
+def _order_autograd(g: Optional[torch.Tensor]) -> None:
+    """Hook of a weight in an arena: runs once a pass, behind all of the weight's uses, when autograd is about to add ``g`` (``None``:
+    every use added its part itself) to the gradient, which kernels on the side stream may still be adding to."""
+    if g is not None:
+        from ..ops import streams
+        streams.order(g.device)
 
 
 def _dense(p: torch.Tensor) -> bool:
