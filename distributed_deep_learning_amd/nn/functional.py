@@ -964,6 +964,12 @@ def _weight16(w: torch.Tensor) -> torch.Tensor:
     return w.detach()
 
 
+def _adds_to_arena(w: torch.Tensor) -> bool:
+    """Whether a weight's gradient can be added to its place in an arena by the kernel itself."""
+    arena = getattr(w, "_ddl_arena", None)
+    return arena is not None and arena.grad_is_arena_view(w) and w.grad.is_contiguous()
+
+
 def _gated_forward(x, w_gate, w_up, w_down, activation, train):
     shape, (F_, D) = x.shape, w_gate.shape
     M = x.numel() // D
@@ -974,7 +980,8 @@ def _gated_forward(x, w_gate, w_up, w_down, activation, train):
 
 class GatedMLP(torch.autograd.Function):
     """The gated feed-forward block on ``csrc/gated.hip``: two products forward, three backward.  Use :func:`gated_mlp`.  Gradients of fp32
-    weights that live in an arena are added straight into it (on the side stream, like every other weight gradient)."""
+    weights that live in an arena are added straight into it (on the side stream, like every other weight gradient), whatever the call's
+    other weights are; a weight in two places of one call is left to autograd (one launch would add to one place twice at once)."""
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation):
@@ -994,25 +1001,23 @@ class GatedMLP(torch.autograd.Function):
             dx = None if not need[0] else x.new_empty(shape) if x_dtype is BF16 else x.new_empty(shape, dtype=x_dtype)
             dgu = K.gated_dh(dy, wg, wu, wd, kept, M, D, F_, dx) if need[0] or need[1] or need[2] else None
             want = [w if n else None for w, n in zip(weights, need[1:4])]
-            live = [w for w in want if w is not None]
-            if not live:
-                return dx, None, None, None, None
-            arena = getattr(live[0], "_ddl_arena", None)
-            if (arena is not None and len({id(w) for w in live}) == len(live)      # a weight in two places: autograd adds its gradients
-                    and all(getattr(w, "_ddl_arena", None) is arena and arena.grad_is_arena_view(w) and w.grad.is_contiguous() for w in live)):
+            direct = [w if w is not None and _adds_to_arena(w) and sum(v is w for v in want) == 1 else None for w in want]
+            rest = [None if d is not None else w for w, d in zip(want, direct)]
+            out = [None, None, None]
+            if any(w is not None for w in direct):
                 with streams.fork(x, dy, kept, *([] if dgu is None else [dgu])):
-                    K.gated_dw(x, dy, kept, dgu, [None if w is None else w.grad for w in want], M, D, F_, accumulate=True)
-                for w in reversed(live):
-                    arena.notify_grad_ready(w)
-                return dx, None, None, None, None
-            if arena is not None:
-                streams.join()                                             # autograd will add to gradients the side stream may be adding to
-            dtype = BF16 if all(w.dtype is BF16 for w in live) else torch.float32
-            like = wg if dtype is BF16 else wg.new_empty(0, dtype=dtype)
-            out = [None if w is None else like.new_empty(w.shape) for w in want]
-            K.gated_dw(x, dy, kept, dgu, out, M, D, F_)
-            if dtype is not BF16:
-                out = [None if w is None else t.to(w.dtype) for w, t in zip(want, out)]
+                    K.gated_dw(x, dy, kept, dgu, [None if w is None else w.grad for w in direct], M, D, F_, accumulate=True)
+                for w in reversed(direct):
+                    if w is not None:
+                        w._ddl_arena.notify_grad_ready(w)                  # noqa: SLF001
+            live = [w for w in rest if w is not None]
+            if live:
+                dtype = BF16 if all(w.dtype is BF16 for w in live) else torch.float32
+                like = wg if dtype is BF16 else wg.new_empty(0, dtype=dtype)
+                out = [None if w is None else like.new_empty(w.shape) for w in rest]
+                K.gated_dw(x, dy, kept, dgu, out, M, D, F_)
+                if dtype is not BF16:
+                    out = [None if w is None else t.to(w.dtype) for w, t in zip(rest, out)]
         return dx, *out, None
 
 

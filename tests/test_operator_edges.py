@@ -79,3 +79,63 @@ def test_penalty_beside_a_direct_gradient_loses_nothing():
             # 100 + g rounds once per addition; Linear's parts meet in any order
             tol = 4 * 2 * H24 * (100 + plain[n].abs()) + (1e-5 * plain[n].abs().max() if n.startswith("1") else 0.0)
             assert float(((p.grad - 100.0 - plain[n]).abs() - tol).max()) <= 0.0, n
+
+
+def _spy_dw(monkeypatch):
+    """What the gated block's weight gradients are computed into: one list of three truth values a launch, and whether it adds."""
+    seen, real = [], K.gated_dw
+
+    def dw(x, dy, kept, dgu, out, M, D, F_, accumulate=False):
+        seen.append(([t is not None for t in out], accumulate))
+        return real(x, dy, kept, dgu, out, M, D, F_, accumulate)
+
+    monkeypatch.setattr(K, "gated_dw", dw)
+    return seen
+
+
+@gpu
+@pytest.mark.parametrize("twice_first", [True, False])
+def test_gated_mlp_arena_weight_alone_in_one_call_and_twice_in_another(monkeypatch, twice_first):
+    """One arena weight, once as gate beside another (added by the kernel) and once as gate and up (left to autograd), in one pass: nothing is
+    lost.  The parts are the same fp32 values everywhere; only up to four additions of them round."""
+    T, D, H = 2048, 256, 1032
+    x, dy = _randn(11, T, D).to(BF).cuda(), _randn(12, T, D, scale=0.1).to(BF).cuda()
+    w = [_randn(13, H, D, scale=D ** -0.5).to(BF), _randn(14, H, D, scale=D ** -0.5).to(BF), _randn(15, D, H, scale=H ** -0.5).to(BF)]
+    leaves = [t.float().cuda().requires_grad_() for t in w]
+    g0, u1, d2 = torch.autograd.grad(F.gated_mlp(x, *leaves), leaves, dy)
+    twin = [leaves[0], leaves[0].detach().clone().requires_grad_(), leaves[2]]
+    ga, gb, gd = torch.autograd.grad(F.gated_mlp(x, *twin), twin, dy)
+    net, arena = _arena(*w, device="cuda")
+    seen = _spy_dw(monkeypatch)
+    calls = [lambda: F.gated_mlp(x, net[0], net[0], net[2]), lambda: F.gated_mlp(x, net[0], net[1], net[2])]
+    for _ in range(3):
+        arena.zero_grad()
+        seen.clear()
+        ys = [f() for f in (calls if twice_first else calls[::-1])]
+        torch.autograd.backward(ys, [dy, dy])
+        assert sorted(seen) == sorted([([False, False, True], True), ([True, True, False], False), ([True, True, True], True)])
+        for p, terms in zip(net, ((g0, ga, gb), (u1,), (d2, gd))):
+            assert arena.grad_is_arena_view(p)
+            tol = 4 * H24 * sum(t.abs() for t in terms)
+            assert float(((p.grad - sum(terms)).abs() - tol).max()) <= 0.0
+
+
+@gpu
+def test_gated_mlp_gate_outside_the_arena_beside_weights_in_it(monkeypatch):
+    """A gate derived from something else (an adapter merged into it): the other weights' gradients still go straight to the arena."""
+    T, D, H = 300, 64, 264
+    x, dy = _randn(21, T, D).to(BF).cuda(), _randn(22, T, D, scale=0.1).to(BF).cuda()
+    w = [_randn(23, H, D, scale=D ** -0.5).to(BF), _randn(24, H, D, scale=D ** -0.5).to(BF), _randn(25, D, H, scale=H ** -0.5).to(BF)]
+    leaves = [t.float().cuda().requires_grad_() for t in w]
+    ref = torch.autograd.grad(F.gated_mlp(x, *leaves), leaves, dy)
+    net, arena = _arena(*w[1:], device="cuda")
+    base = w[0].float().cuda().requires_grad_()
+    seen = _spy_dw(monkeypatch)
+    for dtype in (torch.float32, BF):
+        arena.zero_grad()
+        seen.clear()
+        base.grad = None
+        F.gated_mlp(x, (base * 1.0).to(dtype), net[0], net[1]).backward(dy)
+        assert seen == [([False, True, True], True), ([True, False, False], False)]
+        assert torch.equal(net[0].grad, ref[1]) and torch.equal(net[1].grad, ref[2])
+        assert torch.equal(base.grad, ref[0].to(dtype).float())
