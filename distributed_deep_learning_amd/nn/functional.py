@@ -981,7 +981,9 @@ def _gated_forward(x, w_gate, w_up, w_down, activation, train):
 class GatedMLP(torch.autograd.Function):
     """The gated feed-forward block on ``csrc/gated.hip``: two products forward, three backward.  Use :func:`gated_mlp`.  Gradients of fp32
     weights that live in an arena are added straight into it (on the side stream, like every other weight gradient), whatever the call's
-    other weights are; a weight in two places of one call is left to autograd (one launch would add to one place twice at once)."""
+    other weights are; a weight in two places of one call is left to autograd (one launch would add to one place twice at once).  The
+    data-parallel reducer hears of them from autograd, behind the last use of the weight in the pass: a signal from here would release
+    the bucket of a weight that several blocks share behind the first."""
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation):
@@ -1007,9 +1009,6 @@ class GatedMLP(torch.autograd.Function):
             if any(w is not None for w in direct):
                 with streams.fork(x, dy, kept, *([] if dgu is None else [dgu])):
                     K.gated_dw(x, dy, kept, dgu, [None if w is None else w.grad for w in direct], M, D, F_, accumulate=True)
-                for w in reversed(direct):
-                    if w is not None:
-                        w._ddl_arena.notify_grad_ready(w)                  # noqa: SLF001
             live = [w for w in rest if w is not None]
             if live:
                 dtype = BF16 if all(w.dtype is BF16 for w in live) else torch.float32

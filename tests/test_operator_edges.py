@@ -139,3 +139,29 @@ def test_gated_mlp_gate_outside_the_arena_beside_weights_in_it(monkeypatch):
         assert seen == [([False, True, True], True), ([True, False, False], False)]
         assert torch.equal(net[0].grad, ref[1]) and torch.equal(net[1].grad, ref[2])
         assert torch.equal(base.grad, ref[0].to(dtype).float())
+
+
+@gpu
+def test_reducer_hears_of_a_shared_gated_weight_behind_its_last_use():
+    """Two blocks with the same weights: when the first signal of a tensor arrives (the one the reducer counts), its gradient is whole."""
+    T, D, H = 700, 128, 520
+    x, dy = _randn(31, T, D).to(BF).cuda(), _randn(32, T, D, scale=0.1).to(BF).cuda()
+    block = dnn.GatedMLP(D, H).cuda()
+    arena = ParamArena(block.named_parameters())
+    snaps = {}
+
+    def ready(seg):
+        if seg not in snaps:
+            s = arena.segments[seg]
+            with streams.comm_context(arena.grad):                                    # as a collective would be enqueued
+                snaps[seg] = arena.grad[s.offset:s.offset + s.numel].clone()
+
+    arena.on_grad_ready = ready
+    for p in arena.params:
+        p.register_post_accumulate_grad_hook(lambda p: ready(p._ddl_segment))
+    block(block(x)).backward(dy)
+    torch.cuda.synchronize()
+    assert sorted(snaps) == [0, 1, 2]
+    for seg, snap in snaps.items():
+        s = arena.segments[seg]
+        assert float(snap.abs().sum()) > 0.0 and torch.equal(snap, arena.grad[s.offset:s.offset + s.numel])
