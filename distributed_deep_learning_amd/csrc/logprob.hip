@@ -159,13 +159,14 @@ __device__ __forceinline__ Stat stat_wave(Stat a) {
   return a;
 }
 
+constexpr unsigned NAN_KEY = 0xfffffffeu;                               // one below the top: a candidate is always below ~0, where lists begin
 __device__ __forceinline__ unsigned key_of(float z) {                    // order-preserving; -0 and 0 equal, NaN on top; 0 = absent
   const unsigned b = __float_as_uint(z + 0.f);
-  if (z != z) return 0xffffffffu;
+  if (z != z) return NAN_KEY;
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(unsigned k) {
-  if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
+  if (k == NAN_KEY) return __uint_as_float(0x7fc00000u);
   return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
 __device__ __forceinline__ u64 cand(unsigned key, int j) { return ((u64)key << 32) | (u64)(0xffffffffu - (unsigned)j); }

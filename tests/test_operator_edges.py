@@ -165,3 +165,17 @@ def test_reducer_hears_of_a_shared_gated_weight_behind_its_last_use():
     for seg, snap in snaps.items():
         s = arena.segments[seg]
         assert float(snap.abs().sum()) > 0.0 and torch.equal(snap, arena.grad[s.offset:s.offset + s.numel])
+
+
+# ================================================================================================= token log probabilities
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+@pytest.mark.parametrize("N,V,top", [(520, 5003, 5), (1, 4099, 3), (2, 4096, 64), (1, 70_000, 64), (1, 900, 20)])
+def test_token_logprobs_list_of_rows_of_nothing_but_nan(N, V, top, dtype):
+    """More elements tie at the top than a list holds, the first of them at index 0: in one part, in several, and where the parts are joined."""
+    z = torch.full((N, V), float("nan"), dtype=dtype)
+    z[N // 2, 1:] = 2.0                                                              # and one NaN at index 0 above a long tie
+    tok = torch.zeros(N, dtype=torch.int64)
+    out, cpu = F.token_logprobs(z.cuda(), tok.cuda(), top), F.token_logprobs(z, tok, top)
+    for o in (out, cpu):
+        assert torch.isnan(o[2]).all() and torch.equal(o[3].cpu(), torch.arange(top).expand(N, top))
