@@ -12,6 +12,7 @@ from __future__ import annotations
 import os
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ..ops import kernels as K
@@ -926,6 +927,12 @@ def _token_logprobs_cpu(logits, tokens, top):
     return logp, torch.where(empty[:, 0], 0.0, ent), logq.gather(-1, idx), idx
 
 
+def _refuse_tangents(what: str, *tensors: torch.Tensor) -> None:
+    """Calls that need no backward pass go past their autograd function, which would refuse forward-mode derivatives; so do these."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):     # noqa: SLF001
+        raise NotImplementedError(f"{what}: no forward-mode derivative on the GPU")
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
     """``logits`` bf16 / fp32 ``[..., V]``, ``tokens`` int64 ``[...]`` -> ``(logp, entropy, top_logp, top_index)``: fp32 ``[...]``, ``[...]``,
     ``[..., top]`` and int64 ``[..., top]``.
@@ -934,7 +941,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
     padding), ``entropy`` that of the whole distribution in nats, ``top_logp`` / ``top_index`` the ``top`` (at most 64) most likely tokens,
     descending, equal logits by the lowest index.  All but the indices are differentiable.  Logits of ``-inf`` are masked tokens; a row of
     nothing else gives ``logp = top_logp = -inf``, entropy 0 and no gradient.  Logits that are not contiguous are copied: to leave positions
-    out, give them a token outside ``[0, V)`` rather than slicing the logits."""
+    out, give them a token outside ``[0, V)`` rather than slicing the logits.  Forward-mode derivatives: on the CPU only."""
     if tokens.shape != logits.shape[:-1]:
         raise ValueError(f"token_logprobs: tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")
     lead, V = logits.shape[:-1], logits.shape[-1]
@@ -943,6 +950,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
     flat = len(lead) == 1
     z, t = (logits, tokens) if flat else (logits.reshape(-1, V), tokens.reshape(-1))
     if logits.is_cuda:
+        _refuse_tangents("token_logprobs", logits)
         with device_of(logits):
             if z.requires_grad and torch.is_grad_enabled():
                 out = TokenLogProbs.apply(z, t, int(top))
@@ -1026,7 +1034,7 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 
     On the GPU the products run on bf16 operands (fp32 inputs and weights are rounded, in every call; fp32 weights of an arena use its shadow)
     with fp32 sums, the result is bf16; gradients come in the dtype of what they belong to.  Widths that are no multiples of 8 are copied to
-    padded operands in every call.  On the CPU: plain torch ops in the inputs' dtype."""
+    padded operands in every call.  On the CPU: plain torch ops in the inputs' dtype.  Forward-mode derivatives: on the CPU only."""
     if activation not in K.GATED_ACTIVATIONS:
         raise ValueError(f"gated_mlp: activation must be one of {sorted(K.GATED_ACTIVATIONS)}, got {activation!r}")
     D = x.shape[-1] if x.dim() else -1
@@ -1044,6 +1052,7 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
             raise ValueError("gated_mlp: inputs and weights must be on one device")
     if D == 0 or w_gate.shape[0] == 0:
         raise ValueError("gated_mlp: empty widths")
+    _refuse_tangents("gated_mlp", x, w_gate, w_up, w_down)
     with device_of(x):
         if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
             return GatedMLP.apply(x, w_gate, w_up, w_down, activation)

@@ -1350,7 +1350,8 @@ def orthogonalize(g: torch.Tensor, steps: int = NS_STEPS, coefficients=NS_COEFFI
     """The orthogonal factor of every matrix in ``g`` (``[m, n]`` or ``[batch, m, n]``, bf16 or fp32), approximately: ``steps``
     Newton-Schulz steps ``X <- a X + (b S + c S S) X``, ``S = X X^T``, from ``X = G / (|G|_F + eps)`` (``csrc/ortho.hip``).  The result has
     ``g``'s shape and dtype; fp32 matrices are multiplied to fp32's accuracy, so are bf16 ones of up to 128 rows or
-    columns; larger ones with 11-bit operands, which adds little to the rounding of the result."""
+    columns; larger ones with 11-bit operands, which adds little to the rounding of the result.  For optimizers: no derivative is defined,
+    the result is detached from ``g`` whether ``g`` requires a gradient or not."""
     import ctypes as C
     lib = _lib.require()
     if g.dim() not in (2, 3):

@@ -179,3 +179,35 @@ def test_token_logprobs_list_of_rows_of_nothing_but_nan(N, V, top, dtype):
     out, cpu = F.token_logprobs(z.cuda(), tok.cuda(), top), F.token_logprobs(z, tok, top)
     for o in (out, cpu):
         assert torch.isnan(o[2]).all() and torch.equal(o[3].cpu(), torch.arange(top).expand(N, top))
+
+
+# ================================================================================================= derivatives
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_forward_mode_derivatives_are_right_or_refused(device):
+    """Never a result without its tangent."""
+    import torch.autograd.forward_ad as fw
+    z, t = _randn(41, 4, 30).to(device), _randn(42, 4, 30).to(device)
+    tok = torch.tensor([1, 2, 3, 29]).to(device)
+    x, dx, w, wd = (_randn(43 + i, *s).to(device) for i, s in enumerate(((4, 16), (4, 16), (24, 16), (16, 24))))
+    calls = [lambda f: F.token_logprobs(f(z, t), tok, 2)[0], lambda f: F.gated_mlp(f(x, dx), w, w, wd), lambda f: F.gated_mlp(x, w, f(w, 0.5 * w), wd)]
+    for grad in (True, False):
+        for call in calls:
+            with torch.set_grad_enabled(grad), fw.dual_level():
+                if device == "cuda":
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        call(fw.make_dual)
+                else:
+                    assert fw.unpack_dual(call(fw.make_dual)).tangent is not None
+                assert call(lambda p, _: p) is not None                              # inside a level, without a tangent
+    logq = torch.log_softmax(z.cpu().double(), 1)
+    ref = (t.cpu().double() - (logq.exp() * t.cpu()).sum(1, keepdim=True)).gather(1, tok.cpu()[:, None])[:, 0]
+    if device == "cpu":
+        with fw.dual_level():
+            assert torch.allclose(fw.unpack_dual(calls[0](fw.make_dual)).tangent.double(), ref, atol=1e-5)
+
+
+@gpu
+def test_orthogonalize_is_detached_from_a_weight_that_requires_a_gradient():
+    w = _randn(51, 40, 70).cuda().requires_grad_()
+    out = K.orthogonalize(w)
+    assert not out.requires_grad and torch.equal(out, K.orthogonalize(w.detach()))
