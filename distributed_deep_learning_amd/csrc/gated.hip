@@ -579,7 +579,7 @@ template <int BT, int NST, auto KERNEL> int launch(long long blocks, const Gated
 // Large tiles may take whole rounds of the chip and leave the rest to small ones, whose reductions can be shared: 6000 x 4096 x 11008 forward and
 // backward 4.79 -> 4.30 ms;  3000 x 2048 x 5632 0.85 -> 0.74.
 struct Cut { int first, splits, per; long long tiles; };                    // large tiles;  then small ones
-Cut cut_of(int count, int rows, int cols, int ks, bool few = false) {
+Cut cut_of(int count, int rows, int cols, int ks, bool small_only = false) {
   const long long big = count * tiles(rows, 256) * tiles(cols, 256), rounds = big / gt::CUS, rest = big - rounds * gt::CUS;
   const double round = 1.75 * (ks + 7.5);
   Cut c{0, 1, ks, count * tiles(rows, 128) * tiles(cols, 128)};
@@ -590,7 +590,7 @@ Cut cut_of(int count, int rows, int cols, int ks, bool few = false) {
     const double steps = (double)full + (left == 0 ? 0.0 : left <= gt::CUS ? 0.6 : 1.0), drift = (double)c.tiles / gt::SLOTS + 0.25;
     small = (steps < drift ? steps : drift) * (ks + 6);
   }
-  if (!few && big < (1 << 28)) {
+  if (!small_only && big < (1 << 28)) {
     const int per = rest > 0 ? gt::chunk_for(4 * rest, ks, &ends) : ks;
     const double whole = round * (double)(rounds + (rest > 0)), mixed = round * (double)rounds + ends + 8;      // 8: a launch more
     if (whole < small && whole <= mixed) c = Cut{(int)big, 1, ks, 0};
@@ -636,11 +636,18 @@ template <bool LO> struct Dw {
 };
 
 int stages(int k) { return (int)tiles(k, 64); }
-Cut cut_up(int M, int D, int F) { return cut_of(1, M, 2 * F, stages(D)); }
-Cut cut_down(int M, int D, int F) { return cut_of(1, M, D, stages(F)); }
-Cut cut_dh(int M, int D, int F, bool lo) { return cut_of(1, M, F, stages(D), lo); }
-Cut cut_dx(int M, int D, int F, bool lo) { return cut_of(1, M, D, (lo ? 4 : 2) * stages(F), lo); }
-Cut cut_dw(int M, int D, int F, bool lo) { return cut_of(3, F, D, (lo ? 2 : 1) * stages(M), lo); }
+inline int pad8(int n) { return (n + 7) & ~7; }
+
+// A lane addresses its rows of a tile with 32-bit byte offsets: up to 2^24 elements a row in 128-row tiles (127 * 2^25 bytes), 2^23 in 256-row ones.
+constexpr int WIDEST = 1 << 24, WIDEST_LARGE = 1 << 23;
+bool sizes_ok(int M, int D, int F) { return M > 0 && D > 0 && F > 0 && M <= 0x7fffff00 && D <= WIDEST && F <= WIDEST; }
+bool long_rows(int D, int F) { return pad8(D) > WIDEST_LARGE || pad8(F) > WIDEST_LARGE; }
+
+Cut cut_up(int M, int D, int F) { return cut_of(1, M, 2 * F, stages(D), long_rows(D, F)); }
+Cut cut_down(int M, int D, int F) { return cut_of(1, M, D, stages(F), long_rows(D, F)); }
+Cut cut_dh(int M, int D, int F, bool lo) { return cut_of(1, M, F, stages(D), lo || long_rows(D, F)); }
+Cut cut_dx(int M, int D, int F, bool lo) { return cut_of(1, M, D, (lo ? 4 : 2) * stages(F), lo || long_rows(D, F)); }
+Cut cut_dw(int M, int D, int F, bool lo) { return cut_of(3, F, D, (lo ? 2 : 1) * stages(M), lo || long_rows(D, F)); }
 
 constexpr int FEW = 64;                            // tokens up to which gated_few_kernel is used
 
@@ -669,16 +676,12 @@ bool few(int M, int K) { return M <= FEW && (long long)FEW * K * 2 < 0x7fffffffl
 // h, dg and du as pairs: offsets between the planes in 32 bits too
 bool pairs(int M, int Dp, int Fp) { return few(M, Dp) && (long long)FEW * Fp * 10 < 0x7fffffffll; }
 
-bool sizes_ok(int M, int D, int F) { return M > 0 && D > 0 && F > 0 && D < (1 << 30) && F < (1 << 30); }
-
 template <int ACT> int up(const GatedArgs& a, void* st) {
   const bool save = a.keep16 != nullptr;
   if (few(a.M, a.Dp)) return few_up<ACT>(a, save, st);
   const Cut c = cut_up(a.M, a.D, a.F);
   return save ? product<Up<ACT, true>>(c, a, st) : product<Up<ACT, false>>(c, a, st);
 }
-
-inline int pad8(int n) { return (n + 7) & ~7; }
 
 }  // namespace
 

@@ -981,6 +981,7 @@ def _adds_to_arena(w: torch.Tensor) -> bool:
 def _gated_forward(x, w_gate, w_up, w_down, activation, train):
     shape, (F_, D) = x.shape, w_gate.shape
     M = x.numel() // D
+    K.check_gated_sizes(M, D, F_)
     ops = K.gated_operands((x.detach().reshape(M, D), M, D), (_weight16(w_gate), F_, D), (_weight16(w_up), F_, D), (_weight16(w_down), D, F_))
     y, kept = K.gated_fwd(*ops, M, D, F_, activation, save=train)
     return y if len(shape) == 2 else y.view(shape), (*ops, kept), (M, D, F_)

@@ -1241,6 +1241,13 @@ def token_logprobs_bwd(logits, tokens, norm, entropy, g_logp=None, g_entropy=Non
 
 # ----------------------------------------------------------------------------------------------- gated feed-forward block
 GATED_ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}        # mirrors csrc/gated.hip
+GATED_MAX_TOKENS, GATED_MAX_WIDTH = 0x7fffff00, 1 << 24
+
+
+def check_gated_sizes(M: int, D: int, F_: int) -> None:
+    """Refuses what the kernels' 32-bit counts and offsets do not hold."""
+    if M > GATED_MAX_TOKENS or D > GATED_MAX_WIDTH or F_ > GATED_MAX_WIDTH:
+        raise ValueError(f"gated_mlp: {M} tokens, widths {D} and {F_}: at most {GATED_MAX_TOKENS} tokens and widths of {GATED_MAX_WIDTH}")
 
 
 def gated_operands(*mats):

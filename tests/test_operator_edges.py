@@ -211,3 +211,49 @@ def test_orthogonalize_is_detached_from_a_weight_that_requires_a_gradient():
     w = _randn(51, 40, 70).cuda().requires_grad_()
     out = K.orthogonalize(w)
     assert not out.requires_grad and torch.equal(out, K.orthogonalize(w.detach()))
+
+
+# ================================================================================================= sizes
+def test_gated_mlp_sizes_past_32_bit_offsets_are_refused():
+    """128 rows of more than 2^24 16-bit elements span 4 GiB: a lane's offset would wrap and read another row."""
+    most = 1 << 24
+    K.check_gated_sizes(K.GATED_MAX_TOKENS, most, most)
+    for sizes in ((1, most + 1, 8), (1, 8, most + 1), (K.GATED_MAX_TOKENS + 1, 8, 8), (2 ** 32 + 5, 8, 8), (8, 2 ** 32 + 8, 8)):
+        with pytest.raises(ValueError):
+            K.check_gated_sizes(*sizes)
+    if K._lib.available():
+        work = K._lib.require().ddl_gated_workspace
+        assert work(200, 256, most, 0) > 0
+        for sizes in ((200, most + 1, 256), (200, 256, most + 1), (-1, 8, 8), (0x7fffff01, 8, 8)):
+            assert all(work(*sizes, p) == -1 for p in (0, 1, 2))
+
+
+@gpu
+def test_gated_mlp_refuses_long_rows_before_it_reads_them():
+    one = torch.zeros(1, dtype=BF, device="cuda")
+    for T, D, H in ((1, (1 << 24) + 8, 8), (1, 8, (1 << 24) + 8), (2 ** 32 + 5, 8, 8)):
+        with pytest.raises(ValueError, match="at most"):
+            F.gated_mlp(one.expand(T, D), one.expand(H, D), one.expand(H, D), one.expand(D, H))
+
+
+@gpu
+@pytest.mark.parametrize("T", [3, 130])
+def test_gated_mlp_of_the_widest_rows(T):
+    """Rows of 2^24 elements: the last rows and columns count.  All operands are powers of two with few bits, so every product and sum is exact
+    up to the rounding of h and of the results."""
+    D, H = 1 << 24, 136
+    x = torch.zeros(T, D, dtype=BF, device="cuda")
+    wg, wu = torch.zeros(2, H, D, dtype=BF, device="cuda")
+    wd = torch.zeros(D, H, dtype=BF, device="cuda")
+    k = torch.tensor([0, 1, D // 2 + 3, D - 2, D - 1], device="cuda")
+    r = lambda i, *s: (torch.randint(1, 5, s, generator=torch.Generator().manual_seed(i)).float() / 4).to(BF).cuda()      # noqa: E731
+    x[:, k], wg[:, k], wu[:, k], wd[k] = r(1, T, 5), r(2, H, 5), r(3, H, 5), r(4, 5, H)
+    with torch.no_grad():
+        y = F.gated_mlp(x, wg, wu, wd, activation="relu")
+    g, u = (x[:, k].double() @ w[:, k].double().T for w in (wg, wu))
+    h = g.relu() * u
+    ref = h @ wd[k].double().T
+    tol = (B8 * (h @ wd[k].double().T.abs()) + B8 * ref.abs()) * 1.01
+    assert float(((y[:, k].double() - ref).abs() - tol).max()) <= 0.0
+    y[:, k] = 0
+    assert float(y.abs().max()) == 0.0
