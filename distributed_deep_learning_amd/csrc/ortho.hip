@@ -764,6 +764,15 @@ template <int PROD, bool MUON, bool FULL> int launch_solo(const NsArgs& a, int m
   return wide <= 128 ? launch_solo_t<PROD, 1, MUON, FULL>(a, mats, steps, abc, st) : launch_solo_t<PROD, 2, MUON, FULL>(a, mats, steps, abc, st);
 }
 
+// What 32-bit counts and a lane's 32-bit byte offsets inside a tile hold: 128 K-contiguous rows of X, or a stage of its rows.  (Only the columns of wide
+// matrices are long rows; 256-row tiles of X have rows as long as the thin side.)
+template <int PROD> bool addressable(int rows, int cols) {
+  const long long bytes = 2 * Lay<PROD>(rows, cols).ldx, most = 0xFFFFFFE0ll;
+  return rows > 0 && cols > 0 && rows <= 0x7fffff00 && cols <= 0x7fffff00 && (min(rows, 128) - 1) * bytes + 128 <= most &&
+         min(rows, PROD == 3 ? 32 : 64) * bytes <= most;
+}
+bool addressable(int rows, int cols, int prod) { return prod == 3 ? addressable<3>(rows, cols) : prod == 1 && addressable<1>(rows, cols); }
+
 // blocks of every launch;  maps likewise (null for a plain call: `per` blocks a matrix);  chains: only with PROD = 3
 template <int PROD, bool MUON>
 int run_steps(NsArgs a, const int* blocks, const int2* const* maps, const int* per, int steps, const float* abc, bool chains, hipStream_t st) {
@@ -878,9 +887,9 @@ template <class KS> int set_chunk(const int* thin, int n, KS&& ks) {
 
 }  // namespace
 
-// fp16 elements of workspace for one matrix
+// fp16 elements of workspace for one matrix (-1: it is too large, here and in the other calls)
 extern "C" long long ddl_ns_workspace(int rows, int cols, int prod) {
-  if (rows <= 0 || cols <= 0 || (prod != 1 && prod != 3)) return -1;
+  if (!addressable(rows, cols, prod)) return -1;
   return prod == 3 ? Lay<3>(rows, cols).size : Lay<1>(rows, cols).size;
 }
 
@@ -904,7 +913,7 @@ extern "C" int ddl_ns_chunks(const int* thin, const int* wide, int n, int prod, 
 // For one of `batch` equal matrices (gram_chunk 0), or one of a set of matrices with the chunks of ddl_ns_chunks (batch 1): out[0..1] the splits
 // of the gram and of the square product, out[2..9] blocks of every launch; returns the floats of partial tiles it needs.
 extern "C" long long ddl_ns_shape(int rows, int cols, int prod, int batch, int gram_chunk, int square_chunk, int* out) {
-  if (rows <= 0 || cols <= 0 || batch <= 0 || gram_chunk < 0 || square_chunk < 0 || (gram_chunk == 0) != (square_chunk == 0) || (prod != 1 && prod != 3)) return -1;
+  if (!addressable(rows, cols, prod) || batch <= 0 || gram_chunk < 0 || square_chunk < 0 || (gram_chunk == 0) != (square_chunk == 0)) return -1;
   const Shape h = gram_chunk == 0 ? shape_of_batch(rows, cols, prod, batch) : shape_of(rows, cols, prod, 1, gram_chunk, square_chunk);
   out[0] = h.gram_splits;
   out[1] = h.square_splits;
@@ -928,7 +937,7 @@ extern "C" int ddl_ns_mat_bytes() { return (int)sizeof(NsMat); }
 // ddl_ns_shape(.., batch, 0, 0, ..) returns, floats;  abc on the host
 extern "C" int ddl_orthogonalize(const void* g, int is_bf16, void* out, void* ws, double* parts, float* slabs, int batch, int rows, int cols,
                                  int prod, int steps, const float* abc, float eps, void* stream) {
-  if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || (prod != 1 && prod != 3)) return -1;
+  if (batch <= 0 || !addressable(rows, cols, prod) || steps <= 0) return -1;
   const Shape h = shape_of_batch(rows, cols, prod, batch);
   NsArgs a{};
   a.one.rows = rows; a.one.cols = cols;

@@ -1353,6 +1353,19 @@ def _newton_schulz_range(steps: int, a: float, b: float, c: float) -> tuple:
     return a, b, c
 
 
+def orthogonalize_plan(batch: int, rows: int, cols: int, dtype: torch.dtype) -> tuple:
+    """``(products, workspace)`` of a call: 1 or 3 fp16 products for one, fp16 elements for each matrix (0: one block does it in registers and LDS).
+    Refuses what the kernels' 32-bit counts and offsets do not hold: 2^31 matrices or rows, rows of more than 2^23 elements (of 2^24 in bf16
+    matrices with more than 128 rows and columns, just below 2^30 where there is one row)."""
+    lib = _lib.require()
+    if max(batch, rows, cols) <= 0x7fffff00:
+        prod = lib.ddl_ns_prod(rows, cols, int(dtype == BF16))
+        ws = 0 if lib.ddl_ns_solo(rows, cols) else lib.ddl_ns_workspace(rows, cols, prod)
+        if ws >= 0:
+            return prod, ws
+    raise ValueError(f"orthogonalize: {batch} matrices of {rows} x {cols} are too large")
+
+
 def orthogonalize(g: torch.Tensor, steps: int = NS_STEPS, coefficients=NS_COEFFICIENTS, eps: float = NS_EPS) -> torch.Tensor:
     """The orthogonal factor of every matrix in ``g`` (``[m, n]`` or ``[batch, m, n]``, bf16 or fp32), approximately: ``steps``
     Newton-Schulz steps ``X <- a X + (b S + c S S) X``, ``S = X X^T``, from ``X = G / (|G|_F + eps)`` (``csrc/ortho.hip``).  The result has
@@ -1369,16 +1382,16 @@ def orthogonalize(g: torch.Tensor, steps: int = NS_STEPS, coefficients=NS_COEFFI
     a, b, c = check_newton_schulz(steps, coefficients)
     if g.numel() == 0:
         return torch.empty_like(g)
-    g = _aligned(g)
     batch = g.shape[0] if g.dim() == 3 else 1
     rows, cols = g.shape[-2:]
+    prod, size = orthogonalize_plan(batch, rows, cols, g.dtype)
+    g = _aligned(g)
     is16 = g.dtype == BF16
-    prod = lib.ddl_ns_prod(rows, cols, int(is16))
     out = torch.empty_like(g)
     ws = parts = slabs = None
-    if not lib.ddl_ns_solo(rows, cols):
+    if size:
         slabs = _scratch(g, 4 * batch * lib.ddl_ns_shape(rows, cols, prod, batch, 0, 0, (C.c_int * 10)()))
-        ws = _scratch(g, 2 * batch * lib.ddl_ns_workspace(rows, cols, prod))
+        ws = _scratch(g, 2 * batch * size)
         parts = _scratch(g, 8 * batch * lib.ddl_ns_max_parts())
     check(lib.ddl_orthogonalize(ptr(g), int(is16), ptr(out), ptr(ws), ptr(parts), ptr(slabs), batch, rows, cols, prod, int(steps),
                                 (C.c_float * 3)(a, b, c), float(eps), stream_ptr()), "orthogonalize")

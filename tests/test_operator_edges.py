@@ -257,3 +257,35 @@ def test_gated_mlp_of_the_widest_rows(T):
     assert float(((y[:, k].double() - ref).abs() - tol).max()) <= 0.0
     y[:, k] = 0
     assert float(y.abs().max()) == 0.0
+
+
+def test_orthogonalize_sizes_past_32_bit_offsets_are_refused():
+    """128 split rows of more than 2^23 elements span 4 GiB of hi and lo values: a lane's offset would wrap and read another row."""
+    if not K._lib.available():
+        pytest.skip("kernel library not built")
+    plan, f32 = K.orthogonalize_plan, torch.float32
+    for ok in ((1, 128, 1 << 23, f32), (1, 1 << 26, 128, f32), (1, 2, 1 << 25, f32), (1, 1, (1 << 30) - 64, BF), (1, 200, 1 << 24, BF), (1 << 30, 4, 4, f32)):
+        assert plan(*ok)[1] >= 0
+    for bad in ((1, 128, (1 << 23) + (1 << 17), f32), (1, 64, 1 << 25, f32), (1, 200, (1 << 24) + (1 << 18), BF), (1, 2 ** 32 + 5, 4, f32), (1, 4, 2 ** 32 + 5, BF),
+                (2 ** 32 + 3, 4, 4, f32), (1, 1, 1 << 30, f32)):
+        with pytest.raises(ValueError, match="too large"):
+            plan(*bad)
+    if torch.cuda.is_available():
+        with pytest.raises(ValueError, match="too large"):
+            K.orthogonalize(torch.zeros(1, device="cuda").expand(128, 1 << 24))
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(3, 1 << 22), (1 << 22, 3)])
+def test_orthogonalize_of_long_rows(shape):
+    """Rows far longer than a tile, against 64 bits: as in the small cases, with sums of 2^22 products, sqrt(2^22) 2^-24 each, in one product of three."""
+    g = torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda")
+    x = g.double() / (g.double().norm() + 1e-7)
+    x = x.t() if shape[0] > shape[1] else x
+    a, b, c = K.NS_COEFFICIENTS
+    for _ in range(5):
+        s = x.contiguous() @ x.t().contiguous()
+        x = a * x + (b * s + c * s @ s) @ x
+    ref = x.t() if shape[0] > shape[1] else x
+    tol = 30 * 2.0 ** -22 + 5 * 2048 * H24
+    assert float((K.orthogonalize(g).double() - ref).norm()) <= tol * float(ref.norm())
