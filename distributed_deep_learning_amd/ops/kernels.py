@@ -1169,7 +1169,7 @@ def softmax_xent(logits, target, want_grad=True):
 
 
 # ----------------------------------------------------------------------------------------------- token log probabilities
-LOGPROB_MAX_TOP = 64                     # mirrors csrc/logprob.hip
+LOGPROB_MAX_TOP, LOGPROB_MAX_VOCAB = 64, 0x7fffff00      # mirrors csrc/logprob.hip
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -1203,8 +1203,8 @@ def token_logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     N, V = logits.shape
     if not 0 <= top <= min(V, LOGPROB_MAX_TOP):
         raise ValueError(f"token_logprobs: top must be between 0 and min(V, {LOGPROB_MAX_TOP}), got {top} with V = {V}")
-    if V < 1:
-        raise ValueError("token_logprobs: the vocabulary is empty")
+    if not 1 <= V <= LOGPROB_MAX_VOCAB:
+        raise ValueError(f"token_logprobs: the vocabulary must have between 1 and {LOGPROB_MAX_VOCAB} tokens, got {V}")
     logits, tokens = logits.contiguous(), tokens.contiguous()
     dev = logits.device
     logp = torch.empty(N, dtype=torch.float32, device=dev)

@@ -289,3 +289,11 @@ def test_orthogonalize_of_long_rows(shape):
     ref = x.t() if shape[0] > shape[1] else x
     tol = 30 * 2.0 ** -22 + 5 * 2048 * H24
     assert float((K.orthogonalize(g).double() - ref).norm()) <= tol * float(ref.norm())
+
+
+@gpu
+def test_token_logprobs_refuses_vocabularies_past_31_bits():
+    one = torch.zeros(1, dtype=BF, device="cuda")
+    for V in (2 ** 31, 2 ** 32 + 5):
+        with pytest.raises(ValueError, match="vocabulary"):
+            F.token_logprobs(one.expand(1, V), torch.zeros(1, dtype=torch.int64, device="cuda"))
