@@ -503,6 +503,9 @@ int plan(long long rows, int V, int most) {
 // Rows begin at any alignment: a row has V / 8 pieces at most (fewer behind an unaligned start).
 int parts_of(int V, int per) { const int pieces = V / 8; return pieces == 0 ? 1 : (pieces + per - 1) / per; }
 
+// Rows of one launch, which has less than 2^32 threads: more rows take several.
+long long rows_of_launch(long long parts) { const long long n = 0xffffffffll / NT / parts; return n > 0 ? n : 1; }
+
 // Most pieces a thread keeps in registers: 64 registers of logits, of the 128 that four waves per SIMD have.
 template <typename T> struct MaxPieces { static constexpr int value = sizeof(T) == 2 ? 16 : 8; };
 
@@ -515,17 +518,25 @@ void launch(dim3 grid, hipStream_t st, const T* z, const long long* tokens, int 
 
 template <typename T, bool STREAM>
 int forward(const T* z, const long long* tokens, long long rows, int V, int k, int per, int parts, void* ws, const Outs& o, hipStream_t st) {
-  Stat* const ps = (Stat*)ws;
-  u64* const pt = (u64*)((char*)ws + ((size_t)rows * parts * sizeof(Stat) + 15) / 16 * 16);
-  const dim3 grid((unsigned)(rows * parts));
+  Stat* ps = (Stat*)ws;
+  u64* pt = (u64*)((char*)ws + ((size_t)rows * parts * sizeof(Stat) + 15) / 16 * 16);
   int groups = 1;
   while (groups < k) groups *= 2;
-  if (per <= NT) launch<T, 1, STREAM>(grid, st, z, tokens, V, parts, per, k, groups, ps, pt, o);
-  else if (per <= 4 * NT) launch<T, 4, STREAM>(grid, st, z, tokens, V, parts, per, k, groups, ps, pt, o);
-  else launch<T, MaxPieces<T>::value, STREAM>(grid, st, z, tokens, V, parts, per, k, groups, ps, pt, o);
-  if (parts > 1)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_join_kernel<T>), dim3((unsigned)rows), dim3(NT), 0, st, z, tokens, V, parts, k, groups, ps, pt, o);
-  return (int)hipGetLastError();
+  const long long most = rows_of_launch(parts);
+  int rc = 0;
+  for (long long r = 0; r < rows && rc == 0; r += most) {
+    const long long n = min(most, rows - r);
+    const dim3 grid((unsigned)(n * parts));
+    const Outs p{o.logp + r, o.ent + r, o.norm == nullptr ? nullptr : o.norm + 2 * r, o.top + r * k, o.idx + r * k};
+    if (per <= NT) launch<T, 1, STREAM>(grid, st, z, tokens, V, parts, per, k, groups, ps, pt, p);
+    else if (per <= 4 * NT) launch<T, 4, STREAM>(grid, st, z, tokens, V, parts, per, k, groups, ps, pt, p);
+    else launch<T, MaxPieces<T>::value, STREAM>(grid, st, z, tokens, V, parts, per, k, groups, ps, pt, p);
+    if (parts > 1)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_join_kernel<T>), dim3((unsigned)n), dim3(NT), 0, st, z, tokens, V, parts, k, groups, ps, pt, p);
+    rc = (int)hipGetLastError();
+    z += n * V; tokens += n; ps += n * parts; pt += n * parts * k;
+  }
+  return rc;
 }
 
 int parts_for(long long rows, int V, int is_bf16, int k, int* per) {
@@ -555,7 +566,6 @@ extern "C" int ddl_logprob_fwd(const void* z, int is_bf16, const long long* toke
   if (rows <= 0 || V <= 0 || V > 0x7fffff00 || k < 0 || k > TOP_MAX || k > V) return -1;
   int per;
   const int parts = parts_for(rows, V, is_bf16, k, &per);
-  if (rows * parts > 0x7fffffffll) return -2;
   const Outs o{logp, ent, norm, top, idx};
   hipStream_t st = (hipStream_t)stream;
   if (!train && beyond_cache(rows, V, is_bf16))
@@ -570,14 +580,19 @@ extern "C" int ddl_logprob_bwd(const void* z, int is_bf16, const long long* toke
                                const float* gent, const float* gtop, const long long* idx, long long rows, int V, int k, void* dz, void* stream) {
   if (rows <= 0 || V <= 0 || V > 0x7fffff00 || k < 0 || k > TOP_MAX || (gtop != nullptr && idx == nullptr)) return -1;
   const int per = plan(rows, V, 0x7fffff00), parts = parts_of(V, per);
-  if (rows * parts > 0x7fffffffll) return -2;
-  const dim3 grid((unsigned)(rows * parts));
   hipStream_t st = (hipStream_t)stream;
+  const long long most = rows_of_launch(parts);
+  int rc = 0;
   auto run = [&](auto* kernel, auto* in, auto* out) {
-    hipLaunchKernelGGL(kernel, grid, dim3(NT), 0, st, in, tokens, norm, ent, glogp, gent, gtop, idx, k, out, V, parts, per);
+    auto at = [](auto* p, long long i) { return p == nullptr ? p : p + i; };
+    for (long long r = (rows - 1) / most * most; r >= 0 && rc == 0; r -= most) {           // the last rows first (beyond_cache)
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(min(most, rows - r) * parts)), dim3(NT), 0, st, in + r * V, tokens + r, norm + 2 * r, ent + r,
+                         at(glogp, r), at(gent, r), at(gtop, r * k), at(idx, r * k), k, out + r * V, V, parts, per);
+      rc = (int)hipGetLastError();
+    }
   };
   const bool large = beyond_cache(rows, V, is_bf16);
   if (is_bf16) run(large ? &logprob_bwd_kernel<bf16_t, true> : &logprob_bwd_kernel<bf16_t, false>, (const bf16_t*)z, (bf16_t*)dz);
   else run(large ? &logprob_bwd_kernel<float, true> : &logprob_bwd_kernel<float, false>, (const float*)z, (float*)dz);
-  return (int)hipGetLastError();
+  return rc;
 }

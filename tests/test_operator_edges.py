@@ -297,3 +297,23 @@ def test_token_logprobs_refuses_vocabularies_past_31_bits():
     for V in (2 ** 31, 2 ** 32 + 5):
         with pytest.raises(ValueError, match="vocabulary"):
             F.token_logprobs(one.expand(1, V), torch.zeros(1, dtype=torch.int64, device="cuda"))
+
+
+@gpu
+def test_token_logprobs_of_more_rows_than_a_launch_has_blocks():
+    """2^24 rows and some: forward, list and gradient of rows on both sides of the cut equal those of the rows alone."""
+    N, V = (1 << 24) + 1000, 8
+    z = torch.randn(N, V, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda", dtype=BF).requires_grad_()
+    tok = torch.arange(N, device="cuda") % (V + 1)                                   # every ninth row is padding
+    pick = torch.cat([torch.arange(300), torch.arange((1 << 24) - 300, (1 << 24) + 300), torch.arange(N - 300, N)]).cuda()
+    out = F.token_logprobs(z, tok, 3)
+    heads = [out[0].sum(), out[1].sum(), out[2].square().sum()]
+    (dz,) = torch.autograd.grad(sum(heads), z)
+    few = z.detach()[pick].requires_grad_()
+    ref = F.token_logprobs(few, tok[pick], 3)
+    (dr,) = torch.autograd.grad(ref[0].sum() + ref[1].sum() + ref[2].square().sum(), few)
+    assert all(torch.equal(o[pick], r) for o, r in zip(out, ref)) and torch.equal(dz[pick], dr)
+    for i in range(0, N, 1 << 22):                                                   # gradients of a softmax add up to zero in every row, but for their rounding
+        d = dz[i:i + (1 << 22)].float()
+        size = d.abs().sum(1)
+        assert float((d.sum(1).abs() - 1.01 * B8 * size).max()) <= 1e-3 and float(size.min()) > 0.0
