@@ -31,6 +31,7 @@
 #include "host_util.h"
 #include "gemm_tile.h"
 #include <math.h>
+#include <algorithm>
 
 namespace {
 
@@ -950,21 +951,29 @@ extern "C" int ddl_orthogonalize(const void* g, int is_bf16, void* out, void* ws
   a.parts = parts;
   a.eps = eps;
   if (is_bf16) { a.g16 = (const bf16_t*)g; a.out16 = (bf16_t*)out; } else { a.g32 = (const float*)g; a.out32 = (float*)out; }
-  if (solo(rows, cols)) {
-    a.per = 1;
-    const int wide = max(rows, cols);
-    if (prod != 3) return -1;                             // ddl_ns_prod
-    return is_bf16 ? launch_solo<3, false, false>(a, batch, wide, steps, abc, (hipStream_t)stream)
-                   : launch_solo<3, false, true>(a, batch, wide, steps, abc, (hipStream_t)stream);
-  }
-  int blocks[LAUNCHES];
-  for (int i = 0; i < LAUNCHES; ++i) {
-    if ((long long)h.blocks[i] * batch > 0x7fffffffll) return -2;
-    blocks[i] = h.blocks[i] * batch;
-  }
+  if (solo(rows, cols) && prod != 3) return -1;           // ddl_ns_prod
   const double thin = min(rows, cols), wide = max(rows, cols);
-  return prod == 3 ? run_steps<3, false>(a, blocks, nullptr, h.blocks, steps, abc, use_chains(chained_work(thin, wide), single_work(thin, wide)), (hipStream_t)stream)
-                   : run_steps<1, false>(a, blocks, nullptr, h.blocks, steps, abc, false, (hipStream_t)stream);
+  const bool one = solo(rows, cols), chains = prod == 3 && use_chains(chained_work(thin, wide), single_work(thin, wide));
+  // a launch has less than 2^32 threads: more matrices take several (of all kinds)
+  const long long most = 0xffffffffll / 512 / (one ? 1 : *std::max_element(h.blocks, h.blocks + LAUNCHES));
+  if (most < 1) return -2;
+  int rc = 0;
+  for (long long b = 0; b < batch && rc == 0; b += most) {
+    const int n = (int)min(most, batch - b);
+    a.per = 1;
+    if (one) {
+      rc = is_bf16 ? launch_solo<3, false, false>(a, n, max(rows, cols), steps, abc, (hipStream_t)stream)
+                   : launch_solo<3, false, true>(a, n, max(rows, cols), steps, abc, (hipStream_t)stream);
+    } else {
+      int blocks[LAUNCHES];
+      for (int i = 0; i < LAUNCHES; ++i) blocks[i] = h.blocks[i] * n;
+      rc = prod == 3 ? run_steps<3, false>(a, blocks, nullptr, h.blocks, steps, abc, chains, (hipStream_t)stream)
+                     : run_steps<1, false>(a, blocks, nullptr, h.blocks, steps, abc, false, (hipStream_t)stream);
+      a.ws += n * a.ws_stride; a.slabs += n * a.slab_stride; a.parts += (long long)n * MAX_PARTS;
+    }
+    if (is_bf16) { a.g16 += n * a.g_stride; a.out16 += n * a.g_stride; } else { a.g32 += n * a.g_stride; a.out32 += n * a.g_stride; }
+  }
+  return rc;
 }
 
 // Muon over the matrices of an arena.  table: NsMat[], maps: one int2[] after the other for the 8 launches, on the device;  blocks[8] on the host.

@@ -317,3 +317,15 @@ def test_token_logprobs_of_more_rows_than_a_launch_has_blocks():
         d = dz[i:i + (1 << 22)].float()
         size = d.abs().sum(1)
         assert float((d.sum(1).abs() - 1.01 * B8 * size).max()) <= 1e-3 and float(size.min()) > 0.0
+
+
+@gpu
+@pytest.mark.parametrize("batch,rows,cols,cut", [((1 << 23) + 77, 2, 3, 1 << 23), ((1 << 22) + 5, 1, 257, (1 << 23) // 3)])
+def test_orthogonalize_of_more_matrices_than_a_launch_has_blocks(batch, rows, cols, cut):
+    """Matrices on both sides of the cut equal those of a small call (in one block a matrix, and in the shared launches, three blocks a matrix)."""
+    g = torch.randn(batch, rows, cols, generator=torch.Generator(device="cuda").manual_seed(7), device="cuda", dtype=BF)
+    out = K.orthogonalize(g)
+    for at in (0, cut - 40, batch - 50):
+        assert torch.equal(out[at:at + 50], K.orthogonalize(g[at:at + 50].clone()))
+    for i in range(0, batch, 1 << 21):
+        assert bool((out[i:i + (1 << 21)].float().abs().amax((1, 2)) > 0.04).all())
