@@ -93,7 +93,6 @@ struct Stager {
   int k, kdone;                                    // reduction steps left to stage: k - kdone
   int kchunk;                                      // CONTIG: first reduction step of this lane's chunk
 
-  // `second`: CONTIG only, pieces with (j & pair_bit) != 0 belong to another matrix of the same shape (gate / up pairs)
   __device__ __forceinline__ void init(const Operand& o, int wid, int lane) {
     base = o.base; ld = o.ld; k = o.k; kdone = 0;
     if (MODE == CONTIG) {

@@ -329,3 +329,21 @@ def test_orthogonalize_of_more_matrices_than_a_launch_has_blocks(batch, rows, co
         assert torch.equal(out[at:at + 50], K.orthogonalize(g[at:at + 50].clone()))
     for i in range(0, batch, 1 << 21):
         assert bool((out[i:i + (1 << 21)].float().abs().amax((1, 2)) > 0.04).all())
+
+
+@gpu
+@pytest.mark.parametrize("steps,coef", [(2, (2.0, -0.5, 0.1)), (3, (1.33, 0.0, 0.0)), (5, (1.5, -0.5, 0.0)), (2, (1.0, 0.25, 0.0))])
+def test_orthogonalize_chains_of_polynomials_that_let_singular_values_grow(steps, coef):
+    """Steps on the small side, whose factors are multiplied in fp16 at a scale: singular values that start at one and end above two are in range.
+    A step's operands are rounded to 2^-22 relative; its factor is below 2.5 and what one step leaves grows by the next ones' slopes, 2.5 at most
+    over the whole chain, so 30 2^-22 and the sums as in the other cases, four times."""
+    K.check_newton_schulz(steps, coef)
+    g = (_randn(61, 1024, 1) @ _randn(62, 1, 4096) + 0.05 * _randn(63, 1024, 4096)).cuda()
+    a, b, c = coef
+    x = g.double() / (g.double().norm() + 1e-7)
+    for _ in range(steps):
+        s = x @ x.t().contiguous()
+        x = a * x + (b * s + c * s @ s) @ x
+    out = K.orthogonalize(g, steps=steps, coefficients=coef).double()
+    assert torch.isfinite(out).all()
+    assert float((out - x).norm()) <= 4 * (30 * 2.0 ** -22 + 15 * 71 * H24) * float(x.norm())
