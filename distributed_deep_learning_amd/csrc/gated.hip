@@ -685,9 +685,9 @@ template <int ACT> int up(const GatedArgs& a, void* st) {
 
 }  // namespace
 
-// Floats of partial tiles that a forward (0) or backward pass (1: dh and dx, 2: weight gradients, 3: both) needs
+// Floats of partial tiles that a forward (0) or backward pass (1: dh and dx, 2: weight gradients) needs
 extern "C" long long ddl_gated_workspace(int M, int D, int F, int pass) {
-  if (!sizes_ok(M, D, F) || pass < 0 || pass > 3) return -1;
+  if (!sizes_ok(M, D, F) || pass < 0 || pass > 2) return -1;
   long long n = 0;
   auto most = [&](const Cut& c) { n = max(n, slab_floats(c)); };
   if (pass == 0) {
@@ -695,8 +695,8 @@ extern "C" long long ddl_gated_workspace(int M, int D, int F, int pass) {
     if (!few(M, pad8(F))) most(cut_down(M, D, F));
   }
   const bool lo = pairs(M, pad8(D), pad8(F));
-  if (pass & 1) { most(cut_dh(M, D, F, lo)); most(cut_dx(M, D, F, lo)); }
-  if (pass & 2) most(cut_dw(M, D, F, lo));
+  if (pass == 1) { most(cut_dh(M, D, F, lo)); most(cut_dx(M, D, F, lo)); }
+  if (pass == 2) most(cut_dw(M, D, F, lo));
   return n;
 }
 
@@ -737,12 +737,12 @@ extern "C" int ddl_gated_fwd(const void* x, const void* wg, const void* wu, cons
   return few(M, a.Fp) ? launch_few<false, SILU, false>(a, stream) : product<Down>(cut_down(M, D, F), a, stream);
 }
 
-// pass: 1 dg and du (and dx, unless null), 2 weight gradients (those that are not null; they take dg and du), 3 both.  dy [M][Dp], dgu: dg, du and,
+// pass: 1 dg and du (and dx, unless null), 2 weight gradients (those that are not null; they take dg and du).  dy [M][Dp], dgu: dg, du and,
 // up to 64 tokens, what their rounding left, [M][Fp] each, dx [M][D] bf16 or (dx32) fp32, dwg and dwu [F][D], dwd [D][F]: dw 0 bf16, 1 fp32 that are added to, 2 fp32
 extern "C" int ddl_gated_bwd(const void* x, const void* dy, const void* wg, const void* wu, const void* wd, const void* h, const void* hlo,
                              const void* keep16, const void* keep8, void* dgu, void* dx, int dx32, void* dwg, void* dwu, void* dwd, int dw, float* slabs,
                              int M, int D, int F, int pass, void* stream) {
-  if (!sizes_ok(M, D, F) || pass < 1 || pass > 3 || dw < 0 || dw > 2) return -1;
+  if (!sizes_ok(M, D, F) || pass < 1 || pass > 2 || dw < 0 || dw > 2) return -1;
   GatedArgs a{};
   a.x = (const unsigned short*)x; a.dy = (const unsigned short*)dy;
   a.wg = (const unsigned short*)wg; a.wu = (const unsigned short*)wu; a.wd = (const unsigned short*)wd;
@@ -756,13 +756,8 @@ extern "C" int ddl_gated_bwd(const void* x, const void* dy, const void* wg, cons
   if (dgu != nullptr) { a.du = a.dg + plane; a.dglo = a.du + plane; a.dulo = a.dglo + plane; }
   a.hlo = (unsigned short*)hlo;
   const bool lo = pairs(M, a.Dp, a.Fp);
-  int rc = 0;
-  if (pass & 1) {
-    rc = lo ? product<Dh<true>>(cut_dh(M, D, F, lo), a, stream) : product<Dh<false>>(cut_dh(M, D, F, lo), a, stream);
-    if (rc == 0 && dx != nullptr)
-      rc = lo ? product<Dx<true>>(cut_dx(M, D, F, lo), a, stream) : product<Dx<false>>(cut_dx(M, D, F, lo), a, stream);
-  }
-  if (rc == 0 && (pass & 2))
-    rc = lo ? product<Dw<true>>(cut_dw(M, D, F, lo), a, stream) : product<Dw<false>>(cut_dw(M, D, F, lo), a, stream);
-  return rc;
+  if (pass == 2) return lo ? product<Dw<true>>(cut_dw(M, D, F, lo), a, stream) : product<Dw<false>>(cut_dw(M, D, F, lo), a, stream);
+  const int rc = lo ? product<Dh<true>>(cut_dh(M, D, F, lo), a, stream) : product<Dh<false>>(cut_dh(M, D, F, lo), a, stream);
+  if (rc != 0 || dx == nullptr) return rc;
+  return lo ? product<Dx<true>>(cut_dx(M, D, F, lo), a, stream) : product<Dx<false>>(cut_dx(M, D, F, lo), a, stream);
 }

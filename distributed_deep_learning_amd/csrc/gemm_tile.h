@@ -86,7 +86,6 @@ enum { CONTIG = 0, SLOW = 1 };
 template <int ROWS, int MODE, int PROD>
 struct Stager {
   static constexpr int NP = ROWS / 32;             // 1 KiB pieces per wave and stage
-  static constexpr int BYTES = ROWS * 128;
   unsigned voff[NP];
   const unsigned short* base;
   long long ld;

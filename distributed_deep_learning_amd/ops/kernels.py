@@ -1276,7 +1276,7 @@ def gated_operands(*mats):
 
 def gated_fwd(x, w_gate, w_up, w_down, M: int, D: int, F_: int, activation: str = "silu", save: bool = False):
     """``y = (act(x w_gate^T) * (x w_up^T)) w_down^T`` of :func:`gated_operands` (``csrc/gated.hip``).  Returns ``(y, kept)``: ``y`` bf16
-    ``[M, D]``; with ``save`` (training) ``kept`` is the buffer that :func:`gated_bwd` takes, for every token and (padded) feature
+    ``[M, D]``; with ``save`` (training) ``kept`` is the buffer that :func:`gated_dh` and :func:`gated_dw` take, for every token and (padded) feature
     ``h`` in bf16, the factors ``u act'(g)`` and ``act(g)`` in 24 bits and, up to 64 tokens, what the rounding of ``h`` left, else ``None``."""
     lib = _lib.require()
     _lib.check_device(x, "gated_fwd")
