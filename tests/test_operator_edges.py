@@ -347,3 +347,63 @@ def test_orthogonalize_chains_of_polynomials_that_let_singular_values_grow(steps
     out = K.orthogonalize(g, steps=steps, coefficients=coef).double()
     assert torch.isfinite(out).all()
     assert float((out - x).norm()) <= 4 * (30 * 2.0 ** -22 + 15 * 71 * H24) * float(x.norm())
+
+
+# ================================================================================================= errors that only a rounding of the result may leave
+# Rounding v in [2^e, 2^(e+1)) to bf16 is off by at most 2^(e-8), evenly spread: sqrt(1/3) 2^(e-8) <= 2^-8 |v| / sqrt(3) in the mean square, so the
+# norm of n roundings is below 2^-8 / sqrt(3) = 0.00226 of the result's norm, up to about 1 / sqrt(n) of that by chance (three times that is allowed).
+def _rounding_alone(out, ref, what, extra):
+    ref = ref.to(out.device)
+    tol = B8 / math.sqrt(3) * (1 + 3 / math.sqrt(ref.numel())) + extra
+    err = float((out.double() - ref).norm() / ref.norm())
+    assert err <= tol, (what, err, tol)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(64, 147), (20, 200), (200, 100), (128, 512), (100, 2000)])
+def test_orthogonalize_of_small_bf16_matrices_rounds_its_result_only(shape):
+    """Up to 128 rows or columns the products take 22-bit operands: 30 2^-22 and the sums of up to 2000 products, 15 sqrt(2000) 2^-24."""
+    g = (_randn(sum(shape), *shape) * 1e-3).to(BF).cuda()
+    a, b, c = K.NS_COEFFICIENTS
+    x = g.double() / (g.double().norm() + 1e-7)
+    for _ in range(5):
+        s = x @ x.t().contiguous()
+        x = a * x + (b * s + c * s @ s) @ x
+    _rounding_alone(K.orthogonalize(g), x, "orthogonalize", 30 * 2.0 ** -22 + 15 * 45 * H24)
+
+
+@gpu
+@pytest.mark.parametrize("T,D,H", [(64, 512, 1032), (16, 1024, 520), (5, 2048, 512)])
+def test_gated_mlp_of_few_tokens_rounds_results_only_in_the_mean(T, D, H):
+    """h, dg and du as pairs (2^-16 of them is left), factors in 24 bits (2^-17), act' to 1e-5: 1e-4 covers them and the sums."""
+    x, dy = _randn(71, T, D).to(BF).cuda(), _randn(72, T, D, scale=0.1).to(BF).cuda()
+    w = [_randn(73, H, D, scale=D ** -0.5).to(BF).cuda(), _randn(74, H, D, scale=D ** -0.5).to(BF).cuda(), _randn(75, D, H, scale=H ** -0.5).to(BF).cuda()]
+    leaves = [t.requires_grad_() for t in (x, *w)]
+    y = F.gated_mlp(*leaves)
+    got = (y.detach(), *torch.autograd.grad(y, leaves, dy))
+    exact = [t.detach().double().requires_grad_() for t in leaves]
+    silu = lambda v: v * torch.sigmoid(v)                                            # noqa: E731
+    ye = (silu(exact[0] @ exact[1].t()) * (exact[0] @ exact[2].t())) @ exact[3].t()
+    want = (ye.detach(), *torch.autograd.grad(ye, exact, dy.double()))
+    for what, o, r in zip(("y", "dx", "dwg", "dwu", "dwd"), got, want):
+        if what != "y" or T <= 32:
+            _rounding_alone(o, r, what, 1e-4)
+
+
+@gpu
+@pytest.mark.parametrize("T,D,H", [(1, 1, 1), (3, 1, 5), (70, 2, 1), (65, 1, 9), (129, 7, 3), (64, 15, 17)])
+def test_gated_mlp_of_tiny_widths_and_expanded_gradients(T, D, H):
+    """The smallest widths, from strided operands, with the gradient of a sum (one element, expanded) arriving at the block."""
+    x = _randn(81, T, 2 * D + 1)[:, 1:2 * D:2].to(BF)
+    w = [_randn(82, H, D).to(BF), _randn(83, D, H).to(BF).t(), _randn(84, D, H).to(BF)]
+    net, arena = _arena(*w, device="cuda")
+    xs = torch.zeros(T, 2 * D + 1, dtype=BF, device="cuda")
+    xs[:, 1:2 * D:2] = x.cuda()
+    xs = xs[:, 1:2 * D:2].detach().requires_grad_()
+    F.gated_mlp(xs, *net).sum().backward()
+    exact = [t.detach().double().clone().requires_grad_() for t in (x, *w)]
+    (torch.nn.functional.silu(exact[0] @ exact[1].t()) * (exact[0] @ exact[2].t()) @ exact[3].t()).sum().backward()
+    size = [float(t.grad.abs().max()) for t in exact]
+    for p, e, s in zip((xs, *net), exact, size):
+        # at most three roundings to bf16 (h or dg and du, the result) of terms whose sum of magnitudes is within T + H + D times the largest gradient
+        assert float((p.grad.cpu().double() - e.grad).abs().max()) <= 3 * B8 * (T + H + D) * s
