@@ -233,9 +233,9 @@ template <int BT, int NST, bool JOIN> struct Block {
     tile.template store<false, NJ>(smem, wid, lane, load, f, [](int, int, float*) {}, JOIN ? part : 0);
   }
 };
-// Measured at 8192 tokens, 4096 x 12288 (256 x 256 tiles; the chip's power is what bounds them: the matrix units are busy 53 % of the cycles at
-// 2.0 GHz, and schedules with 10 to 16 % fewer cycles ran at 1.8 GHz, no faster): up 1.39 ms (1.18 PFLOP/s), down 0.66 (1.25), dh 0.85 (0.97),
-// dx 1.38 (1.19), dw 2.06 (1.20); the same products from a library 1.24 to 0.93, without the epilogues.
+// Measured at 8192 tokens, 4096 x 12288 (256 x 256 tiles): up 1.37 ms (1.20 PFLOP/s), down 0.65 (1.26), dh 0.82 (1.00), dx 1.38 (1.20), dw 2.08 (1.19).
+// The clock is at 2.0 to 2.15 GHz and the matrix units are busy 53, 55, 43, 52 and 52 % of its cycles; schedules with 10 to 16 % fewer cycles ran at
+// 1.8 GHz, no faster.  A library's plain products of these sizes reach 1.55, 1.59, 1.30, 1.39 and 1.14 PFLOP/s, without the epilogues.
 // Measured at 517 tokens, 2048 x 5632 (128 x 128 tiles): up 37 us (440 blocks; 0.65 PFLOP/s), down 22 us in 240 parts and 4.5 us to join them,
 // 53 us in 80 whole tiles.
 #define GATED_BOUNDS __launch_bounds__(256, BT == 256 || NST > 2 ? 1 : 2)
