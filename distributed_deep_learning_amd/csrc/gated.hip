@@ -161,10 +161,15 @@ struct GatedArgs {
 };
 
 __device__ __forceinline__ void store8(unsigned short* p, const float* v) { *reinterpret_cast<u32x4*>(p) = pack8(v); }
+// what rounding to bf16 leaves of v; nothing of what is or becomes infinite (inf - inf would make it NaN)
+__device__ __forceinline__ float lower(float v) {
+  const float h = bf16_to_f32(f32_to_bf16(v));
+  return __builtin_isinf(h) ? 0.f : v - h;
+}
 __device__ __forceinline__ void lower8(unsigned short* p, const float* v) {     // what store8 leaves
   float l[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) l[e] = v[e] - bf16_to_f32(f32_to_bf16(v[e]));
+  for (int e = 0; e < 8; ++e) l[e] = lower(v[e]);
   store8(p, l);
 }
 // results have rows of their own length n: columns c .. c + 7 of row r
@@ -544,7 +549,7 @@ __global__ __launch_bounds__(64 * WAVES) void gated_few_kernel(const GatedArgs a
     if (LO && PAIR) {
       float l[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) l[e] = y[e] - bf16_to_f32(f32_to_bf16(y[e]));
+      for (int e = 0; e < 4; ++e) l[e] = lower(y[e]);
       *reinterpret_cast<u32x2*>(a.hlo + o) = u32x2{pack_bf16x2(l[0], l[1]), pack_bf16x2(l[2], l[3])};
     }
     if (PAIR || (N & 3) == 0) {

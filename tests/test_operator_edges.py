@@ -407,3 +407,27 @@ def test_gated_mlp_of_tiny_widths_and_expanded_gradients(T, D, H):
     for p, e, s in zip((xs, *net), exact, size):
         # at most three roundings to bf16 (h or dg and du, the result) of terms whose sum of magnitudes is within T + H + D times the largest gradient
         assert float((p.grad.cpu().double() - e.grad).abs().max()) <= 3 * B8 * (T + H + D) * s
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 9, 32, 50, 64, 65])
+def test_gated_mlp_infinite_hidden_values_stay_infinite(T):
+    """One hidden value overflows: results are infinities of the right sign whatever the number of tokens, not NaN (the pair of bf16 values that few
+    tokens keep must not hold inf - inf)."""
+    D, H = 8, 16
+    x = torch.ones(T, D, dtype=BF, device="cuda")
+    wg, wu = torch.zeros(2, H, D, dtype=BF, device="cuda")
+    wg[3], wu[3] = 1e30, 1e30
+    sign = torch.tensor([1.0, -1.0] * (D // 2), device="cuda")
+    wd = torch.zeros(D, H, dtype=BF, device="cuda")
+    wd[:, 3] = sign
+    leaves = [t.requires_grad_() for t in (x, wg, wu, wd)]
+    y = F.gated_mlp(*leaves)
+    assert torch.equal(y, (sign * float("inf")).to(BF).expand(T, D))
+    with torch.no_grad():
+        assert torch.equal(F.gated_mlp(*leaves), y)
+    dy = torch.zeros(T, D, dtype=BF, device="cuda")
+    dy[:, 0] = 1e10                                                                  # dg = du = 1e10 * 8e30: infinite
+    dx, dwg, dwu, _ = torch.autograd.grad(y, leaves, dy)
+    assert bool((dx == float("inf")).all()) and bool((dwg[3] == float("inf")).all()) and bool((dwu[3] == float("inf")).all())
+    assert float(dwg[:3].abs().max()) == 0.0
