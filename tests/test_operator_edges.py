@@ -431,3 +431,130 @@ def test_gated_mlp_infinite_hidden_values_stay_infinite(T):
     dx, dwg, dwu, _ = torch.autograd.grad(y, leaves, dy)
     assert bool((dx == float("inf")).all()) and bool((dwg[3] == float("inf")).all()) and bool((dwu[3] == float("inf")).all())
     assert float(dwg[:3].abs().max()) == 0.0
+
+
+@gpu
+def test_token_logprobs_of_sliced_logits_strided_tokens_and_no_rows_with_gradients():
+    base = _randn(91, 6, 520).cuda().requires_grad_()
+    pairs = torch.randint(0, 500, (6, 2), generator=torch.Generator().manual_seed(92)).cuda()
+    g = _randn(93, 6).cuda()
+    out = F.token_logprobs(base[:, 3:503], pairs[:, 1], 2)
+    (dz,) = torch.autograd.grad([out[0], out[2].sum(1)], base, [g, g])
+    z = base.detach()[:, 3:503].clone().requires_grad_()
+    ref = F.token_logprobs(z, pairs[:, 1].clone(), 2)
+    (dr,) = torch.autograd.grad([ref[0], ref[2].sum(1)], z, [g, g])
+    assert all(torch.equal(a, b) for a, b in zip(out, ref)) and torch.equal(dz[:, 3:503], dr) and float(dz[:, :3].abs().sum() + dz[:, 503:].abs().sum()) == 0.0
+    turned = _randn(94, 500, 6).cuda().t().requires_grad_()                           # stored column by column
+    (dt,) = torch.autograd.grad(F.token_logprobs(turned, pairs[:, 0])[0], turned, g)
+    straight = turned.detach().contiguous().requires_grad_()
+    assert torch.equal(dt, torch.autograd.grad(F.token_logprobs(straight, pairs[:, 0])[0], straight, g)[0])
+    none = torch.zeros(0, 9, device="cuda", requires_grad=True)
+    out = F.token_logprobs(none, torch.zeros(0, dtype=torch.int64, device="cuda"), 2)
+    assert torch.autograd.grad([out[0].sum() + out[1].sum() + out[2].sum()], none)[0].shape == (0, 9)
+
+
+@gpu
+def test_captured_forward_and_backward_of_block_and_loss_replay():
+    """One graph: block, token loss with a list, gradients of everything; replays with eager work between them equal eager runs to the bit."""
+    T, D, H, V = 96, 64, 136, 1000
+    x = _randn(95, T, D).to(BF).cuda()
+    head = _randn(96, V, D, scale=D ** -0.5).to(BF).cuda()
+    tok = torch.randint(0, V, (T,), generator=torch.Generator().manual_seed(97)).cuda()
+    w = [_randn(98, H, D, scale=D ** -0.5).to(BF).cuda(), _randn(99, H, D, scale=D ** -0.5).to(BF).cuda(), _randn(100, D, H, scale=H ** -0.5).to(BF).cuda()]
+    g = torch.full((T,), -1.0 / T, device="cuda")
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (x, *w)]
+        y = F.gated_mlp(*leaves)
+        logits = (y.detach().float() @ head.float().t()).requires_grad_()
+        out = F.token_logprobs(logits, tok, 3)
+        (dz,) = torch.autograd.grad([out[0], out[1], out[2]], logits, [g, 0.01 * g, g[:, None].expand(T, 3)])
+        return [*out, dz, *torch.autograd.grad(y, leaves, (dz @ head.float()).to(BF))]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for k in range(4):
+        x.copy_(_randn(200 + k, T, D).to(BF))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), k
+
+
+# ================================================================================================= data parallel
+def _muon_worker(rank, world):
+    from distributed_deep_learning_amd.optim import Muon
+    from distributed_deep_learning_amd.parallel import DistributedDataParallel
+    torch.manual_seed(11 + rank)                                                     # the broadcast makes them equal
+    block = dnn.GatedMLP(12, 40)
+    ddp = DistributedDataParallel(block, bucket_mb=1e-3)
+    opt = Muon(ddp.arena, lr=0.05, weight_decay=0.01)
+    start = ddp.arena.master.clone()
+    for s in range(3):
+        ddp(_randn(10 * s + rank, 6, 12)).pow(2).mean().backward()
+        ddp.step(opt)
+    return {"start": start, "end": ddp.arena.master.clone(), "buckets": len(ddp.arena.buckets)}
+
+
+def test_muon_in_data_parallel_equals_one_process_on_the_mean_gradient():
+    from _dist_util import run_ranks
+    from distributed_deep_learning_amd.optim import Muon
+    a, b = run_ranks(_muon_worker, 2)
+    assert a["buckets"] > 1 and torch.equal(a["end"], b["end"]) and torch.equal(a["start"], b["start"])
+    torch.manual_seed(11)
+    block = dnn.GatedMLP(12, 40)
+    arena = ParamArena(block.named_parameters(), bucket_bytes=int(1e-3 * 2 ** 20))         # laid out as the reducer lays it out
+    opt = Muon(arena, lr=0.05, weight_decay=0.01)
+    for s in range(3):
+        sum(block(_randn(10 * s + r, 6, 12)).pow(2).mean() for r in range(2)).backward()
+        arena.grad.mul_(0.5)
+        opt.step()
+    for p, s in zip(arena.params, arena.segments):
+        # three steps of lr times an orthogonal factor in fp32 (1e-5 of it), from the same start
+        assert float((p.detach().reshape(-1) - a["end"][s.offset:s.offset + s.numel]).abs().max()) <= 1e-4
+
+
+@gpu
+def test_shared_gated_weights_under_the_reducer_are_whole_when_their_bucket_goes():
+    """Two blocks with the same weights, beside a Linear, with the collectives of one rank: what a bucket holds when its collective is enqueued
+    is what it holds at the end of the pass, and every bucket goes inside the pass."""
+    import os
+    import torch.distributed as td
+    from distributed_deep_learning_amd.optim import Muon
+    from distributed_deep_learning_amd.parallel import DistributedDataParallel
+    from distributed_deep_learning_amd.utils import GradLedger
+    dev = torch.device("cuda:0")
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT="29653", HSA_ENABLE_IPC_MODE_LEGACY="0")
+    td.init_process_group("nccl", rank=0, world_size=1, device_id=dev)
+    try:
+        torch.manual_seed(12)
+
+        class Net(tnn.Module):
+            def __init__(self):
+                super().__init__()
+                self.inp, self.ff, self.out = dnn.Linear(64, 128), dnn.GatedMLP(128, 520), dnn.Linear(128, 64)
+
+            def forward(self, x):
+                h = self.inp(x)
+                h = h + self.ff(h)
+                return self.out(h + self.ff(h))
+
+        net = Net().to(dev)
+        d = DistributedDataParallel(net, bucket_mb=0.1, force_collectives=True)
+        assert len(d.arena.buckets) > 2
+        ledger = GradLedger(d, snapshot=True)
+        opt = Muon(d.arena, lr=0.01)
+        x = _randn(13, 512, 64).to(dev)
+        for _ in range(3):
+            d(x).float().pow(2).mean().backward()
+            assert d._next_bucket == -1
+            d.step(opt)
+        assert ledger.verified == 3 * len(d.arena.buckets) and not ledger.violations
+    finally:
+        td.destroy_process_group()
