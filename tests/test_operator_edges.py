@@ -558,3 +558,40 @@ def test_shared_gated_weights_under_the_reducer_are_whole_when_their_bucket_goes
         assert ledger.verified == 3 * len(d.arena.buckets) and not ledger.violations
     finally:
         td.destroy_process_group()
+
+
+@gpu
+def test_captured_data_parallel_step_with_a_gated_block_follows_the_eager_one():
+    """Block, Linear and Muon with native collectives (one rank) in one graph: the buckets of the block's weights go from autograd's hooks there too."""
+    import os
+    import torch.distributed as td
+    from distributed_deep_learning_amd.optim import Muon
+    from distributed_deep_learning_amd.parallel import DistributedDataParallel
+    from distributed_deep_learning_amd.utils import GraphedTrainStep
+    dev = torch.device("cuda:0")
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT="29655", HSA_ENABLE_IPC_MODE_LEGACY="0")
+    td.init_process_group("nccl", rank=0, world_size=1, device_id=dev)
+    try:
+        x, y = _randn(14, 256, 64).to(dev), torch.randint(0, 40, (256,), generator=torch.Generator().manual_seed(15)).to(dev)
+
+        def make():
+            torch.manual_seed(16)
+            net = tnn.Sequential(dnn.Linear(64, 128), dnn.GatedMLP(128, 520), dnn.Linear(128, 40)).to(dev)
+            d = DistributedDataParallel(net, bucket_mb=0.1, force_collectives=True, comm="native")
+            opt = Muon(d.arena, lr=0.01)
+            d.attach(opt)
+            return net, d, opt, dnn.SoftmaxCrossEntropyLoss()
+
+        net, d, opt, crit = make()
+        for _ in range(6):
+            crit(d(x), y).backward()
+            d.step(opt)
+        net2, d2, opt2, crit2 = make()
+        step = GraphedTrainStep(net2, crit2, opt2, x, y, warmup=2, ddp=d2)
+        for _ in range(4):
+            step(x, y)
+        torch.cuda.synchronize()
+        a, b = d.arena.master, d2.arena.master
+        assert float((a - b).norm()) <= 1e-3 * float(a.norm())                       # sums of the Linear layers may differ in order
+    finally:
+        td.destroy_process_group()
